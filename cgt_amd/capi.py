@@ -10,6 +10,7 @@ from . import build as _build
 
 c_int = ctypes.c_int
 c_long = ctypes.c_long
+c_uint = ctypes.c_uint
 c_double = ctypes.c_double
 c_void_p = ctypes.c_void_p
 c_char_p = ctypes.c_char_p
@@ -89,6 +90,12 @@ PROTOTYPES = {
     "cgt_amd_elwise_binary": (c_int, [c_int, c_int, c_int, c_long, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]),
     "cgt_amd_repeat": (c_int, [c_void_p, c_int, c_int, ctypes.POINTER(c_long), ctypes.POINTER(c_int), c_void_p, c_void_p]),
     "cgt_amd_sum_f32": (c_int, [c_void_p, c_int, ctypes.POINTER(c_long), ctypes.POINTER(c_int), c_void_p, c_void_p]),
+    "cgt_amd_layer_norm_fwd_f32": (c_int, [c_void_p, c_long, c_long, c_void_p, c_void_p, c_double] + [c_void_p] * 4),
+    "cgt_amd_layer_norm_bwd_f32": (c_int, [c_void_p] * 5 + [c_long, c_long] + [c_void_p] * 4),
+    "cgt_amd_dropout_f32": (c_int, [c_void_p, c_void_p, c_long, c_double, c_void_p, c_uint, c_void_p, c_void_p]),
+    "cgt_amd_dropout_add_layer_norm_fwd_f32": (c_int, [c_void_p, c_void_p, c_long, c_long, c_double, c_void_p, c_uint,
+                                                       c_void_p, c_void_p, c_double] + [c_void_p] * 5),
+    "cgt_amd_dropout_add_layer_norm_bwd_f32": (c_int, [c_void_p] * 6 + [c_long, c_long, c_double, c_void_p, c_uint] + [c_void_p] * 5),
     "cgt_amd_fill_f32": (c_int, [c_void_p, ctypes.c_float, c_long, c_void_p]),
     "cgt_amd_transpose4_f32": (c_int, [c_void_p, ctypes.POINTER(c_long), ctypes.POINTER(c_int),
                                        c_void_p, c_void_p]),

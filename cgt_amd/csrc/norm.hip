@@ -1,0 +1,611 @@
+// Layer norm, dropout and the two in one pass (dropout + residual + layer norm), forward and
+// backward, for gfx950.  All are bound by HBM traffic: every array is read or written once.
+//
+//   mean = sum_c x / C, rstd = 1 / sqrt(sum_c (x - mean)^2 / C + eps)      per row of C columns
+//   xhat = (x - mean) * rstd, y = gamma * xhat + beta
+//   gx = rstd * (g - sum_c(g) / C - xhat * sum_c(g * xhat) / C), g = gy * gamma
+//   ggamma = sum_rows gy * xhat, gbeta = sum_rows gy
+//   dropout: y = x * keep / (share kept) (+ residual), keep from random.h
+//
+// A row is held in registers between its statistics and its result: one wavefront per row up to
+// 1024 columns, one workgroup of four up to 8192; beyond that a workgroup walks the row once per
+// statistic and once for the result (the later walks find it in cache).  The variance is the mean
+// of the squared distances from the mean, not a difference of two sums, so rows far from zero
+// keep their digits.  A lane owns the same columns in every row it meets: gamma and beta are
+// loaded once, and the weights' gradients are summed over a workgroup's rows in registers, left
+// as one partial row per workgroup, and added by a second kernel in a fixed order (no atomics:
+// same input, same bits).
+#include "random.h"
+#include <algorithm>
+
+namespace cgt_amd {
+
+struct __attribute__((packed, aligned(4))) float4a {      // 16 bytes at any 4-byte aligned address
+    float v[4];
+};
+
+constexpr int kNormThreads = 256;
+constexpr int kWideThreads = 1024;
+
+// Columns [c0, c0 + N) of a row, zero outside [0, cols).
+template <int N>
+__device__ __forceinline__ void load_cols(const float* __restrict__ row, int c0, int cols, float (&v)[N]) {
+    if (c0 + N <= cols) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4a q = *reinterpret_cast<const float4a*>(row + c0 + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i + k] = q.v[k];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = c0 + i < cols ? row[c0 + i] : 0.0f;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_cols(float* __restrict__ row, int c0, int cols, const float (&v)[N]) {
+    if (c0 + N <= cols) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            float4a q;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) q.v[k] = v[i + k];
+            *reinterpret_cast<float4a*>(row + c0 + i) = q;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (c0 + i < cols) row[c0 + i] = v[i];
+    }
+}
+
+// keep / (share kept) of eight consecutive elements that start at flat index e0.  They lie in one
+// group of the generator when e0 is a multiple of 8 and in two otherwise.
+__device__ __forceinline__ void keep_factors(const RngState& rng, const DropoutRate& rate, unsigned long long e0, float (&f)[8]) {
+    unsigned w[4];
+    random_group(rng, e0 >> 3, w);
+    const int shift = (int)(e0 & 7);
+    if (shift) {
+        unsigned u[4];
+        random_group(rng, (e0 >> 3) + 1, u);
+        unsigned all[8] = {w[0], w[1], w[2], w[3], u[0], u[1], u[2], u[3]};
+        // all >>= 16 * shift bits
+        if (shift & 4)
+#pragma unroll
+            for (int i = 0; i < 6; ++i) all[i] = all[i + 2];
+        if (shift & 2)
+#pragma unroll
+            for (int i = 0; i < 5; ++i) all[i] = all[i + 1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (shift & 1) ? (all[i] >> 16) | (all[i + 1] << 16) : all[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = random16(w, i) >= rate.threshold ? rate.scale : 0.0f;
+}
+
+// Sum over the THREADS lanes that share a row; every lane gets it.  `red` holds one pair per
+// wavefront; a caller alternates between two of them so that one barrier per call is enough.
+template <int THREADS>
+__device__ __forceinline__ float2 row_sum(float a, float b, float2* red) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        a += __shfl_xor(a, d);
+        b += __shfl_xor(b, d);
+    }
+    if (THREADS > kWave) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.0f;
+#pragma unroll
+        for (int i = 0; i < THREADS / kWave; ++i) {
+            a += red[i].x;
+            b += red[i].y;
+        }
+    }
+    return make_float2(a, b);
+}
+
+struct NormFwd {
+    const float *x, *residual, *gamma, *beta;
+    float *y, *h, *mean, *rstd;      // mean, rstd may be null
+    const long long* rng;
+    DropoutRate rate;
+    unsigned channel;
+    long rows;
+    int cols;
+    float eps;
+};
+
+// FUSED: h = residual + dropout(x) is formed, stored and normalised; DROP: with a mask (p > 0).
+template <int TPR, int CH, int N, bool FUSED, bool DROP>
+__global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormFwd a) {
+    constexpr int RPB = kNormThreads / TPR;
+    __shared__ float2 red[2][kNormThreads / kWave];
+    const int lane = threadIdx.x % TPR;
+    const float inv = 1.0f / (float)a.cols;
+    float gamma[CH][N], beta[CH][N];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        load_cols<N>(a.gamma, (lane + c * TPR) * N, a.cols, gamma[c]);
+        load_cols<N>(a.beta, (lane + c * TPR) * N, a.cols, beta[c]);
+    }
+    RngState rng = {};
+    if (DROP) rng = load_rng(a.rng, a.channel);
+    for (long row = (long)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += (long)gridDim.x * RPB) {
+        const long at = row * a.cols;
+        float v[CH][N];
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) load_cols<N>(a.x + at, (lane + c * TPR) * N, a.cols, v[c]);
+        if (FUSED) {
+            float r[CH][N];
+#pragma unroll
+            for (int c = 0; c < CH; ++c) load_cols<N>(a.residual + at, (lane + c * TPR) * N, a.cols, r[c]);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int c0 = (lane + c * TPR) * N;
+                if constexpr (DROP) {
+                    if (c0 < a.cols) {
+                        float f[8];
+                        keep_factors(rng, a.rate, (unsigned long long)(at + c0), f);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) v[c][i] = f[i] > 0.0f ? v[c][i] * f[i] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[c][i] += r[c][i];
+                store_cols<N>(a.h + at, c0, a.cols, v[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum += v[c][i];
+        const float mean = row_sum<TPR>(sum, 0.0f, red[0]).x * inv;
+        float sq = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float d = v[c][i] - mean;
+                v[c][i] = d;
+                if ((lane + c * TPR) * N + i < a.cols) sq += d * d;
+            }
+        const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, 0.0f, red[1]).x * inv + a.eps);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[c][i] = v[c][i] * rstd * gamma[c][i] + beta[c][i];
+            store_cols<N>(a.y + at, (lane + c * TPR) * N, a.cols, v[c]);
+        }
+        if (lane == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+    }
+}
+
+// Rows longer than the registers hold.  A thread meets the same columns in every walk, so what it
+// reads back from h is what it wrote.
+template <bool FUSED, bool DROP>
+__global__ __launch_bounds__(kWideThreads) void norm_fwd_wide_kernel(NormFwd a) {
+    __shared__ float2 red[2][kWideThreads / kWave];
+    const float inv = 1.0f / (float)a.cols;
+    RngState rng = {};
+    if (DROP) rng = load_rng(a.rng, a.channel);
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const long at = row * a.cols;
+        const float* src = FUSED ? a.h + at : a.x + at;
+        float sum = 0.0f;
+        for (int c0 = threadIdx.x * 8; c0 < a.cols; c0 += kWideThreads * 8) {
+            float v[8];
+            load_cols<8>(a.x + at, c0, a.cols, v);
+            if (FUSED) {
+                float r[8];
+                load_cols<8>(a.residual + at, c0, a.cols, r);
+                if (DROP) {
+                    float f[8];
+                    keep_factors(rng, a.rate, (unsigned long long)(at + c0), f);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = f[i] > 0.0f ? v[i] * f[i] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] += r[i];
+                store_cols<8>(a.h + at, c0, a.cols, v);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += v[i];
+        }
+        const float mean = row_sum<kWideThreads>(sum, 0.0f, red[0]).x * inv;
+        float sq = 0.0f;
+        for (int c0 = threadIdx.x * 8; c0 < a.cols; c0 += kWideThreads * 8) {
+            float v[8];
+            load_cols<8>(src, c0, a.cols, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c0 + i < a.cols) sq += (v[i] - mean) * (v[i] - mean);
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<kWideThreads>(sq, 0.0f, red[1]).x * inv + a.eps);
+        for (int c0 = threadIdx.x * 8; c0 < a.cols; c0 += kWideThreads * 8) {
+            float v[8], g[8], b[8];
+            load_cols<8>(src, c0, a.cols, v);
+            load_cols<8>(a.gamma, c0, a.cols, g);
+            load_cols<8>(a.beta, c0, a.cols, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (v[i] - mean) * rstd * g[i] + b[i];
+            store_cols<8>(a.y + at, c0, a.cols, v);
+        }
+        if (threadIdx.x == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+    }
+}
+
+struct NormBwd {
+    const float *x, *gamma, *mean, *rstd, *gy, *gh;      // gh: cotangent of x itself, or null
+    float *gx, *gdrop;                                   // gdrop: gradient through the dropout (DROP only)
+    float* partial;                                      // [workgroups][2][cols]: sums of gy * xhat, of gy
+    const long long* rng;
+    DropoutRate rate;
+    unsigned channel;
+    long rows;
+    int cols;
+};
+
+template <int TPR, int CH, int N, bool ADD, bool DROP>
+__global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormBwd a) {
+    constexpr int RPB = kNormThreads / TPR;
+    __shared__ float2 red[2][kNormThreads / kWave];
+    __shared__ float join[TPR == kWave ? 3 * kWave * CH * N : 1];
+    const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const float inv = 1.0f / (float)a.cols;
+    float gamma[CH][N], sum_gx[CH][N], sum_g[CH][N];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        load_cols<N>(a.gamma, (lane + c * TPR) * N, a.cols, gamma[c]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum_gx[c][i] = sum_g[c][i] = 0.0f;
+    }
+    RngState rng = {};
+    if (DROP) rng = load_rng(a.rng, a.channel);
+    int turn = 0;
+    for (long row = (long)blockIdx.x * RPB + sub; row < a.rows; row += (long)gridDim.x * RPB, turn ^= 1) {
+        const long at = row * a.cols;
+        float x[CH][N], g[CH][N], add[CH][N];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) load_cols<N>(a.x + at, (lane + c * TPR) * N, a.cols, x[c]);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) load_cols<N>(a.gy + at, (lane + c * TPR) * N, a.cols, g[c]);
+        if (ADD)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) load_cols<N>(a.gh + at, (lane + c * TPR) * N, a.cols, add[c]);
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float xhat = (x[c][i] - mean) * rstd, gy = g[c][i];
+                sum_gx[c][i] += gy * xhat;       // columns beyond the row: gy and gamma are 0, and nothing of them is stored
+                sum_g[c][i] += gy;
+                const float gg = gy * gamma[c][i];
+                x[c][i] = xhat;
+                g[c][i] = gg;
+                if ((lane + c * TPR) * N + i < a.cols) {
+                    s1 += gg;
+                    s2 += gg * xhat;
+                }
+            }
+        const float2 s = row_sum<TPR>(s1, s2, red[turn]);
+        const float m1 = s.x * inv, m2 = s.y * inv;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int c0 = (lane + c * TPR) * N;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                g[c][i] = rstd * (g[c][i] - m1 - x[c][i] * m2);
+                if (ADD) g[c][i] += add[c][i];
+            }
+            store_cols<N>(a.gx + at, c0, a.cols, g[c]);
+            if constexpr (DROP) {
+                if (c0 < a.cols) {
+                    float f[8];
+                    keep_factors(rng, a.rate, (unsigned long long)(at + c0), f);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) g[c][i] = f[i] > 0.0f ? g[c][i] * f[i] : 0.0f;
+                    store_cols<N>(a.gdrop + at, c0, a.cols, g[c]);
+                }
+            }
+        }
+    }
+    float* out = a.partial + (long)blockIdx.x * 2 * a.cols;
+    if constexpr (TPR == kWave) {       // the four wavefronts own the same columns: added in order
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+            if (sub > 0)
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        join[((sub - 1) * CH * N + c * N + i) * kWave + lane] = which ? sum_g[c][i] : sum_gx[c][i];
+            __syncthreads();
+            if (sub == 0)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+#pragma unroll
+                        for (int o = 0; o < 3; ++o) {
+                            const float v = join[(o * CH * N + c * N + i) * kWave + lane];
+                            if (which) sum_g[c][i] += v;
+                            else sum_gx[c][i] += v;
+                        }
+                    store_cols<N>(out + which * a.cols, (lane + c * TPR) * N, a.cols, which ? sum_g[c] : sum_gx[c]);
+                }
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            store_cols<N>(out, (lane + c * TPR) * N, a.cols, sum_gx[c]);
+            store_cols<N>(out + a.cols, (lane + c * TPR) * N, a.cols, sum_g[c]);
+        }
+    }
+}
+
+template <bool ADD, bool DROP>
+__global__ __launch_bounds__(kWideThreads) void norm_bwd_wide_kernel(NormBwd a) {
+    __shared__ float2 red[2][kWideThreads / kWave];
+    const float inv = 1.0f / (float)a.cols;
+    RngState rng = {};
+    if (DROP) rng = load_rng(a.rng, a.channel);
+    int turn = 0;
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const long at = row * a.cols;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int c0 = threadIdx.x * 8; c0 < a.cols; c0 += kWideThreads * 8) {
+            float x[8], g[8], w[8];
+            load_cols<8>(a.x + at, c0, a.cols, x);
+            load_cols<8>(a.gy + at, c0, a.cols, g);
+            load_cols<8>(a.gamma, c0, a.cols, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c0 + i < a.cols) {
+                    const float gg = g[i] * w[i];
+                    s1 += gg;
+                    s2 += gg * ((x[i] - mean) * rstd);
+                }
+        }
+        const float2 s = row_sum<kWideThreads>(s1, s2, red[turn]);
+        const float m1 = s.x * inv, m2 = s.y * inv;
+        for (int c0 = threadIdx.x * 8; c0 < a.cols; c0 += kWideThreads * 8) {
+            float x[8], g[8], w[8];
+            load_cols<8>(a.x + at, c0, a.cols, x);
+            load_cols<8>(a.gy + at, c0, a.cols, g);
+            load_cols<8>(a.gamma, c0, a.cols, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[i] = rstd * (g[i] * w[i] - m1 - (x[i] - mean) * rstd * m2);
+            if (ADD) {
+                float add[8];
+                load_cols<8>(a.gh + at, c0, a.cols, add);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] += add[i];
+            }
+            store_cols<8>(a.gx + at, c0, a.cols, g);
+            if (DROP) {
+                float f[8];
+                keep_factors(rng, a.rate, (unsigned long long)(at + c0), f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] = f[i] > 0.0f ? g[i] * f[i] : 0.0f;
+                store_cols<8>(a.gdrop + at, c0, a.cols, g);
+            }
+        }
+    }
+}
+
+// Partial sums of the weights' gradients for wide rows: workgroup (strip of 64 columns, part of the rows).
+__global__ __launch_bounds__(kNormThreads) void norm_bwd_wide_weights_kernel(NormBwd a, long rows_per) {
+    __shared__ float2 join[kNormThreads];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63);
+    const long first = blockIdx.y * rows_per, last = first + rows_per < a.rows ? first + rows_per : a.rows;
+    float s1 = 0.0f, s2 = 0.0f;
+    if (c < a.cols)
+        for (long row = first + (threadIdx.x >> 6); row < last; row += kNormThreads / 64) {
+            const float g = a.gy[row * a.cols + c];
+            s1 += g * ((a.x[row * a.cols + c] - a.mean[row]) * a.rstd[row]);
+            s2 += g;
+        }
+    join[threadIdx.x] = make_float2(s1, s2);
+    __syncthreads();
+    if (threadIdx.x < 64 && c < a.cols) {
+        for (int o = 1; o < kNormThreads / 64; ++o) {
+            s1 += join[threadIdx.x + o * 64].x;
+            s2 += join[threadIdx.x + o * 64].y;
+        }
+        float* out = a.partial + (long)blockIdx.y * 2 * a.cols;
+        out[c] = s1;
+        out[a.cols + c] = s2;
+    }
+}
+
+// ggamma, gbeta = the partial rows added up: 32 columns per workgroup, 32 groups of rows.
+__global__ __launch_bounds__(1024) void norm_weights_kernel(const float* __restrict__ partial, int parts, int cols,
+                                                            float* __restrict__ ggamma, float* __restrict__ gbeta) {
+    __shared__ float join[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;      // c in [0, 2 * cols)
+    const long pitch = 2L * cols;
+    float s = 0.0f;
+    if (c < 2 * cols) {
+#pragma unroll 8
+        for (int p = g; p < parts; p += 32) s += partial[p * pitch + c];
+    }
+    join[g][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (g == 0 && c < 2 * cols) {
+        for (int o = 1; o < 32; ++o) s += join[o][threadIdx.x];
+        if (c < cols) ggamma[c] = s;
+        else gbeta[c - cols] = s;
+    }
+}
+
+// y = dropout(x) (+ residual): a thread takes whole groups of eight elements, one generator call each.
+template <bool RES>
+__global__ __launch_bounds__(256) void dropout_kernel(const float* __restrict__ x, const float* __restrict__ residual, float* __restrict__ y,
+                                                      const long long* __restrict__ state, DropoutRate rate, unsigned channel, long n) {
+    const RngState rng = load_rng(state, channel);
+    const long groups = (n + 7) >> 3;
+    const long g = (long)blockIdx.x * 256 + threadIdx.x;
+    if (g >= groups) return;
+    const int left = n - 8 * g < 8 ? (int)(n - 8 * g) : 8;
+    float v[8], r[8], f[8];
+    load_cols<8>(x + 8 * g, 0, left, v);
+    if (RES) load_cols<8>(residual + 8 * g, 0, left, r);
+    keep_factors(rng, rate, 8ull * g, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        v[i] = f[i] > 0.0f ? v[i] * f[i] : 0.0f;
+        if (RES) v[i] += r[i];
+    }
+    store_cols<8>(y + 8 * g, 0, left, v);
+}
+
+// ---------------------------------------------------------------- launchers
+
+template <bool FUSED, bool DROP>
+static int launch_norm_fwd(const NormFwd& a, hipStream_t st) {
+    constexpr int N = DROP ? 8 : 4;      // columns per lane and piece: a generator group under dropout
+    auto blocks = [&](int rpb) { return dim3((unsigned)std::min(cdiv(a.rows, rpb), 4L * kNumCU * 2)); };
+    const int pieces = (int)cdiv(a.cols, N);
+    if (pieces <= 64) norm_fwd_kernel<64, 1, N, FUSED, DROP><<<blocks(4), kNormThreads, 0, st>>>(a);
+    else if (pieces <= 128) norm_fwd_kernel<64, 2, N, FUSED, DROP><<<blocks(4), kNormThreads, 0, st>>>(a);
+    else if (N == 4 && pieces <= 256) norm_fwd_kernel<64, 16 / N, N, FUSED, DROP><<<blocks(4), kNormThreads, 0, st>>>(a);
+    else if (pieces <= 4096 / N) norm_fwd_kernel<256, 16 / N, N, FUSED, DROP><<<blocks(1), kNormThreads, 0, st>>>(a);
+    else if (pieces <= 8192 / N) norm_fwd_kernel<256, 32 / N, N, FUSED, DROP><<<blocks(1), kNormThreads, 0, st>>>(a);
+    else norm_fwd_wide_kernel<FUSED, DROP><<<dim3((unsigned)std::min(a.rows, 2L * kNumCU)), kWideThreads, 0, st>>>(a);
+    CGT_LAUNCH_CHECK("layer norm forward");
+    return CGT_AMD_OK;
+}
+
+template <bool ADD, bool DROP>
+static int launch_norm_bwd(NormBwd a, float* ggamma, float* gbeta, void* stream) {
+    constexpr int N = DROP ? 8 : 4;
+    hipStream_t st = as_stream(stream);
+    const int pieces = (int)cdiv(a.cols, N);
+    const bool wave_rows = a.cols <= 1024, wide = a.cols > 8192;
+    long parts = wide ? std::min(cdiv(a.rows, 64), 64L) : std::min(cdiv(a.rows, wave_rows ? 4 : 1), 2L * kNumCU);
+    const long rows_per = wide ? cdiv(a.rows, parts) : 0;
+    if (wide) parts = cdiv(a.rows, rows_per);
+    a.partial = stream_workspace(stream, kWsNorm, (size_t)parts * 2 * a.cols * sizeof(float), "layer norm backward");
+    if (!a.partial) return CGT_AMD_ERR_NOMEM;
+    const dim3 grid((unsigned)parts);
+    if (pieces <= 64) norm_bwd_kernel<64, 1, N, ADD, DROP><<<grid, kNormThreads, 0, st>>>(a);
+    else if (pieces <= 128) norm_bwd_kernel<64, 2, N, ADD, DROP><<<grid, kNormThreads, 0, st>>>(a);
+    else if (N == 4 && pieces <= 256) norm_bwd_kernel<64, 16 / N, N, ADD, DROP><<<grid, kNormThreads, 0, st>>>(a);
+    else if (pieces <= 4096 / N) norm_bwd_kernel<256, 16 / N, N, ADD, DROP><<<grid, kNormThreads, 0, st>>>(a);
+    else if (!wide) norm_bwd_kernel<256, 32 / N, N, ADD, DROP><<<grid, kNormThreads, 0, st>>>(a);
+    else {
+        norm_bwd_wide_kernel<ADD, DROP><<<dim3((unsigned)std::min(a.rows, 2L * kNumCU)), kWideThreads, 0, st>>>(a);
+        CGT_LAUNCH_CHECK("layer norm backward");
+        norm_bwd_wide_weights_kernel<<<dim3((unsigned)cdiv(a.cols, 64), (unsigned)parts), kNormThreads, 0, st>>>(a, rows_per);
+    }
+    CGT_LAUNCH_CHECK("layer norm backward");
+    norm_weights_kernel<<<dim3((unsigned)cdiv(2L * a.cols, 32)), 1024, 0, st>>>(a.partial, (int)parts, a.cols, ggamma, gbeta);
+    CGT_LAUNCH_CHECK("layer norm weight gradient");
+    return CGT_AMD_OK;
+}
+
+static int check_rows(const char* what, long rows, long cols) {
+    CGT_ARG_CHECK(rows >= 0 && cols >= 0, "%s: negative extent (%ld rows, %ld columns)", what, rows, cols);
+    CGT_ARG_CHECK(cols < (1L << 30), "%s: rows of %ld columns are too long (2^30 at most)", what, cols);
+    CGT_ARG_CHECK(cols == 0 || rows < (1L << 60) / cols, "%s: the array is too large", what);
+    return CGT_AMD_OK;
+}
+
+static int zero_weights(float* ggamma, float* gbeta, long cols, void* stream) {
+    CGT_ARG_CHECK(ggamma && gbeta, "layer norm backward: null pointer");
+    const int rc = cgt_amd_fill_u32(ggamma, 0u, cols, stream);
+    return rc == CGT_AMD_OK ? cgt_amd_fill_u32(gbeta, 0u, cols, stream) : rc;
+}
+
+}  // namespace cgt_amd
+
+using namespace cgt_amd;
+
+CGT_API int cgt_amd_layer_norm_fwd_f32(const float* x, long rows, long cols, const float* gamma, const float* beta, double eps,
+                                       float* y, float* mean, float* rstd, void* stream) {
+    if (int rc = check_rows("layer norm", rows, cols)) return rc;
+    CGT_ARG_CHECK(eps >= 0.0, "layer norm: eps must not be negative (got %g)", eps);
+    if (rows == 0 || cols == 0) return CGT_AMD_OK;
+    CGT_ARG_CHECK(x && gamma && beta && y, "layer norm: null pointer");
+    NormFwd a = {};
+    a.x = x, a.gamma = gamma, a.beta = beta, a.y = y, a.mean = mean, a.rstd = rstd;
+    a.rows = rows, a.cols = (int)cols, a.eps = (float)eps;
+    return launch_norm_fwd<false, false>(a, as_stream(stream));
+}
+
+CGT_API int cgt_amd_layer_norm_bwd_f32(const float* x, const float* gamma, const float* mean, const float* rstd, const float* gy,
+                                       long rows, long cols, float* gx, float* ggamma, float* gbeta, void* stream) {
+    if (int rc = check_rows("layer norm backward", rows, cols)) return rc;
+    if (cols == 0) return CGT_AMD_OK;
+    if (rows == 0) return zero_weights(ggamma, gbeta, cols, stream);
+    CGT_ARG_CHECK(x && gamma && mean && rstd && gy && gx && ggamma && gbeta, "layer norm backward: null pointer");
+    NormBwd a = {};
+    a.x = x, a.gamma = gamma, a.mean = mean, a.rstd = rstd, a.gy = gy, a.gx = gx;
+    a.rows = rows, a.cols = (int)cols;
+    return launch_norm_bwd<false, false>(a, ggamma, gbeta, stream);
+}
+
+CGT_API int cgt_amd_dropout_f32(const float* x, const float* residual, long n, double p, const long long* rng, unsigned channel,
+                                float* y, void* stream) {
+    CGT_ARG_CHECK(n >= 0, "dropout: negative count");
+    DropoutRate rate;
+    if (!dropout_rate(p, "dropout", &rate)) return CGT_AMD_ERR_ARG;
+    if (n == 0) return CGT_AMD_OK;
+    CGT_ARG_CHECK(x && y && rng, "dropout: null pointer");
+    const long blocks = cdiv(cdiv(n, 8), 256);
+    CGT_ARG_CHECK(blocks < (1L << 31), "dropout: too many elements");
+    hipStream_t st = as_stream(stream);
+    if (residual) dropout_kernel<true><<<dim3((unsigned)blocks), 256, 0, st>>>(x, residual, y, rng, rate, channel, n);
+    else dropout_kernel<false><<<dim3((unsigned)blocks), 256, 0, st>>>(x, nullptr, y, rng, rate, channel, n);
+    CGT_LAUNCH_CHECK("dropout");
+    return CGT_AMD_OK;
+}
+
+CGT_API int cgt_amd_dropout_add_layer_norm_fwd_f32(const float* x, const float* residual, long rows, long cols, double p,
+                                                   const long long* rng, unsigned channel, const float* gamma, const float* beta,
+                                                   double eps, float* y, float* h, float* mean, float* rstd, void* stream) {
+    if (int rc = check_rows("dropout + add + layer norm", rows, cols)) return rc;
+    CGT_ARG_CHECK(eps >= 0.0, "dropout + add + layer norm: eps must not be negative (got %g)", eps);
+    NormFwd a = {};
+    if (!dropout_rate(p, "dropout + add + layer norm", &a.rate)) return CGT_AMD_ERR_ARG;
+    if (rows == 0 || cols == 0) return CGT_AMD_OK;
+    CGT_ARG_CHECK(x && residual && gamma && beta && y && h, "dropout + add + layer norm: null pointer");
+    CGT_ARG_CHECK(rng || a.rate.threshold == 0, "dropout + add + layer norm: dropout needs the generator's state");
+    a.x = x, a.residual = residual, a.gamma = gamma, a.beta = beta, a.y = y, a.h = h, a.mean = mean, a.rstd = rstd;
+    a.rng = rng, a.channel = channel, a.rows = rows, a.cols = (int)cols, a.eps = (float)eps;
+    return a.rate.threshold ? launch_norm_fwd<true, true>(a, as_stream(stream)) : launch_norm_fwd<true, false>(a, as_stream(stream));
+}
+
+CGT_API int cgt_amd_dropout_add_layer_norm_bwd_f32(const float* h, const float* gamma, const float* mean, const float* rstd,
+                                                   const float* gy, const float* gh, long rows, long cols, double p,
+                                                   const long long* rng, unsigned channel, float* gx, float* gresidual,
+                                                   float* ggamma, float* gbeta, void* stream) {
+    if (int rc = check_rows("dropout + add + layer norm backward", rows, cols)) return rc;
+    NormBwd a = {};
+    if (!dropout_rate(p, "dropout + add + layer norm backward", &a.rate)) return CGT_AMD_ERR_ARG;
+    if (cols == 0) return CGT_AMD_OK;
+    if (rows == 0) return zero_weights(ggamma, gbeta, cols, stream);
+    CGT_ARG_CHECK(h && gamma && mean && rstd && gy && gresidual && ggamma && gbeta, "dropout + add + layer norm backward: null pointer");
+    CGT_ARG_CHECK(a.rate.threshold == 0 || (rng && gx), "dropout + add + layer norm backward: dropout needs the generator's state and gx");
+    a.x = h, a.gamma = gamma, a.mean = mean, a.rstd = rstd, a.gy = gy, a.gh = gh, a.gx = gresidual, a.gdrop = gx;
+    a.rng = rng, a.channel = channel, a.rows = rows, a.cols = (int)cols;
+    if (a.rate.threshold == 0) {
+        // without a mask the two gradients are one array; a caller that wants both gets a copy
+        const int rc = gh ? launch_norm_bwd<true, false>(a, ggamma, gbeta, stream) : launch_norm_bwd<false, false>(a, ggamma, gbeta, stream);
+        if (rc != CGT_AMD_OK || !gx || gx == gresidual) return rc;
+        return cgt_amd_stream_copy(gx, gresidual, rows * cols * (long)sizeof(float), stream);
+    }
+    return gh ? launch_norm_bwd<true, true>(a, ggamma, gbeta, stream) : launch_norm_bwd<false, true>(a, ggamma, gbeta, stream);
+}

@@ -52,6 +52,11 @@ class GpuArray(object):
         """Device address as an int (pass to the C ABI as void*)."""
         return self._buffer.ptr + self._offset
 
+    @property
+    def __cuda_array_interface__(self):
+        """Lets another library view this array without a copy."""
+        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr, False), "strides": None, "version": 2}
+
     def reshape(self, *shape):
         """Zero-copy view with a new shape (the reference's Reshape op is a view
         too, cgt/core.py:1452-1465)."""
@@ -84,6 +89,40 @@ class GpuArray(object):
 
 def empty(shape, dtype=np.float32):
     return GpuArray(shape, dtype)
+
+
+class _Borrowed(object):
+    """Device memory that belongs to another library's array, kept alive by holding on to it."""
+
+    def __init__(self, ptr, nbytes, owner):
+        self.ptr, self.nbytes, self.owner = ptr, nbytes, owner
+
+
+def as_gpuarray(x):
+    """Zero-copy view of another library's device array (anything with `__cuda_array_interface__`, e.g. a torch
+    tensor on this GPU): contiguous, of a type device arrays have.  Calls made with it must be ordered with the
+    other library's work by the caller (the same stream, or synchronisation).  Both libraries have to share one HIP
+    runtime: import torch before the first call into this package."""
+    if isinstance(x, GpuArray):
+        return x
+    info = x.__cuda_array_interface__
+    dtype, shape = np.dtype(info["typestr"]), tuple(int(s) for s in info["shape"])
+    if dtype not in _DTYPES:
+        raise TypeError("unsupported device dtype %s" % dtype)
+    strides = info.get("strides")
+    if strides is not None and 0 not in shape:
+        dense = dtype.itemsize
+        for extent, stride in zip(reversed(shape), reversed(strides)):
+            if extent > 1 and stride != dense:
+                raise ValueError("device arrays are contiguous: shape %s with strides %s is not" % (shape, tuple(strides)))
+            dense *= extent
+    ptr = int(info["data"][0])
+    if ptr == 0 and 0 not in shape:
+        raise ValueError("the array has no device memory")
+    if ptr % dtype.itemsize:
+        raise ValueError("the array is not aligned to its elements")
+    nbytes = int(np.prod(shape, dtype=np.int64)) * dtype.itemsize if shape else dtype.itemsize
+    return GpuArray(shape, dtype, _buffer=_Borrowed(ptr, nbytes, x))
 
 
 def _contiguous(host, dtype=None):

@@ -191,6 +191,110 @@ def transpose4(x, axes, out=None, stream=None):
     return res
 
 
+# ---------------------------------------------------------------- layer norm and dropout
+
+def _rows_cols(x, gamma, *like):
+    """A device array normalised over its last axis, as (rows, columns); `gamma` and what `like` lists must fit it."""
+    if x.ndim < 1:
+        raise ValueError("layer norm takes an array of at least one axis")
+    cols = x.shape[-1]
+    if gamma.shape != (cols,):
+        raise ValueError("weights of shape %s do not fit rows of %d columns" % (gamma.shape, cols))
+    for a in like:
+        if a.shape != x.shape:
+            raise ValueError("operands of shapes %s and %s must be equal" % (a.shape, x.shape))
+    return int(np.prod(x.shape[:-1], dtype=np.int64)), cols
+
+
+def _rng(rng, p):
+    """The generator's state, int64 [seed, step] on the device; None is fine where nothing is dropped."""
+    if rng is None:
+        if p:
+            raise ValueError("dropout needs the generator's state: an int64 device array (seed, step)")
+        return None
+    if not isinstance(rng, GpuArray) or rng.dtype != np.int64 or rng.shape != (2,):
+        raise TypeError("the generator's state is an int64 device array of two elements (seed, step)")
+    return rng.ptr
+
+
+def layer_norm_fwd(x, gamma, beta, eps=1e-5, out=None, stream=None):
+    """Layer norm over the last axis: returns (y, mean, rstd), the statistics with the shape of the other axes."""
+    _f32(x, gamma, beta)
+    rows, cols = _rows_cols(x, gamma)
+    if beta.shape != gamma.shape:
+        raise ValueError("gamma %s and beta %s must have one shape" % (gamma.shape, beta.shape))
+    y, mean, rstd = (_out(o, s) for o, s in zip(out or (None,) * 3, (x.shape, x.shape[:-1], x.shape[:-1])))
+    capi.check(capi.lib().cgt_amd_layer_norm_fwd_f32(x.ptr, rows, cols, gamma.ptr, beta.ptr, float(eps), y.ptr, mean.ptr, rstd.ptr, stream))
+    return y, mean, rstd
+
+
+def layer_norm_bwd(x, gamma, mean, rstd, gy, out=None, stream=None):
+    """The gradients of layer_norm_fwd: returns (gx, ggamma, gbeta)."""
+    _f32(x, gamma, mean, rstd, gy)
+    rows, cols = _rows_cols(x, gamma, gy)
+    if mean.shape != x.shape[:-1] or rstd.shape != mean.shape:
+        raise ValueError("row statistics of shapes %s and %s do not fit x %s" % (mean.shape, rstd.shape, x.shape))
+    gx, ggamma, gbeta = (_out(o, s) for o, s in zip(out or (None,) * 3, (x.shape, gamma.shape, gamma.shape)))
+    capi.check(capi.lib().cgt_amd_layer_norm_bwd_f32(x.ptr, gamma.ptr, mean.ptr, rstd.ptr, gy.ptr, rows, cols,
+                                                     gx.ptr, ggamma.ptr, gbeta.ptr, stream))
+    return gx, ggamma, gbeta
+
+
+def dropout(x, p, rng, channel=0, residual=None, out=None, stream=None):
+    """x with each element dropped with probability p (kept ones divided by the share kept), plus `residual` if
+    given.  The mask is a function of rng = int64 [seed, step] (on the device), `channel` and the element's index
+    (include/cgt_amd.h); the gradient with respect to x is the same call on the cotangent, without residual."""
+    _f32(x)
+    if rng is None:
+        raise ValueError("dropout needs the generator's state: an int64 device array (seed, step)")
+    if residual is not None:
+        _f32(residual)
+        if residual.shape != x.shape:
+            raise ValueError("residual %s must have x's shape %s" % (residual.shape, x.shape))
+    state, channel = _rng(rng, p), _channel(channel)
+    y = _out(out, x.shape)
+    capi.check(capi.lib().cgt_amd_dropout_f32(x.ptr, None if residual is None else residual.ptr, x.size, float(p), state,
+                                              channel, y.ptr, stream))
+    return y
+
+
+def _channel(channel):
+    if not 0 <= channel < 1 << 32:
+        raise ValueError("channel must be a whole number of 32 bits (got %s)" % (channel,))
+    return int(channel)
+
+
+def dropout_add_layer_norm_fwd(x, residual, gamma, beta, p=0.0, rng=None, channel=0, eps=1e-5, out=None, stream=None):
+    """h = residual + dropout(x), y = layer norm of h over the last axis, in one pass: returns (y, h, mean, rstd)."""
+    _f32(x, residual, gamma, beta)
+    rows, cols = _rows_cols(x, gamma, residual)
+    if beta.shape != gamma.shape:
+        raise ValueError("gamma %s and beta %s must have one shape" % (gamma.shape, beta.shape))
+    state, channel = _rng(rng, p), _channel(channel)
+    y, h, mean, rstd = (_out(o, s) for o, s in zip(out or (None,) * 4, (x.shape, x.shape, x.shape[:-1], x.shape[:-1])))
+    capi.check(capi.lib().cgt_amd_dropout_add_layer_norm_fwd_f32(
+        x.ptr, residual.ptr, rows, cols, float(p), state, channel, gamma.ptr, beta.ptr, float(eps),
+        y.ptr, h.ptr, mean.ptr, rstd.ptr, stream))
+    return y, h, mean, rstd
+
+
+def dropout_add_layer_norm_bwd(h, gamma, mean, rstd, gy, gh=None, p=0.0, rng=None, channel=0, out=None, stream=None):
+    """The gradients of dropout_add_layer_norm_fwd from the cotangents of y and (unless None) of h: returns
+    (gx, gresidual, ggamma, gbeta)."""
+    _f32(h, gamma, mean, rstd, gy)
+    if gh is not None:
+        _f32(gh)
+    rows, cols = _rows_cols(h, gamma, gy, *(() if gh is None else (gh,)))
+    if mean.shape != h.shape[:-1] or rstd.shape != mean.shape:
+        raise ValueError("row statistics of shapes %s and %s do not fit h %s" % (mean.shape, rstd.shape, h.shape))
+    state, channel = _rng(rng, p), _channel(channel)
+    gx, gres, ggamma, gbeta = (_out(o, s) for o, s in zip(out or (None,) * 4, (h.shape, h.shape, gamma.shape, gamma.shape)))
+    capi.check(capi.lib().cgt_amd_dropout_add_layer_norm_bwd_f32(
+        h.ptr, gamma.ptr, mean.ptr, rstd.ptr, gy.ptr, None if gh is None else gh.ptr, rows, cols, float(p), state,
+        channel, gx.ptr, gres.ptr, ggamma.ptr, gbeta.ptr, stream))
+    return gx, gres, ggamma, gbeta
+
+
 # ---------------------------------------------------------------- conv-layer glue
 
 UNARY_OPS = ["abs", "cos", "exp", "log", "neg", "sign", "sin", "square", "sqrt", "tanh", "sigmoid"]

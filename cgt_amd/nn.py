@@ -21,7 +21,9 @@ from . import core
 from .nn_ops import conv_col, conv_same
 from .nn_ops import cross_channel_lrn as _lrn
 from .nn_ops.cross_channel_lrn import cross_channel_lrn  # noqa: F401
+from .nn_ops.dropout import dropout, rng_state  # noqa: F401
 from .nn_ops.im2col import im2col
+from .nn_ops.layer_norm import dropout_add_layer_norm, layer_norm  # noqa: F401
 from .nn_ops.max_pool_2d import MaxPool, PoolInfo
 
 
@@ -159,6 +161,22 @@ class Affine(object):
 
     def __call__(self, x):
         return core.broadcast("+", core.dot(core.as_node(x), self.weight), self.bias, "xx,1x")
+
+
+class LayerNorm(object):
+    """layer_norm over rows of `size` columns with its own weights: gamma [size] (ones by default), beta [size]
+    (zeros by default), device-resident leaf nodes."""
+
+    def __init__(self, size, eps=1e-5, name=None, weight_init=None, bias_init=None):
+        import numpy as np
+        size = int(size)
+        self.eps = float(eps)
+        self.name = "unnamed" if name is None else name
+        self.weight = core.constant(np.ones(size, np.float32) if weight_init is None else np.asarray(weight_init, np.float32).reshape(size))
+        self.bias = core.constant(np.zeros(size, np.float32) if bias_init is None else np.asarray(bias_init, np.float32).reshape(size))
+
+    def __call__(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
 
 
 def softmax(x, axis=1):

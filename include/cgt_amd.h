@@ -285,6 +285,63 @@ int cgt_amd_lrn_bwd_from_x_f32(const float *x, const float *top_diff, long N, lo
                                long W, int size, double alpha, double beta, double k,
                                float *bottom_diff, void *stream);
 
+/* ---------------------------------------------------------------- layer norm and dropout
+ *
+ * The reference has no counterpart of these; they stand beside cross-channel
+ * LRN (normalisation) and the elementwise ops.  Arrays are [rows][cols],
+ * row-major; a row is normalised over its columns.  Any cols below 2^30, any
+ * 4-byte alignment.  Input and output ranges must not overlap.  Sums run in a
+ * fixed order: same input, same bits. */
+
+/* mean[r] = sum_c x / cols, rstd[r] = 1 / sqrt(sum_c (x - mean)^2 / cols + eps),
+ * y = gamma[c] * (x - mean) * rstd + beta[c].  mean / rstd (rows floats each,
+ * the operands of the gradient) may be NULL. */
+int cgt_amd_layer_norm_fwd_f32(const float *x, long rows, long cols, const float *gamma,
+                               const float *beta, double eps, float *y, float *mean, float *rstd,
+                               void *stream);
+
+/* gx = rstd * (g - sum_c(g) / cols - xhat * sum_c(g * xhat) / cols) with
+ * g = gy * gamma, xhat = (x - mean) * rstd; ggamma[c] = sum_r gy * xhat,
+ * gbeta[c] = sum_r gy (zero for no rows).  Uses a workspace owned by the
+ * library (one partial row of each weight gradient per workgroup). */
+int cgt_amd_layer_norm_bwd_f32(const float *x, const float *gamma, const float *mean,
+                               const float *rstd, const float *gy, long rows, long cols, float *gx,
+                               float *ggamma, float *gbeta, void *stream);
+
+/* Random numbers.  Dropout takes its mask from a counter-based generator
+ * (Philox4x32, 7 rounds) and stores none: the gradient calls the same entry
+ * point on the cotangent.  `rng` is DEVICE memory, two 64-bit integers: the
+ * seed (the generator's key) and a step (its low 32 bits are used).  Kernels
+ * read it when they run, so a replayed graph draws the numbers of the step that
+ * is in it then.  `channel` tells apart the uses within one step (one per
+ * layer, say).  Group g of a use is Philox(counter = {g low, g high, channel,
+ * step}) = four 32-bit words = eight 16-bit numbers, low half first; flat
+ * element e takes number e % 8 of group e / 8.  An element is dropped when its
+ * number is below floor(65536 p + 1/2): probabilities are multiples of 2^-16,
+ * and kept values are multiplied by the reciprocal of the share kept, so
+ * expectations are exact.  0 <= p < 1 - 2^-17. */
+
+/* y = x * keep / share (+ residual, unless NULL), n elements.  A dropped
+ * element contributes 0 whatever x holds there. */
+int cgt_amd_dropout_f32(const float *x, const float *residual, long n, double p, const long long *rng,
+                        unsigned channel, float *y, void *stream);
+
+/* h = residual + dropout(x), y = layer norm of h, in one pass (the end of a
+ * residual sub-layer).  rng may be NULL if p rounds to 0. */
+int cgt_amd_dropout_add_layer_norm_fwd_f32(const float *x, const float *residual, long rows, long cols,
+                                           double p, const long long *rng, unsigned channel,
+                                           const float *gamma, const float *beta, double eps, float *y,
+                                           float *h, float *mean, float *rstd, void *stream);
+
+/* Its gradients from the cotangents gy of y and gh of h (NULL: none):
+ * gresidual = gh + layer norm gradient of gy, gx = dropout(gresidual).  With p
+ * rounding to 0 the two are equal and gx may be NULL or gresidual itself. */
+int cgt_amd_dropout_add_layer_norm_bwd_f32(const float *h, const float *gamma, const float *mean,
+                                           const float *rstd, const float *gy, const float *gh, long rows,
+                                           long cols, double p, const long long *rng, unsigned channel,
+                                           float *gx, float *gresidual, float *ggamma, float *gbeta,
+                                           void *stream);
+
 /* ---------------------------------------------------------------- GEMM */
 
 /* Row-major C[M,N] = op(A) . op(B), alpha = 1, beta = 0, true fp32 (MFMA
