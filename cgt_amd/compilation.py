@@ -211,7 +211,6 @@ def prebuild_standard_ops():
     linfo = nn_ops.cross_channel_lrn.LRNInfo(5, 1e-4, 0.75)
     cinfo = nn_ops.conv_same.ConvSameInfo(3, 3)
     T1 = core.TensorType("f4", 1)
-    R = core.TensorType("i8", 1)
     todo = [
         (nn_ops.im2col.Im2Col(info), [T4]),
         (nn_ops.im2col.Col2Im(info), [T4, S, S, S, S]),
@@ -238,11 +237,6 @@ def prebuild_standard_ops():
         (nn_ops.conv_col.ConvPatchForward(info, True, True), [T4, T4, T4]),
         (nn_ops.conv_col.ConvPatchBackwardData(info), [T4, T4, T4]),
         (nn_ops.conv_col.ConvPatchBackwardFilter(info), [T4, T4, T4]),
-        (nn_ops.layer_norm.LayerNorm(1e-5), [T2, T1, T1]),
-        (nn_ops.layer_norm.LayerNormBackward(), [T2, T1, T1, T1, T2]),
-        (nn_ops.layer_norm.DropoutAddLayerNorm(0.1, 1e-5, 0), [T2, T2, T1, T1, R]),
-        (nn_ops.layer_norm.DropoutAddLayerNormBackward(0.1, 0, True), [T2, T1, T1, T1, T2, T2, R]),
-        (nn_ops.dropout.Dropout(0.1, 0), [T2, R]),
         (core.Transport("gpu"), [T4]),
         # conv-layer glue: the closure code is generic over element type and
         # rank, so one library per op class serves every use
@@ -256,6 +250,24 @@ def prebuild_standard_ops():
         (core.Reshape(), [T4, S, S]),
         (core.TupleIndex(0), [core.TupleType(T4, I4)]),
     ]
+    return _prebuild(todo)
+
+
+def prebuild_transformer_ops():
+    """The same for the ops of a transformer layer."""
+    from . import nn_ops
+    T1, T2 = core.TensorType("f4", 1), core.TensorType("f4", 2)
+    R = core.TensorType("i8", 1)
+    return _prebuild([
+        (nn_ops.layer_norm.LayerNorm(1e-5), [T2, T1, T1]),
+        (nn_ops.layer_norm.LayerNormBackward(), [T2, T1, T1, T1, T2]),
+        (nn_ops.layer_norm.DropoutAddLayerNorm(0.1, 1e-5, 0), [T2, T2, T1, T1, R]),
+        (nn_ops.layer_norm.DropoutAddLayerNormBackward(0.1, 0, True), [T2, T1, T1, T1, T2, T2, R]),
+        (nn_ops.dropout.Dropout(0.1, 0), [T2, R]),
+    ])
+
+
+def _prebuild(todo):
     built = []
     for op, types in todo:
         nci = op.get_native_compile_info(types, "gpu")
