@@ -26,7 +26,7 @@ CPP_FLAGS = ["-fvisibility=hidden", "-std=c++11", "-fPIC", "-O3", "-DNDEBUG"]
 INCLUDE = os.path.join(ROOT, "include")
 
 SOURCES = ["runtime.hip", "im2col.hip", "pool.hip", "lrn.hip", "gemm.hip", "glue.hip", "elwise.hip", "conv.hip",
-           "norm.hip"]
+           "norm.hip", "attention.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

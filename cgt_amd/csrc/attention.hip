@@ -1,0 +1,725 @@
+// Attention with a learned relative position bias, forward and backward, for gfx950.
+//
+//   s_ij = scale * q_i . k_j + table[bucket(j - i - offset)][head]
+//   p_ij = exp(s_ij - lse_i), lse_i = log sum_j exp(s_ij) over the keys query i may see
+//   o_i = sum_j p_ij keep_ij v_j
+//   gv_j = sum_i p_ij keep_ij go_i
+//   ds_ij = p_ij (keep_ij go_i . v_j - go_i . o_i)
+//   gq_i = scale sum_j ds_ij k_j,  gk_j = scale sum_i ds_ij q_i
+//   gtable[c] = sum of ds_ij over batch, i and j with bucket(j - i - offset) = c
+//
+// The scores never leave the registers: a pass walks the keys (or the queries) in tiles of 32 and
+// keeps a running maximum and sum of every row.  The backward pass forms the probabilities again
+// from lse: one kernel per block of queries leaves gq and the table's gradient, one per block of
+// keys gk and gv, so no sum is shared between workgroups and results do not depend on the order
+// they run in.
+//
+// Matrix products are v_mfma_f32_32x32x2_f32 (true fp32).  A wavefront owns 32 columns (queries in
+// the first two kernels, keys in the third) and forms the *transposed* score tile, rows = the other
+// side: lane l then holds, for column l % 32, rows 8 g + 4 (l / 32) + t in register 4 g + t.  With
+// the k steps of the next product taken in that same order the score tile is that product's B
+// operand as it stands, with no exchange between lanes.
+#include "random.h"
+#include <algorithm>
+#include <cmath>
+
+namespace cgt_amd {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+struct __attribute__((packed, aligned(4))) float4p {      // 16 bytes at any 4-byte aligned address
+    float x, y, z, w;
+};
+
+constexpr int kAttnThreads = 256;
+constexpr int kAttnCols = 128;     // columns (queries or keys) per workgroup: 32 per wavefront
+constexpr int kAttnRows = 32;      // rows of the tile that the four wavefronts share
+constexpr int kMaxBuckets = 256;
+constexpr int kMaxDistance = 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct BucketRule {
+    int buckets, bidirectional, max_distance, first, side;
+    int edge[kMaxBuckets / 2 + 1];      // edge[e]: the smallest distance of logarithmic bucket e of a side, e >= 1
+};
+
+struct Attn {
+    const float *q, *k, *v, *table;
+    const int *q_lengths, *k_lengths;
+    const long long* rng;
+    long q_b, q_h, q_t, k_b, k_h, k_t;      // strides in floats; o, go, gq as q, and v, gk, gv as k
+    int B, H, Tq, Tk, D, causal, q_offset;
+    float scale;
+    DropoutRate rate;
+    unsigned channel;
+    BucketRule rule;
+};
+
+// Bucket of relative position `rel` (key minus query).
+__host__ __device__ inline int bucket_of(const BucketRule& r, int rel) {
+    const int n = r.bidirectional ? (rel < 0 ? -rel : rel) : (rel < 0 ? -rel : 0);
+    int b = n;
+    if (n >= r.first) {
+        b = r.first;
+        for (int e = 1; e < r.side - r.first; ++e) b += n >= r.edge[e] ? 1 : 0;
+    }
+    return b + (r.bidirectional && rel > 0 ? r.side : 0);
+}
+
+// ---- the bias in LDS: one value per relative position in [-reach, reach], reach = max_distance + 62.
+// A wavefront's tile spans 63 relative positions around its origin, so an origin clamped to
+// +-(max_distance + 31) keeps every index inside and leaves every value as it was: beyond
+// max_distance all positions of a side are in its last bucket.
+__host__ __device__ inline int bias_reach(const BucketRule& r) { return r.max_distance + 62; }
+__host__ __device__ inline int bias_window(const BucketRule& r) { return 2 * bias_reach(r) + 1; }
+__device__ __forceinline__ int clamp_origin(const BucketRule& r, int rel0) {
+    const int lim = r.max_distance + 31;
+    return rel0 < -lim ? -lim : rel0 > lim ? lim : rel0;
+}
+__device__ __forceinline__ void fill_bias(const Attn& a, int head, float* win) {
+    const int n = bias_window(a.rule), reach = bias_reach(a.rule);
+    for (int s = threadIdx.x; s < n; s += kAttnThreads) win[s] = a.table[(long)bucket_of(a.rule, s - reach) * a.H + head];
+}
+
+// Four floats of a row of D at column c; zero beyond the row's end.
+__device__ __forceinline__ float4 load4(const float* row, int c, int D) {
+    if (c + 4 <= D) {
+        const float4p v = *reinterpret_cast<const float4p*>(row + c);
+        return make_float4(v.x, v.y, v.z, v.w);
+    }
+    return make_float4(c < D ? row[c] : 0.0f, c + 1 < D ? row[c + 1] : 0.0f, c + 2 < D ? row[c + 2] : 0.0f, 0.0f);
+}
+__device__ __forceinline__ void store4(float* row, int c, int D, float x, float y, float z, float w) {
+    if (c + 4 <= D) {
+        *reinterpret_cast<float4p*>(row + c) = {x, y, z, w};
+    } else {
+        if (c < D) row[c] = x;
+        if (c + 1 < D) row[c + 1] = y;
+        if (c + 2 < D) row[c + 2] = z;
+    }
+}
+
+// Rows 8 g + 4 half .. + 3 of a 32-row result block, times f; zero where the column is none.
+__device__ __forceinline__ void store_scaled(float* row, int c, int D, const v16f& v, int g, bool valid, float f) {
+    store4(row, c, D, valid ? v[4 * g] * f : 0.0f, valid ? v[4 * g + 1] * f : 0.0f, valid ? v[4 * g + 2] * f : 0.0f, valid ? v[4 * g + 3] * f : 0.0f);
+}
+
+// A tile of 32 rows: loaded into registers by all 256 threads (rows at or beyond `end` are zero and
+// not read), later written to LDS with a row pitch of DP + 4 floats (16-byte reads of 32
+// consecutive rows then start in different banks).
+template <int DP>
+struct TileRegs {
+    float4 v[DP / 32];
+};
+template <int DP>
+__device__ __forceinline__ void tile_load(TileRegs<DP>& t, const float* base, long stride, int row0, int end, int D) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+        const int idx = threadIdx.x + i * kAttnThreads, row = row0 + idx / (DP / 4), c = (idx % (DP / 4)) * 4;
+        t.v[i] = row < end ? load4(base + row * stride, c, D) : make_float4(0, 0, 0, 0);
+    }
+}
+template <int DP>
+__device__ __forceinline__ void tile_store(const TileRegs<DP>& t, float* lds) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+        const int idx = threadIdx.x + i * kAttnThreads;
+        *reinterpret_cast<float4*>(lds + (idx / (DP / 4)) * (DP + 4) + (idx % (DP / 4)) * 4) = t.v[i];
+    }
+}
+
+// The lane's column as a B operand: d = 8 c + 4 half + t in register 4 c + t.
+template <int DP>
+__device__ __forceinline__ void column_load(float (&r)[DP / 2], const float* row, bool valid, int D, float scale) {
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+        const float4 v = valid ? load4(row, 8 * c + 4 * half, D) : make_float4(0, 0, 0, 0);
+        r[4 * c] = v.x * scale;
+        r[4 * c + 1] = v.y * scale;
+        r[4 * c + 2] = v.z * scale;
+        r[4 * c + 3] = v.w * scale;
+    }
+}
+
+// acc[row][col] += sum_d tile[row][d] * column[d]
+template <int DP>
+__device__ __forceinline__ v16f product_rows(v16f acc, const float* lds, const float (&col)[DP / 2]) {
+    const int lane = threadIdx.x & 63;
+    const float* row = lds + (lane & 31) * (DP + 4) + 4 * (lane >> 5);
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+        const float4 v = *reinterpret_cast<const float4*>(row + 8 * c);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.x, col[4 * c], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.y, col[4 * c + 1], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.z, col[4 * c + 2], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.w, col[4 * c + 3], acc, 0, 0, 0);
+    }
+    return acc;
+}
+// acc[d][col] += sum_row tile[row][d] * p[row][col]
+template <int DP>
+__device__ __forceinline__ void product_cols(v16f (&acc)[DP / 32], const float* lds, const v16f& p) {
+    const int lane = threadIdx.x & 63;
+    const float* at = lds + 4 * (lane >> 5) * (DP + 4) + (lane & 31);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (r >> 2) + (r & 3)) * (DP + 4) + 32 * d], p[r], acc[d], 0, 0, 0);
+}
+
+__device__ __forceinline__ int tile_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (r & 3); }
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+struct Where {
+    int b, h, tile;
+};
+// Workgroups of one head follow each other on one XCD (ids go round the eight of them), so that its
+// keys and values are read into one L2.
+__device__ __forceinline__ Where where(const Attn& a, int tiles) {
+    const int heads = a.B * a.H, id = blockIdx.x;
+    int head, tile;
+    if (heads % kNumXCD == 0) {
+        const int slot = id / kNumXCD;
+        head = id % kNumXCD + kNumXCD * (slot / tiles);
+        tile = slot % tiles;
+    } else {
+        head = id / tiles;
+        tile = id % tiles;
+    }
+    return {head / a.H, head % a.H, tile};
+}
+__device__ __forceinline__ int length_of(const int* lengths, int b, int T) {
+    if (!lengths) return T;
+    const int n = lengths[b];
+    return n < 0 ? 0 : n > T ? T : n;
+}
+
+// Which of a tile's 16 elements of a lane are hidden; rows are keys, the column is a query.
+__device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_end) {
+    return key >= k_end || (a.causal && key > query + a.q_offset);
+}
+
+// ---------------------------------------------------------------- forward
+
+template <int DP, bool BIAS, bool DROP>
+__global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(Attn a, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
+    extern __shared__ float lds[];
+    float *kt = lds, *vt = kt + kAttnRows * (DP + 4), *win = vt + kAttnRows * (DP + 4);
+    const Where w = where(a, tiles * splits);
+    const int split = w.tile % splits, q0 = w.tile / splits * kAttnCols;
+    const int lane = threadIdx.x & 63, qw = q0 + (threadIdx.x >> 6) * 32, query = qw + (lane & 31);
+    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
+    const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
+    const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
+    const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
+    if (BIAS) fill_bias(a, w.h, win);
+    // keys this workgroup walks: to the last one its last query sees, cut into `splits` runs of whole tiles
+    int last = k_end;
+    if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
+    if (q0 >= q_end) last = 0;
+    const int run = (last + kAttnRows * splits - 1) / (kAttnRows * splits) * kAttnRows;
+    const int first = split * run;
+    last = min(last, first + run);
+
+    float qreg[DP / 2];
+    column_load<DP>(qreg, a.q + qrow, query < q_end, a.D, a.scale);
+    RngState rng = {};
+    unsigned long long group0 = 0;
+    if (DROP) {
+        rng = load_rng(a.rng, a.channel);
+        group0 = ((unsigned long long)(w.b * a.H + w.h) * a.Tq + query) * ((a.Tk + 15) / 16) * 2 + (lane >> 5);
+    }
+    v16f acc[DP / 32] = {};
+    float m = -INFINITY, l = 0.0f;
+    TileRegs<DP> kr, vr;
+    tile_load<DP>(kr, kbase, a.k_t, first, last, a.D);
+    tile_load<DP>(vr, vbase, a.k_t, first, last, a.D);
+    for (int j0 = first; j0 < last; j0 += kAttnRows) {
+        __syncthreads();
+        tile_store<DP>(kr, kt);
+        tile_store<DP>(vr, vt);
+        __syncthreads();
+        if (j0 + kAttnRows < last) {
+            tile_load<DP>(kr, kbase, a.k_t, j0 + kAttnRows, last, a.D);
+            tile_load<DP>(vr, vbase, a.k_t, j0 + kAttnRows, last, a.D);
+        }
+        if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;      // nothing here for this wavefront
+        v16f s = {};
+        if (BIAS) {
+            const float* at = win + bias_reach(a.rule) + clamp_origin(a.rule, j0 - qw - a.q_offset) - (lane & 31);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = at[tile_row(r)];
+        }
+        s = product_rows<DP>(s, kt, qreg);
+        if (j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (hidden(a, j0 + tile_row(r), query, k_end)) s[r] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        top = fmaxf(m, fmaxf(top, other_half(top)));
+        const float ref = top == -INFINITY ? 0.0f : top;      // a row that has seen nothing yet
+        if (__any(top > m)) {
+            const float f = exp2f((m - ref) * kLog2e);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        }
+        m = top;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = exp2f((s[r] - ref) * kLog2e);
+            l += s[r];
+        }
+        if (DROP) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                unsigned u[4];
+                random_group(rng, group0 + 2ull * (j0 / 16 + b), u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[8 * b + e] = random16(u, e) >= a.rate.threshold ? s[8 * b + e] * a.rate.scale : 0.0f;
+            }
+        }
+        product_cols<DP>(acc, vt, s);
+    }
+    if (query >= a.Tq) return;
+    l += other_half(l);
+    const int half4 = 4 * (lane >> 5);
+    const long stat = ((long)w.b * a.H + w.h) * a.Tq + query;
+    if (splits > 1) {
+        const long row = (long)split * a.B * a.H * a.Tq + stat;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                store4(part + row * a.D, 32 * d + 8 * g + half4, a.D, acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
+        if (half4 == 0) part_ml[row] = make_float2(m, l);
+        return;
+    }
+    const bool saw = query < q_end && l != 0.0f;      // a row that saw no key is zero, whatever the values hold
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) store_scaled(o + qrow, 32 * d + 8 * g + half4, a.D, acc[d], g, saw, inv);
+    if (half4 == 0) lse[stat] = saw ? m + logf(l) : -INFINITY;
+}
+
+// o and lse from the pieces of a split key axis, joined in order.  One wavefront per row.
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(Attn a, float* o, float* lse, const float* part, const float2* part_ml, int splits) {
+    const long rows = (long)a.B * a.H * a.Tq, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63, query = (int)(row % a.Tq);
+    const long head = row / a.Tq;
+    const int b = (int)(head / a.H), h = (int)(head % a.H);
+    const bool valid = query < length_of(a.q_lengths, b, a.Tq);
+    float m = -INFINITY, l = 0.0f;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[s * rows + row].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float acc[2] = {0.0f, 0.0f};
+    for (int s = 0; s < splits; ++s) {
+        const float2 ml = part_ml[s * rows + row];
+        const float f = exp2f((ml.x - ref) * kLog2e);
+        l += ml.y * f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+            if (lane + 64 * c < a.D) acc[c] += part[(s * rows + row) * a.D + lane + 64 * c] * f;
+    }
+    const bool saw = valid && l != 0.0f;
+    const float inv = 1.0f / l;
+    float* out = o + b * a.q_b + h * a.q_h + query * a.q_t;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        if (lane + 64 * c < a.D) out[lane + 64 * c] = saw ? acc[c] * inv : 0.0f;
+    if (lane == 0) lse[row] = saw ? m + logf(l) : -INFINITY;
+}
+
+// ---------------------------------------------------------------- backward: queries
+
+// gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.
+template <int DP, bool BIAS, bool DROP>
+__global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(Attn a, const float* o, const float* lse, const float* go, float* gq, float* delta,
+                                                                 float* part_table, int tiles) {
+    extern __shared__ float lds[];
+    float *kt = lds, *vt = kt + kAttnRows * (DP + 4), *win = vt + kAttnRows * (DP + 4);
+    const int window = BIAS ? bias_window(a.rule) : 0;
+    float* diag = win + window;      // [wavefront][half][window]: sums of ds by relative position
+    const Where w = where(a, tiles);
+    const int q0 = w.tile * kAttnCols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qw = q0 + wave * 32, query = qw + (lane & 31);
+    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
+    const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
+    const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
+    const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
+    if (BIAS) {
+        fill_bias(a, w.h, win);
+        for (int s = threadIdx.x; s < 8 * window; s += kAttnThreads) diag[s] = 0.0f;
+    }
+    int last = k_end;
+    if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
+    if (q0 >= q_end) last = 0;
+    const bool valid = query < q_end;
+    const long stat = ((long)w.b * a.H + w.h) * a.Tq + query;
+    float qreg[DP / 2], greg[DP / 2];
+    column_load<DP>(qreg, a.q + qrow, valid, a.D, a.scale);
+    column_load<DP>(greg, go + qrow, valid, a.D, 1.0f);
+    float dl = 0.0f;
+    {
+        float oreg[DP / 2];
+        column_load<DP>(oreg, o + qrow, valid, a.D, 1.0f);
+#pragma unroll
+        for (int i = 0; i < DP / 2; ++i) dl += oreg[i] * greg[i];
+        dl += other_half(dl);
+    }
+    if (query < a.Tq && lane < 32) delta[stat] = dl;
+    float row_lse = valid ? lse[stat] : INFINITY;
+    if (row_lse == -INFINITY) row_lse = INFINITY;      // a row that saw nothing: every probability is 0
+    RngState rng = {};
+    unsigned long long group0 = 0;
+    if (DROP) {
+        rng = load_rng(a.rng, a.channel);
+        group0 = (unsigned long long)stat * ((a.Tk + 15) / 16) * 2 + (lane >> 5);
+    }
+    v16f acc[DP / 32] = {};
+    TileRegs<DP> kr, vr;
+    tile_load<DP>(kr, kbase, a.k_t, 0, last, a.D);
+    tile_load<DP>(vr, vbase, a.k_t, 0, last, a.D);
+    for (int j0 = 0; j0 < last; j0 += kAttnRows) {
+        __syncthreads();
+        tile_store<DP>(kr, kt);
+        tile_store<DP>(vr, vt);
+        __syncthreads();
+        if (j0 + kAttnRows < last) {
+            tile_load<DP>(kr, kbase, a.k_t, j0 + kAttnRows, last, a.D);
+            tile_load<DP>(vr, vbase, a.k_t, j0 + kAttnRows, last, a.D);
+        }
+        if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;
+        const int origin = BIAS ? bias_reach(a.rule) + clamp_origin(a.rule, j0 - qw - a.q_offset) - (lane & 31) : 0;
+        v16f s = {}, dp = {};
+        if (BIAS)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = win[origin + tile_row(r)];
+        s = product_rows<DP>(s, kt, qreg);
+        dp = product_rows<DP>(dp, vt, greg);
+        const bool edge = j0 + kAttnRows > k_end || qw + 32 > q_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset);
+        if (DROP) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                unsigned u[4];
+                random_group(rng, group0 + 2ull * (j0 / 16 + b), u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dp[8 * b + e] = random16(u, e) >= a.rate.threshold ? dp[8 * b + e] * a.rate.scale : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float p = exp2f((s[r] - row_lse) * kLog2e);
+            s[r] = edge && (!valid || hidden(a, j0 + tile_row(r), query, k_end)) ? 0.0f : p * (dp[r] - dl);
+        }
+        if (BIAS) {
+            // sums along the diagonals.  The array is this wavefront's and this half's own, lanes of a half
+            // meet different positions in one instruction, and LDS takes a wavefront's instructions in
+            // order: the order of the additions is fixed.
+            float* mine = diag + (wave * 2 + (lane >> 5)) * window + origin;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(mine + tile_row(r), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        product_cols<DP>(acc, kt, s);
+    }
+    if (query < a.Tq) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                store_scaled(gq + qrow, 32 * d + 8 * g + 4 * (lane >> 5), a.D, acc[d], g, valid, a.scale);
+    }
+    if (BIAS) {
+        __syncthreads();
+        for (int s = threadIdx.x; s < window; s += kAttnThreads) {
+            float sum = diag[s];
+            for (int i = 1; i < 8; ++i) sum += diag[i * window + s];
+            win[s] = sum;
+        }
+        __syncthreads();
+        const int reach = bias_reach(a.rule);
+        for (int s = threadIdx.x; s < window; s += kAttnThreads) diag[s] = (float)bucket_of(a.rule, s - reach);
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.rule.buckets; c += kAttnThreads) {
+            float sum = 0.0f;
+            for (int s = 0; s < window; ++s)
+                if (diag[s] == (float)c) sum += win[s];
+            part_table[(((long)w.b * tiles + w.tile) * a.H + w.h) * a.rule.buckets + c] = sum;
+        }
+    }
+}
+
+// gtable[c][h] = the partial rows of head h added up in order.
+__global__ __launch_bounds__(kAttnThreads) void attn_table_kernel(const float* part, int parts, int H, int buckets, float* gtable) {
+    __shared__ float join[kAttnThreads];
+    const int at = blockIdx.x * 16 + (threadIdx.x & 15), n = H * buckets, group = threadIdx.x >> 4;
+    float s = 0.0f;
+    if (at < n)
+        for (int p = group; p < parts; p += 16) s += part[(long)p * n + at];
+    join[threadIdx.x] = s;
+    __syncthreads();
+    if (group == 0 && at < n) {
+        for (int g = 1; g < 16; ++g) s += join[g * 16 + threadIdx.x];
+        gtable[(at % buckets) * H + at / buckets] = s;
+    }
+}
+
+// ---------------------------------------------------------------- backward: keys
+
+template <int DP, bool BIAS, bool DROP>
+__global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(Attn a, const float* lse, const float* delta, const float* go, float* gk, float* gv, int tiles) {
+    extern __shared__ float lds[];
+    float *qt = lds, *gt = qt + kAttnRows * (DP + 4), *stats = gt + kAttnRows * (DP + 4), *win = stats + 2 * kAttnRows;
+    const Where w = where(a, tiles);
+    const int k0 = w.tile * kAttnCols, lane = threadIdx.x & 63, kw = k0 + (threadIdx.x >> 6) * 32, key = kw + (lane & 31);
+    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
+    const float* qbase = a.q + w.b * a.q_b + w.h * a.q_h;
+    const float* gbase = go + w.b * a.q_b + w.h * a.q_h;
+    const long krow = w.b * a.k_b + w.h * a.k_h + key * a.k_t;
+    if (BIAS) fill_bias(a, w.h, win);
+    // queries this workgroup walks: from the first that sees its first key
+    int first = 0, last = q_end;
+    if (a.causal) first = max(0, k0 - a.q_offset) / kAttnRows * kAttnRows;
+    if (k0 >= k_end) last = 0;
+    const bool valid = key < k_end;
+    float kreg[DP / 2], vreg[DP / 2];
+    column_load<DP>(kreg, a.k + krow, valid, a.D, a.scale);
+    column_load<DP>(vreg, a.v + krow, valid, a.D, 1.0f);
+    const long stat0 = ((long)w.b * a.H + w.h) * a.Tq;
+    RngState rng = {};
+    if (DROP) rng = load_rng(a.rng, a.channel);
+    v16f acck[DP / 32] = {}, accv[DP / 32] = {};
+    TileRegs<DP> qr, gr;
+    tile_load<DP>(qr, qbase, a.q_t, first, last, a.D);
+    tile_load<DP>(gr, gbase, a.q_t, first, last, a.D);
+    for (int i0 = first; i0 < last; i0 += kAttnRows) {
+        __syncthreads();
+        tile_store<DP>(qr, qt);
+        tile_store<DP>(gr, gt);
+        if (threadIdx.x < kAttnRows) {
+            const int i = i0 + threadIdx.x;
+            const float v = i < last ? lse[stat0 + i] : INFINITY;
+            stats[threadIdx.x] = v == -INFINITY ? INFINITY : v;
+            stats[kAttnRows + threadIdx.x] = i < last ? delta[stat0 + i] : 0.0f;
+        }
+        __syncthreads();
+        if (i0 + kAttnRows < last) {
+            tile_load<DP>(qr, qbase, a.q_t, i0 + kAttnRows, last, a.D);
+            tile_load<DP>(gr, gbase, a.q_t, i0 + kAttnRows, last, a.D);
+        }
+        if (kw >= k_end || (a.causal && kw > i0 + 31 + a.q_offset)) continue;
+        v16f s = {}, dp = {};
+        if (BIAS) {
+            const float* at = win + bias_reach(a.rule) + clamp_origin(a.rule, kw - i0 - a.q_offset) + (lane & 31);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = at[-tile_row(r)];
+        }
+        s = product_rows<DP>(s, qt, kreg);
+        dp = product_rows<DP>(dp, gt, vreg);
+        const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + a.q_offset);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = tile_row(r);
+            float p = exp2f((s[r] - stats[row]) * kLog2e);
+            if (edge && hidden(a, key, i0 + row, k_end)) p = 0.0f;      // rows beyond the queries: p is 0 by their lse
+            float f = 1.0f;
+            if (DROP) {
+                unsigned u[4];
+                random_group(rng, ((unsigned long long)(stat0 + i0 + row) * ((a.Tk + 15) / 16) + (key >> 4)) * 2 + (key >> 2 & 1), u);
+                const int e = (key & 3) + 4 * (key >> 3 & 1);
+                const unsigned word = (e >> 1) == 0 ? u[0] : (e >> 1) == 1 ? u[1] : (e >> 1) == 2 ? u[2] : u[3];
+                f = ((e & 1) ? word >> 16 : word & 0xffffu) >= a.rate.threshold ? a.rate.scale : 0.0f;
+            }
+            s[r] = p * f;
+            dp[r] = p * (dp[r] * f - stats[kAttnRows + row]);
+        }
+        product_cols<DP>(accv, gt, s);
+        product_cols<DP>(acck, qt, dp);
+    }
+    if (key >= a.Tk) return;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * d + 8 * g + 4 * (lane >> 5);
+            store_scaled(gk + krow, c, a.D, acck[d], g, valid, a.scale);
+            store_scaled(gv + krow, c, a.D, accv[d], g, valid, 1.0f);
+        }
+}
+
+// ---------------------------------------------------------------- launchers
+
+// Chooses the instantiation: head width rounded up, bias, dropout.
+#define ATTN_DISPATCH(KERNEL, ...)                                                          \
+    do {                                                                                    \
+        const bool bias_ = a.table != nullptr, drop_ = a.rate.threshold != 0;               \
+        if (a.D <= 32) ATTN_FLAGS(KERNEL, 32, __VA_ARGS__);                                 \
+        else if (a.D <= 64) ATTN_FLAGS(KERNEL, 64, __VA_ARGS__);                            \
+        else ATTN_FLAGS(KERNEL, 128, __VA_ARGS__);                                          \
+    } while (0)
+#define ATTN_FLAGS(KERNEL, DP, ...)                                                         \
+    do {                                                                                    \
+        if (bias_ && drop_) ATTN_LAUNCH((KERNEL<DP, true, true>), __VA_ARGS__);             \
+        else if (bias_) ATTN_LAUNCH((KERNEL<DP, true, false>), __VA_ARGS__);                \
+        else if (drop_) ATTN_LAUNCH((KERNEL<DP, false, true>), __VA_ARGS__);                \
+        else ATTN_LAUNCH((KERNEL<DP, false, false>), __VA_ARGS__);                          \
+    } while (0)
+#define ATTN_LAUNCH(KERNEL, ...)                                                            \
+    do {                                                                                    \
+        if (lds_bytes > 65536)                                                              \
+            CGT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes)); \
+        KERNEL<<<grid, kAttnThreads, lds_bytes, st>>>(__VA_ARGS__);                         \
+    } while (0)
+
+static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+// The rule of the buckets: per side (all of them, or half when positions after the query have their
+// own) the first half one distance each, then logarithmic up to max_distance.  Bucket e of the
+// logarithmic part begins at the smallest n with (n / first)^(side - first) >= (max / first)^e; the
+// logarithms are compared in double with a slack far below the gap between whole distances, so that
+// the exact ties of the rule (first 8, max 128: at 16, 32, 64) fall where the real numbers say.
+static int bucket_rule(const char* what, int buckets, int bidirectional, int max_distance, BucketRule* r) {
+    CGT_ARG_CHECK(buckets >= (bidirectional ? 4 : 2) && buckets <= kMaxBuckets && (!bidirectional || buckets % 2 == 0),
+                  "%s: %d buckets (%s, and %d at most)", what, buckets,
+                  bidirectional ? "an even number, 4 at least, where positions after the query have their own" : "2 at least", kMaxBuckets);
+    r->buckets = buckets;
+    r->bidirectional = bidirectional != 0;
+    r->max_distance = max_distance;
+    r->side = bidirectional ? buckets / 2 : buckets;
+    r->first = r->side / 2;
+    CGT_ARG_CHECK(max_distance > r->first && max_distance <= kMaxDistance, "%s: max_distance %d must be above %d and at most %d", what, max_distance,
+                  r->first, kMaxDistance);
+    const int logs = r->side - r->first;
+    int n = r->first;
+    for (int e = 1; e < logs; ++e) {
+        const double want = e * std::log((double)max_distance / r->first);
+        while (n < max_distance && logs * std::log((double)n / r->first) < want - 1e-11) ++n;
+        r->edge[e] = n;
+    }
+    return CGT_AMD_OK;
+}
+
+static int attn_setup(const char* what, Attn* a, long B, long H, long Tq, long Tk, long D, int layout, const float* table, long buckets,
+                      int bidirectional, long max_distance, double scale, int causal, long q_offset, double p, const long long* rng, unsigned channel) {
+    CGT_ARG_CHECK(B >= 0 && H >= 0 && Tq >= 0 && Tk >= 0, "%s: negative extent", what);
+    CGT_ARG_CHECK(D >= 1 && D <= 128, "%s: heads of %ld columns (1 to 128)", what, D);
+    CGT_ARG_CHECK(Tq < (1L << 29) && Tk < (1L << 29) && q_offset > -(1L << 29) && q_offset < (1L << 29), "%s: lengths and offset must be below 2^29", what);
+    CGT_ARG_CHECK(B * H < (1L << 22) && B < (1L << 22) && H < (1L << 22), "%s: too many heads", what);
+    CGT_ARG_CHECK(layout == 0 || layout == 1, "%s: layout %d (0: heads before positions, 1: after them)", what, layout);
+    CGT_ARG_CHECK(std::isfinite(scale), "%s: scale must be finite", what);
+    if (!dropout_rate(p, what, &a->rate)) return CGT_AMD_ERR_ARG;
+    CGT_ARG_CHECK(rng || a->rate.threshold == 0, "%s: dropout needs the generator's state", what);
+    a->table = table;
+    if (table) {
+        if (int rc = bucket_rule(what, (int)std::min(buckets, 1L << 20), bidirectional, (int)std::min(max_distance, 1L << 20), &a->rule)) return rc;
+    }
+    a->B = (int)B, a->H = (int)H, a->Tq = (int)Tq, a->Tk = (int)Tk, a->D = (int)D;
+    a->causal = causal != 0, a->q_offset = (int)q_offset, a->scale = (float)scale, a->rng = rng, a->channel = channel;
+    a->q_b = H * Tq * D, a->k_b = H * Tk * D;
+    a->q_h = layout ? D : Tq * D, a->k_h = layout ? D : Tk * D;
+    a->q_t = a->k_t = layout ? H * D : D;
+    return CGT_AMD_OK;
+}
+
+}  // namespace cgt_amd
+
+using namespace cgt_amd;
+
+CGT_API int cgt_amd_rel_bucket(long rel, int buckets, int bidirectional, int max_distance) {
+    BucketRule r;
+    if (bucket_rule("rel_bucket", buckets, bidirectional, max_distance, &r)) return -1;
+    const long lim = 2L * kMaxDistance;
+    return bucket_of(r, (int)std::max(-lim, std::min(lim, rel)));
+}
+
+CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const float* v, const float* table, long B, long H, long Tq, long Tk, long D,
+                                          int layout, long buckets, int bidirectional, long max_distance, double scale, int causal, long q_offset,
+                                          const int* q_lengths, const int* k_lengths, double p, const long long* rng, unsigned channel,
+                                          float* o, float* lse, void* stream) {
+    Attn a = {};
+    if (int rc = attn_setup("attention", &a, B, H, Tq, Tk, D, layout, table, buckets, bidirectional, max_distance, scale, causal, q_offset, p, rng, channel))
+        return rc;
+    if (B * H * Tq == 0) return CGT_AMD_OK;
+    CGT_ARG_CHECK(q && o && lse && (Tk == 0 || (k && v)), "attention: null pointer");
+    a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths;
+    hipStream_t st = as_stream(stream);
+    const int DP = padded_dim(a.D), tiles = (int)cdiv(Tq, kAttnCols);
+    const long heads = B * H, whole = heads * tiles;
+    // too few blocks of queries to fill the chip: the keys are cut too, into runs of 128 at least
+    const int splits = whole >= kNumCU ? 1 : (int)std::max(1L, std::min({cdiv(2L * kNumCU, whole), Tk / 128, 64L}));
+    CGT_ARG_CHECK(whole * splits < (1L << 31), "attention: too many workgroups");
+    float* part = nullptr;
+    float2* ml = nullptr;
+    if (splits > 1) {
+        const size_t rows = (size_t)heads * Tq * splits;
+        part = stream_workspace(stream, kWsAttention, rows * (D + 2) * sizeof(float), "attention");
+        if (!part) return CGT_AMD_ERR_NOMEM;
+        ml = reinterpret_cast<float2*>(part);      // first, for its alignment
+        part += 2 * rows;
+    }
+    const size_t lds_bytes = (2 * kAttnRows * (DP + 4) + (table ? bias_window(a.rule) : 0)) * sizeof(float);
+    const dim3 grid((unsigned)(whole * splits));
+    ATTN_DISPATCH(attn_fwd_kernel, a, o, lse, part, ml, tiles, splits);
+    CGT_LAUNCH_CHECK("attention forward");
+    if (splits > 1) {
+        attn_join_kernel<<<dim3((unsigned)cdiv(heads * Tq, 4)), kAttnThreads, 0, st>>>(a, o, lse, part, ml, splits);
+        CGT_LAUNCH_CHECK("attention join");
+    }
+    return CGT_AMD_OK;
+}
+
+CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const float* v, const float* table, const float* o, const float* lse,
+                                          const float* go, long B, long H, long Tq, long Tk, long D, int layout, long buckets, int bidirectional,
+                                          long max_distance, double scale, int causal, long q_offset, const int* q_lengths, const int* k_lengths,
+                                          double p, const long long* rng, unsigned channel, float* gq, float* gk, float* gv, float* gtable, void* stream) {
+    Attn a = {};
+    if (int rc = attn_setup("attention backward", &a, B, H, Tq, Tk, D, layout, table, buckets, bidirectional, max_distance, scale, causal, q_offset, p, rng,
+                            channel))
+        return rc;
+    CGT_ARG_CHECK(!table || gtable, "attention backward: null pointer");
+    const long heads = B * H;
+    if (heads == 0 || (Tq == 0 && Tk == 0) || Tq == 0) {
+        if (table)
+            if (int rc = cgt_amd_fill_u32(gtable, 0u, buckets * H, stream)) return rc;
+        if (heads * Tk == 0) return CGT_AMD_OK;
+        CGT_ARG_CHECK(gk && gv, "attention backward: null pointer");
+        if (int rc = cgt_amd_fill_u32(gk, 0u, heads * Tk * D, stream)) return rc;
+        return cgt_amd_fill_u32(gv, 0u, heads * Tk * D, stream);
+    }
+    CGT_ARG_CHECK(q && o && lse && go && gq && (Tk == 0 || (k && v && gk && gv)), "attention backward: null pointer");
+    a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths;
+    hipStream_t st = as_stream(stream);
+    const int DP = padded_dim(a.D), qtiles = (int)cdiv(Tq, kAttnCols), ktiles = (int)cdiv(Tk, kAttnCols);
+    CGT_ARG_CHECK(heads * qtiles < (1L << 31) && heads * ktiles < (1L << 31), "attention backward: too many workgroups");
+    const long parts = B * qtiles;
+    const size_t need = (size_t)(heads * Tq + (table ? parts * H * buckets : 0)) * sizeof(float);
+    float* delta = stream_workspace(stream, kWsAttention, need, "attention backward");
+    if (!delta) return CGT_AMD_ERR_NOMEM;
+    float* part = delta + heads * Tq;
+    const int window = table ? bias_window(a.rule) : 0;
+    {
+        const size_t lds_bytes = (2 * kAttnRows * (DP + 4) + 9 * window) * sizeof(float);
+        const dim3 grid((unsigned)(heads * qtiles));
+        ATTN_DISPATCH(attn_bwd_q_kernel, a, o, lse, go, gq, delta, part, qtiles);
+        CGT_LAUNCH_CHECK("attention backward (queries)");
+    }
+    if (table) {
+        attn_table_kernel<<<dim3((unsigned)cdiv(H * buckets, 16)), kAttnThreads, 0, st>>>(part, (int)parts, a.H, a.rule.buckets, gtable);
+        CGT_LAUNCH_CHECK("attention backward (table)");
+    }
+    if (ktiles) {
+        const size_t lds_bytes = (2 * kAttnRows * (DP + 4) + 2 * kAttnRows + window) * sizeof(float);
+        const dim3 grid((unsigned)(heads * ktiles));
+        ATTN_DISPATCH(attn_bwd_kv_kernel, a, lse, delta, go, gk, gv, ktiles);
+        CGT_LAUNCH_CHECK("attention backward (keys)");
+    }
+    return CGT_AMD_OK;
+}

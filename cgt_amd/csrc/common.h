@@ -23,7 +23,7 @@ inline hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
 // HIP graph may have its address baked in), with the stream (cgt_amd_stream_destroy).
 // Growth while the stream is being captured is refused (an allocation would break the
 // capture): returns nullptr with the message set.
-enum WorkspaceUser { kWsGemm = 0, kWsSum = 1, kWsConvFilter = 2, kWsConvTable = 3, kWsConvData = 4, kWsNorm = 5, kWsUsers = 6 };
+enum WorkspaceUser { kWsGemm = 0, kWsSum = 1, kWsConvFilter = 2, kWsConvTable = 3, kWsConvData = 4, kWsNorm = 5, kWsAttention = 6, kWsUsers = 7 };
 float* stream_workspace(void* stream, WorkspaceUser user, size_t bytes, const char* what);
 void release_stream_workspaces(void* stream);
 

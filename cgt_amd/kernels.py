@@ -295,6 +295,75 @@ def dropout_add_layer_norm_bwd(h, gamma, mean, rstd, gy, gh=None, p=0.0, rng=Non
     return gx, gres, ggamma, gbeta
 
 
+# ---------------------------------------------------------------- attention with a relative position bias
+
+def rel_bucket(rel, buckets, bidirectional, max_distance):
+    """Bucket of a relative position (key minus query), the rule include/cgt_amd.h states."""
+    b = capi.lib().cgt_amd_rel_bucket(int(rel), int(buckets), int(bool(bidirectional)), int(max_distance))
+    if b < 0:
+        raise ValueError(capi.last_error())
+    return b
+
+
+def _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_offset, q_lengths, k_lengths, p, rng, channel, layout):
+    """Checks the operands both directions share; returns (leading dims B, H, Tq, Tk, D, and the C arguments behind them)."""
+    _f32(q, k, v)
+    if layout not in ("bhtd", "bthd"):
+        raise ValueError("layout is 'bhtd' or 'bthd' (got %r)" % (layout,))
+    if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape:
+        raise ValueError("attention takes q, k and v of four axes, k and v of one shape (got %s, %s, %s)" % (q.shape, k.shape, v.shape))
+    t = 2 if layout == "bhtd" else 1
+    B, H, Tq, D = q.shape[0], q.shape[3 - t], q.shape[t], q.shape[3]
+    Tk = k.shape[t]
+    if (k.shape[0], k.shape[3 - t], k.shape[3]) != (B, H, D):
+        raise ValueError("q %s and k %s differ in batch, heads or head width" % (q.shape, k.shape))
+    buckets = 0
+    if table is not None:
+        _f32(table)
+        if table.ndim != 2 or table.shape[1] != H:
+            raise ValueError("the bias table %s must be [buckets, %d heads]" % (table.shape, H))
+        buckets = table.shape[0]
+    for n, name in ((q_lengths, "q_lengths"), (k_lengths, "k_lengths")):
+        if n is not None and (n.dtype != np.int32 or n.shape != (B,)):
+            raise ValueError("%s must be an int32 array of %d elements" % (name, B))
+    if bidirectional is None:
+        bidirectional = not causal
+    if scale is None:
+        scale = D ** -0.5 if D else 1.0
+    ptr = lambda x: None if x is None else x.ptr      # noqa: E731
+    return (B, H, Tq, Tk, D, int(layout == "bthd"), buckets, int(bool(bidirectional)), int(max_distance), float(scale),
+            int(bool(causal)), int(q_offset), ptr(q_lengths), ptr(k_lengths), float(p), _rng(rng, p), _channel(channel))
+
+
+def rel_attention_fwd(q, k, v, table=None, scale=None, causal=False, bidirectional=None, max_distance=128, q_offset=0,
+                      q_lengths=None, k_lengths=None, p=0.0, rng=None, channel=0, layout="bhtd", out=None, stream=None):
+    """softmax(scale * q k^T + table[bucket(key - query position)]) v per batch item and head, with dropout of the
+    softmax's values: returns (o, lse).  q [B,H,Tq,D] and k, v [B,H,Tk,D] (layout "bthd": [B,T,H,D]); table
+    [buckets, H] or None.  scale is D^-1/2 and bidirectional is `not causal` unless given; include/cgt_amd.h states
+    the rule of the buckets, of the lengths and of the generator."""
+    args = _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_offset, q_lengths, k_lengths, p, rng, channel, layout)
+    o, lse = (_out(a, s) for a, s in zip(out or (None, None), (q.shape, args[:3])))
+    capi.check(capi.lib().cgt_amd_rel_attention_fwd_f32(q.ptr, k.ptr, v.ptr, None if table is None else table.ptr, *args, o.ptr, lse.ptr, stream))
+    return o, lse
+
+
+def rel_attention_bwd(q, k, v, table, o, lse, go, scale=None, causal=False, bidirectional=None, max_distance=128, q_offset=0,
+                      q_lengths=None, k_lengths=None, p=0.0, rng=None, channel=0, layout="bhtd", out=None, stream=None):
+    """The gradients of rel_attention_fwd from the cotangent of o, given its results: returns (gq, gk, gv, gtable),
+    gtable None without a table."""
+    args = _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_offset, q_lengths, k_lengths, p, rng, channel, layout)
+    _f32(o, lse, go)
+    if o.shape != q.shape or go.shape != q.shape or lse.shape != args[:3]:
+        raise ValueError("results %s, %s and cotangent %s do not fit q %s" % (o.shape, lse.shape, go.shape, q.shape))
+    shapes = [q.shape, k.shape, v.shape] + ([table.shape] if table is not None else [])
+    outs = [_out(a, s) for a, s in zip(out or (None,) * 4, shapes)]
+    gtable = outs[3] if table is not None else None
+    capi.check(capi.lib().cgt_amd_rel_attention_bwd_f32(
+        q.ptr, k.ptr, v.ptr, None if table is None else table.ptr, o.ptr, lse.ptr, go.ptr, *args, outs[0].ptr, outs[1].ptr, outs[2].ptr,
+        None if gtable is None else gtable.ptr, stream))
+    return outs[0], outs[1], outs[2], gtable
+
+
 # ---------------------------------------------------------------- conv-layer glue
 
 UNARY_OPS = ["abs", "cos", "exp", "log", "neg", "sign", "sin", "square", "sqrt", "tanh", "sigmoid"]

@@ -20,6 +20,7 @@ conv_algo("im2col") keeps the literal composition, every op on the GPU.
 from . import core
 from .nn_ops import conv_col, conv_same
 from .nn_ops import cross_channel_lrn as _lrn
+from .nn_ops.attention import relative_attention  # noqa: F401
 from .nn_ops.cross_channel_lrn import cross_channel_lrn  # noqa: F401
 from .nn_ops.dropout import dropout, rng_state  # noqa: F401
 from .nn_ops.im2col import im2col

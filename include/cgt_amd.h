@@ -342,6 +342,62 @@ int cgt_amd_dropout_add_layer_norm_bwd_f32(const float *h, const float *gamma, c
                                            float *gx, float *gresidual, float *ggamma, float *gbeta,
                                            void *stream);
 
+/* ---------------------------------------------------------------- attention with a relative position bias
+ *
+ * For every batch item and head (no counterpart in the reference):
+ *   s[i][j] = scale * q[i] . k[j] + table[bucket(j - i - q_offset)][head]
+ *   o[i] = sum_j softmax_j(s[i])[j] * v[j],  lse[i] = log sum_j exp(s[i][j])
+ * over the keys j that query i may see: j < k_lengths[b] and, if causal,
+ * j <= i + q_offset (q_offset is the position of the first query among the
+ * keys: Tk - Tq where new tokens meet a cache).  The scores are never stored.
+ *
+ * q, o are [B][H][Tq][D] (layout 0) or [B][Tq][H][D] (layout 1), k, v the same
+ * with Tk, fp32; lse is [B][H][Tq].  1 <= D <= 128; lengths and |q_offset|
+ * below 2^29; B * H below 2^22.
+ *
+ * table [buckets][H] (NULL: no bias) is the learned bias, one value per bucket
+ * and head.  Relative positions (key minus query) fall into buckets: with
+ * bidirectional != 0 the second half of the buckets is for keys after the
+ * query and |rel| counts, otherwise all keys after the query share the bucket
+ * of distance 0.  Of the n buckets of a side the first n / 2 hold one distance
+ * each and the others divide [n / 2, max_distance) logarithmically; the last
+ * holds everything beyond.  buckets <= 256, max_distance <= 1024.
+ *
+ * q_lengths, k_lengths (int32 [B], NULL: full; clamped to [0, T]) describe a
+ * padded batch.  What lies behind them in q, k, v and go is not read; such rows
+ * of o, gq, gk, gv are 0.  A query that sees no key (or only scores of -inf)
+ * has o = 0 and lse = -inf and contributes to no gradient.
+ *
+ * p is the dropout probability of the softmax's values, from the generator
+ * described above (rng, channel; rng may be NULL if p rounds to 0): row
+ * r = (b * H + h) * Tq + i owns 2 * ceil(Tk / 16) groups, and key j takes number
+ * (j & 3) + 4 * (j >> 3 & 1) of group 2 * (r * ceil(Tk / 16) + j / 16) + (j >> 2 & 1).
+ *
+ * Uses workspaces owned by the library.  Sums run in a fixed order: same input,
+ * same bits.  Inputs and outputs must not overlap. */
+
+/* Bucket of a relative position under that rule (host only); -1 and an error
+ * for a rule that is refused. */
+int cgt_amd_rel_bucket(long rel, int buckets, int bidirectional, int max_distance);
+
+int cgt_amd_rel_attention_fwd_f32(const float *q, const float *k, const float *v, const float *table,
+                                  long B, long H, long Tq, long Tk, long D, int layout, long buckets,
+                                  int bidirectional, long max_distance, double scale, int causal,
+                                  long q_offset, const int *q_lengths, const int *k_lengths, double p,
+                                  const long long *rng, unsigned channel, float *o, float *lse,
+                                  void *stream);
+
+/* The gradients from go, the cotangent of o, given what the forward call left
+ * in o and lse (same arguments otherwise).  gtable [buckets][H] is the sum over
+ * the batch and all pairs of a bucket; NULL without a table. */
+int cgt_amd_rel_attention_bwd_f32(const float *q, const float *k, const float *v, const float *table,
+                                  const float *o, const float *lse, const float *go, long B, long H,
+                                  long Tq, long Tk, long D, int layout, long buckets, int bidirectional,
+                                  long max_distance, double scale, int causal, long q_offset,
+                                  const int *q_lengths, const int *k_lengths, double p,
+                                  const long long *rng, unsigned channel, float *gq, float *gk, float *gv,
+                                  float *gtable, void *stream);
+
 /* ---------------------------------------------------------------- GEMM */
 
 /* Row-major C[M,N] = op(A) . op(B), alpha = 1, beta = 0, true fp32 (MFMA

@@ -137,3 +137,57 @@ def test_views_of_other_libraries_arrays_are_checked():
         gpuarray.as_gpuarray(Foreign(data=(0, False)))
     with pytest.raises(ValueError):
         gpuarray.as_gpuarray(Foreign(data=(4097, False)))
+
+
+@pytest.mark.parametrize("bidirectional", [False, True])
+def test_buckets_follow_the_rule_in_whole_numbers(bidirectional):
+    from cgt_amd import kernels as K
+    for buckets in (4, 6, 8, 16, 32, 64, 100, 256):
+        for max_distance in (3, 5, 16, 20, 64, 100, 128, 200, 500, 1000, 1024):
+            first = buckets // (4 if bidirectional else 2)
+            if max_distance <= first:
+                with pytest.raises(ValueError):
+                    K.rel_bucket(0, buckets, bidirectional, max_distance)
+                continue
+            for rel in list(range(-140, 141, 1 if max_distance == 128 else 3)) + [-255, -256, -257, -511, -512, -513, -1024, -(10 ** 12), 999, 10 ** 12]:
+                assert K.rel_bucket(rel, buckets, bidirectional, max_distance) == T.bucket(rel, buckets, max_distance, bidirectional), \
+                    (rel, buckets, max_distance)
+    for bad in ((1, False, 128), (2, True, 128), (7, True, 128), (258, False, 1024), (8, True, 1025), (8, True, 2)):
+        with pytest.raises(ValueError):
+            K.rel_bucket(0, *bad)
+
+
+def test_attention_refusals():
+    from cgt_amd import capi, kernels as K
+    q, k, lse, table, rng = _fake((2, 3, 4, 8)), _fake((2, 3, 6, 8)), _fake((2, 3, 4)), _fake((8, 3)), _fake((2,), np.int64)
+    out = (q, lse)
+    for bad in [dict(k=_fake((2, 3, 6, 9))), dict(k=_fake((2, 4, 6, 8))), dict(k=_fake((1, 3, 6, 8))), dict(v=_fake((2, 3, 7, 8))),
+                dict(q=_fake((2, 3, 8))), dict(table=_fake((8, 4))), dict(table=_fake((8,))), dict(q_lengths=_fake((3,), np.int32)),
+                dict(k_lengths=_fake((2,), np.int64)), dict(layout="thbd"), dict(channel=-1), dict(p=0.5), dict(out=(q, _fake((2, 3, 5))))]:
+        args = dict(dict(q=q, k=k, v=bad.get("k", k), table=table, out=out), **bad)
+        with pytest.raises((ValueError, TypeError)):
+            K.rel_attention_fwd(**args)
+    with pytest.raises(TypeError):
+        K.rel_attention_fwd(q, k, k, _fake((8, 3), np.int32), out=out)
+    with pytest.raises(TypeError):
+        K.rel_attention_fwd(q, k, k, table, p=0.5, rng=_fake((2,), np.int32), out=out)
+    for bad in [dict(max_distance=2), dict(max_distance=1025), dict(table=_fake((7, 3))), dict(table=_fake((258, 3))), dict(p=1.0, rng=rng),
+                dict(p=-0.5, rng=rng), dict(scale=float("nan")), dict(q_offset=1 << 30), dict(q_offset=-(1 << 40))]:
+        args = dict(dict(q=q, k=k, v=k, table=table, out=out), **bad)
+        with pytest.raises(capi.CgtAmdError):
+            K.rel_attention_fwd(**args)
+    wide = _fake((1, 1, 1, 129))
+    with pytest.raises(capi.CgtAmdError, match="columns"):
+        K.rel_attention_fwd(wide, wide, wide, out=(wide, _fake((1, 1, 1))))
+    for bad in [dict(o=_fake((2, 3, 5, 8))), dict(lse=_fake((2, 3, 5))), dict(go=k)]:
+        args = dict(dict(q=q, k=k, v=k, table=table, o=q, lse=lse, go=q), **bad)
+        with pytest.raises(ValueError):
+            K.rel_attention_bwd(**args)
+    lib = capi.lib()
+    rest = (0, 8, 1, 128, 0.5, 0, 0, None, None, 0.0, None, 0)
+    assert lib.cgt_amd_rel_attention_fwd_f32(None, None, None, None, 1, 1, 4, 4, 8, *rest, None, None, None) == 1 and "null" in capi.last_error()
+    assert lib.cgt_amd_rel_attention_fwd_f32(None, None, None, None, 1, 1, 0, 4, 8, *rest, None, None, None) == 0
+    assert lib.cgt_amd_rel_attention_fwd_f32(None, None, None, None, 1, 1, -1, 4, 8, *rest, None, None, None) == 1
+    assert lib.cgt_amd_rel_attention_fwd_f32(None, None, None, None, 1, 1, 1 << 29, 4, 8, *rest, None, None, None) == 1
+    assert lib.cgt_amd_rel_attention_fwd_f32(None, None, None, None, 1 << 11, 1 << 11, 4, 4, 8, *rest, None, None, None) == 1
+    assert lib.cgt_amd_rel_attention_bwd_f32(None, None, None, None, None, None, None, 1, 1, 4, 4, 8, *rest, None, None, None, None, None) == 1
