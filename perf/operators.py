@@ -383,7 +383,7 @@ def _run_own(s):
             kernels.rel_attention_fwd(a["q"], a["k"], a["v"], a["table"], **more)
         else:
             kernels.rel_attention_bwd(a["q"], a["k"], a["v"], a["table"], a["o"], a["lse"], a["go"], **more)
-    return results
+    return results if len(results) > 1 else results[0]
 
 
 def run(state):
