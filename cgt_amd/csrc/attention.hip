@@ -22,6 +22,7 @@
 #include "random.h"
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace cgt_amd {
 
@@ -339,6 +340,144 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(Attn a, float* 
     if (lane == 0) lse[row] = saw ? m + logf(l) : -INFINITY;
 }
 
+// ---------------------------------------------------------------- forward: a few queries against many keys
+
+// exp(x) of a non-positive difference of scores; below 2^-126 it is 0.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// Sum over aligned groups of N lanes (8, 16 or 32); every lane gets it.
+template <int N>
+__device__ __forceinline__ float group_sum(float x) {
+    auto add = [](float v, auto ctrl) {
+        return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    x = add(x, std::integral_constant<int, 0xB1>());       // lane ^ 1
+    x = add(x, std::integral_constant<int, 0x4E>());       // lane ^ 2
+    x = add(x, std::integral_constant<int, 0x141>());      // mirrored within 8: the other quad
+    if (N >= 16) x = add(x, std::integral_constant<int, 0x140>());      // mirrored within 16: the other eight
+    if (N >= 32) x += __shfl_xor(x, 16);
+    return x;
+}
+
+// One workgroup per head and run of keys; up to NQ queries share what is read.  DP / 4 lanes hold a
+// key's columns, so a wavefront's load covers 256 / DP neighbouring keys, and kTokenUnroll of those
+// are in flight at once.  Every group of lanes keeps a running maximum, sum and result of its own
+// keys; they are joined at the end, first in the wavefront, then through LDS, then (splits > 1) by
+// attn_join_kernel.  No matrix instructions: with a few rows the time is that of reading k and v.
+constexpr int kTokenUnroll = 4;
+template <int DP, int NQ, bool BIAS>
+__global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float* o, float* lse, float* part, float2* part_ml, int splits) {
+    constexpr int LANES = DP / 4, GROUPS = kWave / LANES, STEP = GROUPS * kTokenUnroll;      // keys per wavefront and trip
+    extern __shared__ float win[];
+    __shared__ float4 join_o[NQ][4][LANES];
+    __shared__ float2 join_ml[NQ][4];
+    const Where w = where(a, splits);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % LANES * 4, group = lane / LANES, split = w.tile;
+    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
+    int last = k_end;
+    if (a.causal) last = min(last, max(0, a.Tq + a.q_offset));
+    if (q_end == 0) last = 0;
+    const int run = (last + 4 * STEP * splits - 1) / (4 * STEP * splits) * 4 * STEP;
+    const int first = split * run;
+    last = min(last, first + run);
+    if (BIAS && first < last) fill_bias(a, w.h, win);
+    const int reach = BIAS ? bias_reach(a.rule) : 0;
+    __syncthreads();
+    const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
+    const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
+    float4 q[NQ], acc[NQ];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        q[i] = i < q_end ? load4(a.q + w.b * a.q_b + w.h * a.q_h + i * a.q_t, c, a.D) : make_float4(0, 0, 0, 0);
+        q[i] = make_float4(q[i].x * a.scale, q[i].y * a.scale, q[i].z * a.scale, q[i].w * a.scale);
+        acc[i] = make_float4(0, 0, 0, 0);
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+    }
+    for (int j0 = first + wave * STEP; j0 < last; j0 += 4 * STEP) {
+        float4 kv[kTokenUnroll], vv[kTokenUnroll];
+#pragma unroll
+        for (int u = 0; u < kTokenUnroll; ++u) {
+            const int j = j0 + u * GROUPS + group;
+            kv[u] = j < last ? load4(kbase + j * a.k_t, c, a.D) : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < kTokenUnroll; ++u) {
+            const int j = j0 + u * GROUPS + group;
+            vv[u] = j < last ? load4(vbase + j * a.k_t, c, a.D) : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            float s[kTokenUnroll], top = m[i];
+#pragma unroll
+            for (int u = 0; u < kTokenUnroll; ++u) {
+                const int j = j0 + u * GROUPS + group;
+                s[u] = group_sum<LANES>(kv[u].x * q[i].x + kv[u].y * q[i].y + (kv[u].z * q[i].z + kv[u].w * q[i].w));
+                if (BIAS) s[u] += win[reach + max(-reach, min(reach, j - i - a.q_offset))];
+                if (j >= last || (a.causal && j > i + a.q_offset)) s[u] = -INFINITY;
+                top = fmaxf(top, s[u]);
+            }
+            const float ref = top == -INFINITY ? 0.0f : top, f = exp_of(m[i] - ref);
+            m[i] = top;
+            l[i] *= f;
+            acc[i] = make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f);
+#pragma unroll
+            for (int u = 0; u < kTokenUnroll; ++u) {
+                const float p = exp_of(s[u] - ref);
+                l[i] += p;
+                acc[i] = make_float4(acc[i].x + p * vv[u].x, acc[i].y + p * vv[u].y, acc[i].z + p * vv[u].z, acc[i].w + p * vv[u].w);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        float top = m[i];
+#pragma unroll
+        for (int d = LANES; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float f = exp_of(m[i] - (top == -INFINITY ? 0.0f : top));
+        l[i] *= f;
+        acc[i] = make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f);
+#pragma unroll
+        for (int d = LANES; d < kWave; d <<= 1) {
+            l[i] += __shfl_xor(l[i], d);
+            acc[i].x += __shfl_xor(acc[i].x, d);
+            acc[i].y += __shfl_xor(acc[i].y, d);
+            acc[i].z += __shfl_xor(acc[i].z, d);
+            acc[i].w += __shfl_xor(acc[i].w, d);
+        }
+        if (group == 0) join_o[i][wave][lane] = acc[i];
+        if (lane == 0) join_ml[i][wave] = make_float2(top, l[i]);
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < NQ * LANES; t += kAttnThreads) {
+        const int i = t / LANES, col = t % LANES;
+        if (i >= a.Tq) continue;
+        float top = -INFINITY, sum = 0.0f;
+        for (int o4 = 0; o4 < 4; ++o4) top = fmaxf(top, join_ml[i][o4].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 r = make_float4(0, 0, 0, 0);
+        for (int o4 = 0; o4 < 4; ++o4) {
+            const float f = exp_of(join_ml[i][o4].x - ref);
+            const float4 v = join_o[i][o4][col];
+            sum += join_ml[i][o4].y * f;
+            r = make_float4(r.x + v.x * f, r.y + v.y * f, r.z + v.z * f, r.w + v.w * f);
+        }
+        const long stat = ((long)w.b * a.H + w.h) * a.Tq + i;
+        if (splits > 1) {
+            const long row = (long)split * a.B * a.H * a.Tq + stat;
+            store4(part + row * a.D, col * 4, a.D, r.x, r.y, r.z, r.w);
+            if (col == 0) part_ml[row] = make_float2(top, sum);
+        } else {
+            const bool saw = i < q_end && sum != 0.0f;
+            const float inv = 1.0f / sum;
+            store4(o + w.b * a.q_b + w.h * a.q_h + i * a.q_t, col * 4, a.D, saw ? r.x * inv : 0.0f, saw ? r.y * inv : 0.0f, saw ? r.z * inv : 0.0f,
+                   saw ? r.w * inv : 0.0f);
+            if (col == 0) lse[stat] = saw ? top + logf(sum) : -INFINITY;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- backward: queries
 
 // gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.
@@ -572,6 +711,20 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(Attn a, const
         else if (drop_) ATTN_LAUNCH((KERNEL<DP, false, true>), __VA_ARGS__);                \
         else ATTN_LAUNCH((KERNEL<DP, false, false>), __VA_ARGS__);                          \
     } while (0)
+// The same for a few queries: one or up to four of them.
+#define ATTN_TOKEN(...)                                                                     \
+    do {                                                                                    \
+        if (a.D <= 32) ATTN_TOKEN_FLAGS(32, __VA_ARGS__);                                   \
+        else if (a.D <= 64) ATTN_TOKEN_FLAGS(64, __VA_ARGS__);                              \
+        else ATTN_TOKEN_FLAGS(128, __VA_ARGS__);                                            \
+    } while (0)
+#define ATTN_TOKEN_FLAGS(DP, ...)                                                           \
+    do {                                                                                    \
+        if (table && a.Tq == 1) ATTN_LAUNCH((attn_token_kernel<DP, 1, true>), __VA_ARGS__); \
+        else if (table) ATTN_LAUNCH((attn_token_kernel<DP, 4, true>), __VA_ARGS__);         \
+        else if (a.Tq == 1) ATTN_LAUNCH((attn_token_kernel<DP, 1, false>), __VA_ARGS__);    \
+        else ATTN_LAUNCH((attn_token_kernel<DP, 4, false>), __VA_ARGS__);                   \
+    } while (0)
 #define ATTN_LAUNCH(KERNEL, ...)                                                            \
     do {                                                                                    \
         if (lds_bytes > 65536)                                                              \
@@ -651,10 +804,13 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
     CGT_ARG_CHECK(q && o && lse && (Tk == 0 || (k && v)), "attention: null pointer");
     a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths;
     hipStream_t st = as_stream(stream);
-    const int DP = padded_dim(a.D), tiles = (int)cdiv(Tq, kAttnCols);
+    // Up to four queries read k and v once on the vector units; more rows go through the matrix cores.
+    const bool token = Tq <= 4 && a.rate.threshold == 0;
+    const int DP = padded_dim(a.D), tiles = token ? 1 : (int)cdiv(Tq, kAttnCols);
     const long heads = B * H, whole = heads * tiles;
-    // too few blocks of queries to fill the chip: the keys are cut too, into runs of 128 at least
-    const int splits = whole >= kNumCU ? 1 : (int)std::max(1L, std::min({cdiv(2L * kNumCU, whole), Tk / 128, 64L}));
+    // Too few workgroups to fill the chip: the keys are cut too, into runs of 128 at least.
+    const int want = token ? 8 * kNumCU : 2 * kNumCU;
+    const int splits = whole >= want / 2 ? 1 : (int)std::max(1L, std::min({cdiv(want, whole), Tk / 128, 64L}));
     CGT_ARG_CHECK(whole * splits < (1L << 31), "attention: too many workgroups");
     float* part = nullptr;
     float2* ml = nullptr;
@@ -665,9 +821,10 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
         ml = reinterpret_cast<float2*>(part);      // first, for its alignment
         part += 2 * rows;
     }
-    const size_t lds_bytes = (2 * kAttnRows * (DP + 4) + (table ? bias_window(a.rule) : 0)) * sizeof(float);
+    const size_t lds_bytes = ((token ? 0 : 2 * kAttnRows * (DP + 4)) + (table ? bias_window(a.rule) : 0)) * sizeof(float);
     const dim3 grid((unsigned)(whole * splits));
-    ATTN_DISPATCH(attn_fwd_kernel, a, o, lse, part, ml, tiles, splits);
+    if (token) ATTN_TOKEN(a, o, lse, part, ml, splits);
+    else ATTN_DISPATCH(attn_fwd_kernel, a, o, lse, part, ml, tiles, splits);
     CGT_LAUNCH_CHECK("attention forward");
     if (splits > 1) {
         attn_join_kernel<<<dim3((unsigned)cdiv(heads * Tq, 4)), kAttnThreads, 0, st>>>(a, o, lse, part, ml, splits);
