@@ -14,11 +14,19 @@
 // keys gk and gv, so no sum is shared between workgroups and results do not depend on the order
 // they run in.
 //
-// Matrix products are v_mfma_f32_32x32x2_f32 (true fp32).  A wavefront owns 32 columns (queries in
-// the first two kernels, keys in the third) and forms the *transposed* score tile, rows = the other
-// side: lane l then holds, for column l % 32, rows 8 g + 4 (l / 32) + t in register 4 g + t.  With
-// the k steps of the next product taken in that same order the score tile is that product's B
-// operand as it stands, with no exchange between lanes.
+// Matrix products run at float32 accuracy on the bf16 matrix cores: every operand is cut into three
+// bf16 terms, x = h + m + l (each the rounded rest of the one before: 24 bits and the sign), and the six products
+// hh, hm, mh, mm, hl, lh are accumulated in float32; the three left out are below 2^-26 of |x y|.
+// Six v_mfma_f32_32x32x16_bf16 do in 6 x 32 cycles what eight v_mfma_f32_32x32x2_f32 do in 8 x 64, and the
+// vector units work beside them (fp32 matrix instructions keep them busy).  The range is float32's
+// own; an infinite q, k, v or go makes NaN of what it reaches.
+//
+// A wavefront owns 32 columns (queries in the forward and the first backward kernel, keys in the
+// second) and forms the *transposed* score tile, rows = the other side: lane l then holds, for
+// column l % 32, rows 8 g + 4 (l / 32) + t in register 4 g + t.  With the k positions of the next
+// product's 16-wide step taken in the order (row 8 b + 4 half + t at position 8 half + 4 b + t)
+// the score tile, cut into its three terms, is that product's B operand as it stands, with no
+// exchange between lanes; the other operand is laid out in that order when it is put into LDS.
 #include "random.h"
 #include <algorithm>
 #include <cmath>
@@ -29,6 +37,10 @@ namespace cgt_amd {
 typedef float v16f __attribute__((ext_vector_type(16)));
 struct __attribute__((packed, aligned(4))) float4p {      // 16 bytes at any 4-byte aligned address
     float x, y, z, w;
+};
+
+struct __attribute__((packed, aligned(4))) float2p {
+    float x, y;
 };
 
 constexpr int kAttnThreads = 256;
@@ -67,15 +79,12 @@ __host__ __device__ inline int bucket_of(const BucketRule& r, int rel) {
 }
 
 // ---- the bias in LDS: one value per relative position in [-reach, reach], reach = max_distance + 62.
-// A wavefront's tile spans 63 relative positions around its origin, so an origin clamped to
-// +-(max_distance + 31) keeps every index inside and leaves every value as it was: beyond
-// max_distance all positions of a side are in its last bucket.
+// A wavefront's tile spans 63 relative positions around its origin (that of its first row and
+// column).  An origin max_distance + 31 or more away makes the tile far: all of it is in the last
+// bucket of a side.  Any other origin keeps every index inside the window.
 __host__ __device__ inline int bias_reach(const BucketRule& r) { return r.max_distance + 62; }
 __host__ __device__ inline int bias_window(const BucketRule& r) { return 2 * bias_reach(r) + 1; }
-__device__ __forceinline__ int clamp_origin(const BucketRule& r, int rel0) {
-    const int lim = r.max_distance + 31;
-    return rel0 < -lim ? -lim : rel0 > lim ? lim : rel0;
-}
+__device__ __forceinline__ bool far_tile(const BucketRule& r, int rel0) { return rel0 >= r.max_distance + 31 || rel0 <= -r.max_distance - 31; }
 __device__ __forceinline__ void fill_bias(const Attn& a, int head, float* win) {
     const int n = bias_window(a.rule), reach = bias_reach(a.rule);
     for (int s = threadIdx.x; s < n; s += kAttnThreads) win[s] = a.table[(long)bucket_of(a.rule, s - reach) * a.H + head];
@@ -104,71 +113,240 @@ __device__ __forceinline__ void store_scaled(float* row, int c, int D, const v16
     store4(row, c, D, valid ? v[4 * g] * f : 0.0f, valid ? v[4 * g + 1] * f : 0.0f, valid ? v[4 * g + 2] * f : 0.0f, valid ? v[4 * g + 3] * f : 0.0f);
 }
 
-// A tile of 32 rows: loaded into registers by all 256 threads (rows at or beyond `end` are zero and
-// not read), later written to LDS with a row pitch of DP + 4 floats (16-byte reads of 32
-// consecutive rows then start in different banks).
-template <int DP>
-struct TileRegs {
-    float4 v[DP / 32];
-};
-template <int DP>
-__device__ __forceinline__ void tile_load(TileRegs<DP>& t, const float* base, long stride, int row0, int end, int D) {
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-        const int idx = threadIdx.x + i * kAttnThreads, row = row0 + idx / (DP / 4), c = (idx % (DP / 4)) * 4;
-        t.v[i] = row < end ? load4(base + row * stride, c, D) : make_float4(0, 0, 0, 0);
-    }
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef unsigned v4u32 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ unsigned to_bf16x2(float lo, float hi) {
+    const v2f v = {lo, hi};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, v2bf));
 }
-template <int DP>
-__device__ __forceinline__ void tile_store(const TileRegs<DP>& t, float* lds) {
+__device__ __forceinline__ float bf16_lo(unsigned v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf16_hi(unsigned v) { return __uint_as_float(v & 0xffff0000u); }
+
+// The three bf16 terms of two floats, packed (first in the low half).
+struct Terms {
+    unsigned t[3];
+};
+__device__ __forceinline__ Terms split2(float x, float y) {
+    Terms r;
+    r.t[0] = to_bf16x2(x, y);
+    x -= bf16_lo(r.t[0]);
+    y -= bf16_hi(r.t[0]);
+    r.t[1] = to_bf16x2(x, y);
+    x -= bf16_lo(r.t[1]);
+    y -= bf16_hi(r.t[1]);
+    r.t[2] = to_bf16x2(x, y);
+    return r;
+}
+// An operand of one 16-wide step: 8 values of the lane, three terms.
+struct Frag {
+    v8bf t[3];
+};
+__device__ __forceinline__ Frag split8(const float (&x)[8]) {
+    v4u32 w[3];
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-        const int idx = threadIdx.x + i * kAttnThreads;
-        *reinterpret_cast<float4*>(lds + (idx / (DP / 4)) * (DP + 4) + (idx % (DP / 4)) * 4) = t.v[i];
+    for (int i = 0; i < 4; ++i) {
+        const Terms t = split2(x[2 * i], x[2 * i + 1]);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) w[n][i] = t.t[n];
     }
+    Frag f;
+#pragma unroll
+    for (int n = 0; n < 3; ++n) f.t[n] = __builtin_bit_cast(v8bf, w[n]);
+    return f;
+}
+// acc += a * b by the six products: the five that are at most 2^-8 of the first in `low`.  A matrix
+// instruction cuts what it adds to the accumulator at the accumulator's last bit, always downwards;
+// kept apart, the small products lose nothing to that.  Measured on 32 x 32 products of 64 (128) normal values: error
+// 4.9e-8 (6.5e-8) of the results' rms with two accumulators, mean 1e-10; 1.1e-7 (1.6e-7), mean -7e-9 (-9e-9) with one;
+// 1.4e-7 (2.0e-7) for the fp32 matrix instructions.
+__device__ __forceinline__ v16f mul_low(v16f low, const Frag& a, const Frag& b) {
+    low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[2], b.t[0], low, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[2], low, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[1], low, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[0], low, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[1], low, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mul_high(v16f acc, const Frag& a, const Frag& b) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[0], acc, 0, 0, 0);
 }
 
-// The lane's column as a B operand: d = 8 c + 4 half + t in register 4 c + t.
+// A tile of 32 rows of DP columns, shared by the workgroup.  A thread loads four neighbouring rows of
+// DP / 32 columns (rows at or beyond `end` are zero and not read), cuts them into terms and writes
+// them to LDS in one or both of two layouts, three planes (terms) each:
+//   by rows:    [row][DP + 8]  the A operand whose rows are the tile's
+//   by columns: [column][40]   the A operand whose rows are the tile's columns; the 32 rows in the
+//                              order of the score tile's registers (see above)
+// With these pitches the 16-byte reads of eight neighbouring rows start in different banks.
 template <int DP>
-__device__ __forceinline__ void column_load(float (&r)[DP / 2], const float* row, bool valid, int D, float scale) {
-    const int half = (threadIdx.x & 63) >> 5;
+struct Tile {
+    static constexpr int E = DP / 32, kRowPitch = DP + 8, kColPitch = 40;
+    static constexpr int kRowPlane = kAttnRows * kRowPitch, kColPlane = DP * kColPitch;      // in bf16
+    static constexpr int kRowBytes = 3 * kRowPlane * 2, kColBytes = 3 * kColPlane * 2;
+    float v[4][E];
+
+    // Rows row0 .. row0 + 31.  At least one row has to lie before `end`; the others are read from the last that
+    // does (so that all loads are issued together) and set to zero by clear().
+    __device__ __forceinline__ void load(const float* base, long stride, int row0, int end, int D) {
+        const int c = (threadIdx.x & 31) * E, r0 = row0 + (threadIdx.x >> 5) * 4;
+        const float* row[4];
 #pragma unroll
-    for (int c = 0; c < DP / 8; ++c) {
-        const float4 v = valid ? load4(row, 8 * c + 4 * half, D) : make_float4(0, 0, 0, 0);
-        r[4 * c] = v.x * scale;
-        r[4 * c + 1] = v.y * scale;
-        r[4 * c + 2] = v.z * scale;
-        r[4 * c + 3] = v.w * scale;
+        for (int r = 0; r < 4; ++r) row[r] = base + min(r0 + r, end - 1) * stride;
+        if (D == DP) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (E == 4) {
+                    const float4p q = *reinterpret_cast<const float4p*>(row[r] + c);
+                    v[r][0] = q.x, v[r][1] = q.y, v[r][2] = q.z, v[r][3] = q.w;
+                } else if constexpr (E == 2) {
+                    const float2p q = *reinterpret_cast<const float2p*>(row[r] + c);
+                    v[r][0] = q.x, v[r][1] = q.y;
+                } else {
+                    v[r][0] = row[r][c];
+                }
+            }
+        } else {        // heads narrower than DP: columns beyond theirs are zero
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float x = row[r][min(c + e, D - 1)];
+                    v[r][e] = c + e < D ? x : 0.0f;
+                }
+        }
     }
-}
+    __device__ __forceinline__ void clear(int row0, int end) {
+        if (row0 + kAttnRows <= end) return;
+        const int r0 = row0 + (threadIdx.x >> 5) * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[r][e] = r0 + r < end ? v[r][e] : 0.0f;
+    }
+    __device__ __forceinline__ void scale(float f) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[r][e] *= f;
+    }
+    template <bool ROWS, bool COLS>
+    __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols) const {
+        const int c = (threadIdx.x & 31) * E, rb = threadIdx.x >> 5;
+        const int pos = 16 * (rb >> 2) + 8 * (rb & 1) + 4 * ((rb >> 1) & 1);
+        Terms t[E][2];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            t[e][0] = split2(v[0][e], v[1][e]);
+            t[e][1] = split2(v[2][e], v[3][e]);
+        }
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            if (COLS) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    *reinterpret_cast<uint2*>(cols + n * kColPlane + (c + e) * kColPitch + pos) = make_uint2(t[e][0].t[n], t[e][1].t[n]);
+            }
+            if (ROWS) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    unsigned short* to = rows + n * kRowPlane + (4 * rb + r) * kRowPitch + c;
+                    if constexpr (E == 1) {
+                        *to = (unsigned short)(t[0][r >> 1].t[n] >> (16 * (r & 1)));
+                    } else {
+                        unsigned w[E / 2];
+#pragma unroll
+                        for (int e = 0; e < E; e += 2)      // the same half of two columns' words
+                            w[e / 2] = __builtin_amdgcn_perm(t[e + 1][r >> 1].t[n], t[e][r >> 1].t[n], (r & 1) ? 0x07060302u : 0x05040100u);
+                        if constexpr (E == 2) *reinterpret_cast<unsigned*>(to) = w[0];
+                        else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+                    }
+                }
+            }
+        }
+    }
+};
+
+// The lane's column as a B operand: d = 16 s + 8 half + 0..7 in step s.
+template <int DP>
+struct Column {
+    Frag s[DP / 16];
+    __device__ __forceinline__ void load(const float* row, bool valid, int D, float scale) {
+        const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const float4 x = valid ? load4(row, 16 * i + 8 * half, D) : make_float4(0, 0, 0, 0);
+            const float4 y = valid ? load4(row, 16 * i + 8 * half + 4, D) : make_float4(0, 0, 0, 0);
+            const float v[8] = {x.x * scale, x.y * scale, x.z * scale, x.w * scale, y.x * scale, y.y * scale, y.z * scale, y.w * scale};
+            s[i] = split8(v);
+        }
+    }
+};
 
 // acc[row][col] += sum_d tile[row][d] * column[d]
 template <int DP>
-__device__ __forceinline__ v16f product_rows(v16f acc, const float* lds, const float (&col)[DP / 2]) {
+__device__ __forceinline__ v16f product_rows(v16f acc, const unsigned short* rows, const Column<DP>& col) {
     const int lane = threadIdx.x & 63;
-    const float* row = lds + (lane & 31) * (DP + 4) + 4 * (lane >> 5);
+    const unsigned short* at = rows + (lane & 31) * Tile<DP>::kRowPitch + 8 * (lane >> 5);
+    v16f low = {};
 #pragma unroll
-    for (int c = 0; c < DP / 8; ++c) {
-        const float4 v = *reinterpret_cast<const float4*>(row + 8 * c);
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.x, col[4 * c], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.y, col[4 * c + 1], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.z, col[4 * c + 2], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.w, col[4 * c + 3], acc, 0, 0, 0);
+    for (int i = 0; i < DP / 16; ++i) {
+        Frag f;
+#pragma unroll
+        for (int n = 0; n < 3; ++n) f.t[n] = *reinterpret_cast<const v8bf*>(at + n * Tile<DP>::kRowPlane + 16 * i);
+        low = mul_low(low, f, col.s[i]);
+        acc = mul_high(acc, f, col.s[i]);
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] += low[r];
     return acc;
 }
 // acc[d][col] += sum_row tile[row][d] * p[row][col]
 template <int DP>
-__device__ __forceinline__ void product_cols(v16f (&acc)[DP / 32], const float* lds, const v16f& p) {
+__device__ __forceinline__ void product_cols(v16f (&acc)[DP / 32], const unsigned short* cols, const v16f& p) {
     const int lane = threadIdx.x & 63;
-    const float* at = lds + 4 * (lane >> 5) * (DP + 4) + (lane & 31);
+    const unsigned short* at = cols + (lane & 31) * Tile<DP>::kColPitch + 8 * (lane >> 5);
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int i = 0; i < 2; ++i) {
+        const float v[8] = {p[8 * i], p[8 * i + 1], p[8 * i + 2], p[8 * i + 3], p[8 * i + 4], p[8 * i + 5], p[8 * i + 6], p[8 * i + 7]};
+        const Frag b = split8(v);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (r >> 2) + (r & 3)) * (DP + 4) + 32 * d], p[r], acc[d], 0, 0, 0);
+        for (int d = 0; d < DP / 32; ++d) {
+            Frag f;
+#pragma unroll
+            for (int n = 0; n < 3; ++n) f.t[n] = *reinterpret_cast<const v8bf*>(at + n * Tile<DP>::kColPlane + 32 * d * Tile<DP>::kColPitch + 16 * i);
+            acc[d] = mul_high(mul_low(acc[d], f, b), f, b);
+        }
+    }
 }
 
+// The bias of a score tile of origin rel0; sign 1: rows are keys, -1: rows are queries.
+template <bool BIAS>
+__device__ __forceinline__ v16f tile_bias(const BucketRule& rule, const float* win, int rel0, bool far, int sign) {
+    v16f s = {};
+    if (BIAS) {
+        if (far) {
+            const float v = win[rel0 < 0 ? 0 : bias_window(rule) - 1];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = v;
+        } else {
+            const float* at = win + bias_reach(rule) + rel0 + sign * (4 * ((threadIdx.x & 63) >> 5) - (int)(threadIdx.x & 31));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = at[sign * (8 * (r >> 2) + (r & 3))];
+        }
+    }
+    return s;
+}
+// Between LDS writes and reads of one wavefront, by different lanes.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+constexpr int kSquarePitch = 36, kSquare = 32 * kSquarePitch;
+
+// exp(x) of a non-positive difference of scores; below 2^-126 it is 0.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ __forceinline__ int tile_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (r & 3); }
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
@@ -204,9 +382,10 @@ __device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_
 // ---------------------------------------------------------------- forward
 
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(Attn a, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
-    extern __shared__ float lds[];
-    float *kt = lds, *vt = kt + kAttnRows * (DP + 4), *win = vt + kAttnRows * (DP + 4);
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 3) void attn_fwd_kernel(Attn a, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
+    extern __shared__ __align__(16) unsigned short lds[];
+    unsigned short *kt = lds, *vt = kt + Tile<DP>::kRowBytes / 2;
+    float* win = reinterpret_cast<float*>(vt + Tile<DP>::kColBytes / 2);
     const Where w = where(a, tiles * splits);
     const int split = w.tile % splits, q0 = w.tile / splits * kAttnCols;
     const int lane = threadIdx.x & 63, qw = q0 + (threadIdx.x >> 6) * 32, query = qw + (lane & 31);
@@ -223,8 +402,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(Attn a, float* o
     const int first = split * run;
     last = min(last, first + run);
 
-    float qreg[DP / 2];
-    column_load<DP>(qreg, a.q + qrow, query < q_end, a.D, a.scale);
+    Column<DP> qcol;
+    qcol.load(a.q + qrow, query < q_end, a.D, a.scale);
     RngState rng = {};
     unsigned long long group0 = 0;
     if (DROP) {
@@ -233,26 +412,26 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(Attn a, float* o
     }
     v16f acc[DP / 32] = {};
     float m = -INFINITY, l = 0.0f;
-    TileRegs<DP> kr, vr;
-    tile_load<DP>(kr, kbase, a.k_t, first, last, a.D);
-    tile_load<DP>(vr, vbase, a.k_t, first, last, a.D);
+    Tile<DP> kr, vr;
+    if (first < last) {
+        kr.load(kbase, a.k_t, first, last, a.D);
+        vr.load(vbase, a.k_t, first, last, a.D);
+    }
     for (int j0 = first; j0 < last; j0 += kAttnRows) {
+        kr.clear(j0, last);
+        vr.clear(j0, last);
         __syncthreads();
-        tile_store<DP>(kr, kt);
-        tile_store<DP>(vr, vt);
+        kr.template store<true, false>(kt, nullptr);
+        vr.template store<false, true>(nullptr, vt);
         __syncthreads();
         if (j0 + kAttnRows < last) {
-            tile_load<DP>(kr, kbase, a.k_t, j0 + kAttnRows, last, a.D);
-            tile_load<DP>(vr, vbase, a.k_t, j0 + kAttnRows, last, a.D);
+            kr.load(kbase, a.k_t, j0 + kAttnRows, last, a.D);
+            vr.load(vbase, a.k_t, j0 + kAttnRows, last, a.D);
         }
         if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;      // nothing here for this wavefront
-        v16f s = {};
-        if (BIAS) {
-            const float* at = win + bias_reach(a.rule) + clamp_origin(a.rule, j0 - qw - a.q_offset) - (lane & 31);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = at[tile_row(r)];
-        }
-        s = product_rows<DP>(s, kt, qreg);
+        const int rel0 = j0 - qw - a.q_offset;
+        v16f s = tile_bias<BIAS>(a.rule, win, rel0, BIAS && far_tile(a.rule, rel0), 1);
+        s = product_rows<DP>(s, kt, qcol);
         if (j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset)) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -264,7 +443,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(Attn a, float* o
         top = fmaxf(m, fmaxf(top, other_half(top)));
         const float ref = top == -INFINITY ? 0.0f : top;      // a row that has seen nothing yet
         if (__any(top > m)) {
-            const float f = exp2f((m - ref) * kLog2e);
+            const float f = exp_of(m - ref);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
@@ -272,24 +451,32 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(Attn a, float* o
                 for (int r = 0; r < 16; ++r) acc[d][r] *= f;
         }
         m = top;
+        float part_l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = exp2f((s[r] - ref) * kLog2e);
-            l += s[r];
+            s[r] = exp_of(s[r] - ref);
+            part_l[r & 3] += s[r];
         }
+        l += (part_l[0] + part_l[1]) + (part_l[2] + part_l[3]);
         if (DROP) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 unsigned u[4];
                 random_group(rng, group0 + 2ull * (j0 / 16 + b), u);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s[8 * b + e] = random16(u, e) >= a.rate.threshold ? s[8 * b + e] * a.rate.scale : 0.0f;
+                for (int e = 0; e < 8; ++e) s[8 * b + e] = random16(u, e) >= a.rate.threshold ? s[8 * b + e] : 0.0f;      // scaled at the end
             }
         }
         product_cols<DP>(acc, vt, s);
     }
     if (query >= a.Tq) return;
     l += other_half(l);
+    if (DROP) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= a.rate.scale;
+    }
     const int half4 = 4 * (lane >> 5);
     const long stat = ((long)w.b * a.H + w.h) * a.Tq + query;
     if (splits > 1) {
@@ -325,7 +512,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(Attn a, float* 
     float acc[2] = {0.0f, 0.0f};
     for (int s = 0; s < splits; ++s) {
         const float2 ml = part_ml[s * rows + row];
-        const float f = exp2f((ml.x - ref) * kLog2e);
+        const float f = exp_of(ml.x - ref);
         l += ml.y * f;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -341,9 +528,6 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(Attn a, float* 
 }
 
 // ---------------------------------------------------------------- forward: a few queries against many keys
-
-// exp(x) of a non-positive difference of scores; below 2^-126 it is 0.
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // Sum over aligned groups of N lanes (8, 16 or 32); every lane gets it.
 template <int N>
@@ -482,12 +666,14 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
 
 // gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(Attn a, const float* o, const float* lse, const float* go, float* gq, float* delta,
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_kernel(Attn a, const float* o, const float* lse, const float* go, float* gq, float* delta,
                                                                  float* part_table, int tiles) {
-    extern __shared__ float lds[];
-    float *kt = lds, *vt = kt + kAttnRows * (DP + 4), *win = vt + kAttnRows * (DP + 4);
+    extern __shared__ __align__(16) unsigned short lds[];
+    unsigned short *kt = lds, *kc = kt + Tile<DP>::kRowBytes / 2, *vt = kc + Tile<DP>::kColBytes / 2;
+    float* square = reinterpret_cast<float*>(vt + Tile<DP>::kRowBytes / 2);      // [wavefront][32][36]
+    float* win = square + (BIAS ? 4 * kSquare : 0);
     const int window = BIAS ? bias_window(a.rule) : 0;
-    float* diag = win + window;      // [wavefront][half][window]: sums of ds by relative position
+    float* diag = win + window;      // [wavefront][window]: sums of ds by relative position
     const Where w = where(a, tiles);
     const int q0 = w.tile * kAttnCols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qw = q0 + wave * 32, query = qw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
@@ -496,24 +682,25 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(Attn a, const 
     const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
     if (BIAS) {
         fill_bias(a, w.h, win);
-        for (int s = threadIdx.x; s < 8 * window; s += kAttnThreads) diag[s] = 0.0f;
+        for (int s = threadIdx.x; s < 4 * window; s += kAttnThreads) diag[s] = 0.0f;
     }
     int last = k_end;
     if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
     if (q0 >= q_end) last = 0;
     const bool valid = query < q_end;
     const long stat = ((long)w.b * a.H + w.h) * a.Tq + query;
-    float qreg[DP / 2], greg[DP / 2];
-    column_load<DP>(qreg, a.q + qrow, valid, a.D, a.scale);
-    column_load<DP>(greg, go + qrow, valid, a.D, 1.0f);
     float dl = 0.0f;
-    {
-        float oreg[DP / 2];
-        column_load<DP>(oreg, o + qrow, valid, a.D, 1.0f);
-#pragma unroll
-        for (int i = 0; i < DP / 2; ++i) dl += oreg[i] * greg[i];
-        dl += other_half(dl);
+    if (valid) {
+        const float *orow = o + qrow, *grow = go + qrow;
+        for (int c = 4 * (lane >> 5); c < a.D; c += 8) {
+            const float4 x = load4(orow, c, a.D), y = load4(grow, c, a.D);
+            dl += (x.x * y.x + x.y * y.y) + (x.z * y.z + x.w * y.w);
+        }
     }
+    dl += other_half(dl);
+    Column<DP> qcol, gcol;
+    qcol.load(a.q + qrow, valid, a.D, a.scale);
+    gcol.load(go + qrow, valid, a.D, DROP ? a.rate.scale : 1.0f);
     if (query < a.Tq && lane < 32) delta[stat] = dl;
     float row_lse = valid ? lse[stat] : INFINITY;
     if (row_lse == -INFINITY) row_lse = INFINITY;      // a row that saw nothing: every probability is 0
@@ -523,27 +710,30 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(Attn a, const 
         rng = load_rng(a.rng, a.channel);
         group0 = (unsigned long long)stat * ((a.Tk + 15) / 16) * 2 + (lane >> 5);
     }
+    float far_before = 0.0f, far_after = 0.0f;
     v16f acc[DP / 32] = {};
-    TileRegs<DP> kr, vr;
-    tile_load<DP>(kr, kbase, a.k_t, 0, last, a.D);
-    tile_load<DP>(vr, vbase, a.k_t, 0, last, a.D);
+    Tile<DP> kr, vr;
+    if (last > 0) {
+        kr.load(kbase, a.k_t, 0, last, a.D);
+        vr.load(vbase, a.k_t, 0, last, a.D);
+    }
     for (int j0 = 0; j0 < last; j0 += kAttnRows) {
+        kr.clear(j0, last);
+        vr.clear(j0, last);
         __syncthreads();
-        tile_store<DP>(kr, kt);
-        tile_store<DP>(vr, vt);
+        kr.template store<true, true>(kt, kc);
+        vr.template store<true, false>(vt, nullptr);
         __syncthreads();
         if (j0 + kAttnRows < last) {
-            tile_load<DP>(kr, kbase, a.k_t, j0 + kAttnRows, last, a.D);
-            tile_load<DP>(vr, vbase, a.k_t, j0 + kAttnRows, last, a.D);
+            kr.load(kbase, a.k_t, j0 + kAttnRows, last, a.D);
+            vr.load(vbase, a.k_t, j0 + kAttnRows, last, a.D);
         }
         if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;
-        const int origin = BIAS ? bias_reach(a.rule) + clamp_origin(a.rule, j0 - qw - a.q_offset) - (lane & 31) : 0;
-        v16f s = {}, dp = {};
-        if (BIAS)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = win[origin + tile_row(r)];
-        s = product_rows<DP>(s, kt, qreg);
-        dp = product_rows<DP>(dp, vt, greg);
+        const int rel0 = j0 - qw - a.q_offset;
+        const bool far = BIAS && far_tile(a.rule, rel0);
+        v16f s = tile_bias<BIAS>(a.rule, win, rel0, far, 1), dp = {};
+        s = product_rows<DP>(s, kt, qcol);
+        dp = product_rows<DP>(dp, vt, gcol);
         const bool edge = j0 + kAttnRows > k_end || qw + 32 > q_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset);
         if (DROP) {
 #pragma unroll
@@ -551,23 +741,49 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(Attn a, const 
                 unsigned u[4];
                 random_group(rng, group0 + 2ull * (j0 / 16 + b), u);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dp[8 * b + e] = random16(u, e) >= a.rate.threshold ? dp[8 * b + e] * a.rate.scale : 0.0f;
+                for (int e = 0; e < 8; ++e) dp[8 * b + e] = random16(u, e) >= a.rate.threshold ? dp[8 * b + e] : 0.0f;
             }
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float p = exp2f((s[r] - row_lse) * kLog2e);
+            const float p = exp_of(s[r] - row_lse);
             s[r] = edge && (!valid || hidden(a, j0 + tile_row(r), query, k_end)) ? 0.0f : p * (dp[r] - dl);
         }
         if (BIAS) {
-            // sums along the diagonals.  The array is this wavefront's and this half's own, lanes of a half
-            // meet different positions in one instruction, and LDS takes a wavefront's instructions in
-            // order: the order of the additions is fixed.
-            float* mine = diag + (wave * 2 + (lane >> 5)) * window + origin;
+            if (far) {      // one bucket has the whole tile
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(mine + tile_row(r), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                for (int r = 0; r < 16; ++r) sum[r & 3] += s[r];
+                (rel0 < 0 ? far_before : far_after) += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            } else {
+                // Sums along the tile's 63 diagonals: element (row, column) goes to row (row - column) mod 32 of a
+                // 32 x 36 square, where lane l finds half of diagonals l and l - 32.  (Atomic additions in LDS
+                // take about 180 cycles an instruction: 2900 for this tile, all wavefronts together.)
+                float* sq = square + wave * kSquare;
+                wave_lds_fence();
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sq[((tile_row(r) - lane) & 31) * kSquarePitch + tile_row(r)] = s[r];
+                wave_lds_fence();
+                const int d = lane & 31, row0 = 16 * (lane >> 5);
+                float same = 0.0f, less = 0.0f;       // diagonals d and d - 32
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 v = *reinterpret_cast<const float4*>(sq + d * kSquarePitch + row0 + 4 * i);
+                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        same += row0 + 4 * i + t >= d ? e[t] : 0.0f;
+                        less += row0 + 4 * i + t >= d ? 0.0f : e[t];
+                    }
+                }
+                same += other_half(same);
+                less += other_half(less);
+                // the wavefront's own sums by relative position: lanes 0-31 add the upper diagonals, 32-63 the lower
+                float* mine = diag + wave * window + bias_reach(a.rule) + rel0 + d - (lane < 32 ? 0 : 32);
+                if (lane != 32) *mine += lane < 32 ? same : less;      // (there is no diagonal -32)
+            }
         }
-        product_cols<DP>(acc, kt, s);
+        product_cols<DP>(acc, kc, s);
     }
     if (query < a.Tq) {
 #pragma unroll
@@ -577,20 +793,27 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(Attn a, const 
                 store_scaled(gq + qrow, 32 * d + 8 * g + 4 * (lane >> 5), a.D, acc[d], g, valid, a.scale);
     }
     if (BIAS) {
-        __syncthreads();
-        for (int s = threadIdx.x; s < window; s += kAttnThreads) {
-            float sum = diag[s];
-            for (int i = 1; i < 8; ++i) sum += diag[i * window + s];
-            win[s] = sum;
+        // by bucket: the window's sums of the four wavefronts and the far tiles' in the window's ends
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            far_before += __shfl_xor(far_before, d);
+            far_after += __shfl_xor(far_after, d);
+        }
+        if (lane == 0) {
+            diag[wave * window] += far_before;
+            diag[wave * window + window - 1] += far_after;
         }
         __syncthreads();
         const int reach = bias_reach(a.rule);
-        for (int s = threadIdx.x; s < window; s += kAttnThreads) diag[s] = (float)bucket_of(a.rule, s - reach);
+        int* bucket = reinterpret_cast<int*>(square);
+        for (int s = threadIdx.x; s < window; s += kAttnThreads) {
+            win[s] = (diag[s] + diag[window + s]) + (diag[2 * window + s] + diag[3 * window + s]);
+            bucket[s] = bucket_of(a.rule, s - reach);
+        }
         __syncthreads();
         for (int c = threadIdx.x; c < a.rule.buckets; c += kAttnThreads) {
             float sum = 0.0f;
-            for (int s = 0; s < window; ++s)
-                if (diag[s] == (float)c) sum += win[s];
+            for (int s = 0; s < window; ++s) sum += bucket[s] == c ? win[s] : 0.0f;
             part_table[(((long)w.b * tiles + w.tile) * a.H + w.h) * a.rule.buckets + c] = sum;
         }
     }
@@ -614,9 +837,12 @@ __global__ __launch_bounds__(kAttnThreads) void attn_table_kernel(const float* p
 // ---------------------------------------------------------------- backward: keys
 
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(Attn a, const float* lse, const float* delta, const float* go, float* gk, float* gv, int tiles) {
-    extern __shared__ float lds[];
-    float *qt = lds, *gt = qt + kAttnRows * (DP + 4), *stats = gt + kAttnRows * (DP + 4), *win = stats + 2 * kAttnRows;
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, const float* lse, const float* delta, const float* go, float* gk, float* gv, int tiles) {
+    extern __shared__ __align__(16) unsigned short lds[];
+    unsigned short *qt = lds, *gt = qt + Tile<DP>::kRowBytes / 2, *qc = gt + Tile<DP>::kRowBytes / 2, *gc = qc + Tile<DP>::kColBytes / 2;
+    float* stats = reinterpret_cast<float*>(gc + Tile<DP>::kColBytes / 2);
+    unsigned* bits = reinterpret_cast<unsigned*>(stats + 2 * kAttnRows);      // [wavefront][half][query]: 16 keep bits each
+    float* win = stats + 2 * kAttnRows + (DROP ? kAttnThreads : 0);
     const Where w = where(a, tiles);
     const int k0 = w.tile * kAttnCols, lane = threadIdx.x & 63, kw = k0 + (threadIdx.x >> 6) * 32, key = kw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
@@ -629,20 +855,25 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(Attn a, const
     if (a.causal) first = max(0, k0 - a.q_offset) / kAttnRows * kAttnRows;
     if (k0 >= k_end) last = 0;
     const bool valid = key < k_end;
-    float kreg[DP / 2], vreg[DP / 2];
-    column_load<DP>(kreg, a.k + krow, valid, a.D, a.scale);
-    column_load<DP>(vreg, a.v + krow, valid, a.D, 1.0f);
+    Column<DP> kcol, vcol;
+    kcol.load(a.k + krow, valid, a.D, a.scale);
+    vcol.load(a.v + krow, valid, a.D, 1.0f);
     const long stat0 = ((long)w.b * a.H + w.h) * a.Tq;
     RngState rng = {};
     if (DROP) rng = load_rng(a.rng, a.channel);
     v16f acck[DP / 32] = {}, accv[DP / 32] = {};
-    TileRegs<DP> qr, gr;
-    tile_load<DP>(qr, qbase, a.q_t, first, last, a.D);
-    tile_load<DP>(gr, gbase, a.q_t, first, last, a.D);
+    Tile<DP> qr, gr;
+    if (first < last) {
+        qr.load(qbase, a.q_t, first, last, a.D);
+        gr.load(gbase, a.q_t, first, last, a.D);
+    }
     for (int i0 = first; i0 < last; i0 += kAttnRows) {
+        qr.clear(i0, last);
+        gr.clear(i0, last);
+        if (DROP) gr.scale(a.rate.scale);
         __syncthreads();
-        tile_store<DP>(qr, qt);
-        tile_store<DP>(gr, gt);
+        qr.template store<true, true>(qt, qc);
+        gr.template store<true, true>(gt, gc);
         if (threadIdx.x < kAttnRows) {
             const int i = i0 + threadIdx.x;
             const float v = i < last ? lse[stat0 + i] : INFINITY;
@@ -651,37 +882,47 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(Attn a, const
         }
         __syncthreads();
         if (i0 + kAttnRows < last) {
-            tile_load<DP>(qr, qbase, a.q_t, i0 + kAttnRows, last, a.D);
-            tile_load<DP>(gr, gbase, a.q_t, i0 + kAttnRows, last, a.D);
+            qr.load(qbase, a.q_t, i0 + kAttnRows, last, a.D);
+            gr.load(gbase, a.q_t, i0 + kAttnRows, last, a.D);
         }
         if (kw >= k_end || (a.causal && kw > i0 + 31 + a.q_offset)) continue;
-        v16f s = {}, dp = {};
-        if (BIAS) {
-            const float* at = win + bias_reach(a.rule) + clamp_origin(a.rule, kw - i0 - a.q_offset) + (lane & 31);
+        const int rel0 = kw - i0 - a.q_offset;
+        v16f s = tile_bias<BIAS>(a.rule, win, rel0, BIAS && far_tile(a.rule, rel0), -1), dp = {};
+        unsigned word[16];
+        if (DROP) {
+            // The generator's groups run along the keys of a query.  Lane l forms the numbers of query l % 32 and
+            // its half's 16 keys of this tile, bit 8 b + e for number e of 16-key block b, and leaves the bits in LDS,
+            // where the lane that owns one of these keys finds all its queries.
+            unsigned* mine = bits + (threadIdx.x >> 6) * kWave;
+            unsigned mask = 0;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = at[-tile_row(r)];
+            for (int b = 0; b < 2; ++b) {
+                unsigned u[4];
+                random_group(rng, ((unsigned long long)(stat0 + i0 + (lane & 31)) * ((a.Tk + 15) / 16) + kw / 16 + b) * 2 + (lane >> 5), u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mask |= random16(u, e) >= a.rate.threshold ? 1u << (8 * b + e) : 0u;
+            }
+            wave_lds_fence();
+            mine[lane] = mask;
+            wave_lds_fence();
+            const int c = lane & 31, bit = 8 * (c >> 4) + 4 * (c >> 3 & 1) + (c & 3);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) word[r] = mine[32 * (c >> 2 & 1) + tile_row(r)] >> bit & 1u;
         }
-        s = product_rows<DP>(s, qt, kreg);
-        dp = product_rows<DP>(dp, gt, vreg);
+        s = product_rows<DP>(s, qt, kcol);
+        dp = product_rows<DP>(dp, gt, vcol);
         const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + a.q_offset);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int row = tile_row(r);
-            float p = exp2f((s[r] - stats[row]) * kLog2e);
+            float p = exp_of(s[r] - stats[row]);
             if (edge && hidden(a, key, i0 + row, k_end)) p = 0.0f;      // rows beyond the queries: p is 0 by their lse
-            float f = 1.0f;
-            if (DROP) {
-                unsigned u[4];
-                random_group(rng, ((unsigned long long)(stat0 + i0 + row) * ((a.Tk + 15) / 16) + (key >> 4)) * 2 + (key >> 2 & 1), u);
-                const int e = (key & 3) + 4 * (key >> 3 & 1);
-                const unsigned word = (e >> 1) == 0 ? u[0] : (e >> 1) == 1 ? u[1] : (e >> 1) == 2 ? u[2] : u[3];
-                f = ((e & 1) ? word >> 16 : word & 0xffffu) >= a.rate.threshold ? a.rate.scale : 0.0f;
-            }
-            s[r] = p * f;
-            dp[r] = p * (dp[r] * f - stats[kAttnRows + row]);
+            const bool keep = !DROP || word[r];
+            s[r] = keep ? p : 0.0f;
+            dp[r] = p * ((keep ? dp[r] : 0.0f) - stats[kAttnRows + row]);
         }
-        product_cols<DP>(accv, gt, s);
-        product_cols<DP>(acck, qt, dp);
+        product_cols<DP>(accv, gc, s);
+        product_cols<DP>(acck, qc, dp);
     }
     if (key >= a.Tk) return;
 #pragma unroll
@@ -732,6 +973,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(Attn a, const
         KERNEL<<<grid, kAttnThreads, lds_bytes, st>>>(__VA_ARGS__);                         \
     } while (0)
 
+static size_t row_bytes(int DP) { return DP == 32 ? Tile<32>::kRowBytes : DP == 64 ? Tile<64>::kRowBytes : Tile<128>::kRowBytes; }
+static size_t col_bytes(int DP) { return DP == 32 ? Tile<32>::kColBytes : DP == 64 ? Tile<64>::kColBytes : Tile<128>::kColBytes; }
 static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // The rule of the buckets: per side (all of them, or half when positions after the query have their
@@ -821,7 +1064,7 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
         ml = reinterpret_cast<float2*>(part);      // first, for its alignment
         part += 2 * rows;
     }
-    const size_t lds_bytes = ((token ? 0 : 2 * kAttnRows * (DP + 4)) + (table ? bias_window(a.rule) : 0)) * sizeof(float);
+    const size_t lds_bytes = (token ? 0 : row_bytes(DP) + col_bytes(DP)) + (table ? bias_window(a.rule) * sizeof(float) : 0);
     const dim3 grid((unsigned)(whole * splits));
     if (token) ATTN_TOKEN(a, o, lse, part, ml, splits);
     else ATTN_DISPATCH(attn_fwd_kernel, a, o, lse, part, ml, tiles, splits);
@@ -863,7 +1106,7 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
     float* part = delta + heads * Tq;
     const int window = table ? bias_window(a.rule) : 0;
     {
-        const size_t lds_bytes = (2 * kAttnRows * (DP + 4) + 9 * window) * sizeof(float);
+        const size_t lds_bytes = 2 * row_bytes(DP) + col_bytes(DP) + (table ? 4 * kSquare + 5 * window : 0) * sizeof(float);
         const dim3 grid((unsigned)(heads * qtiles));
         ATTN_DISPATCH(attn_bwd_q_kernel, a, o, lse, go, gq, delta, part, qtiles);
         CGT_LAUNCH_CHECK("attention backward (queries)");
@@ -873,7 +1116,7 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
         CGT_LAUNCH_CHECK("attention backward (table)");
     }
     if (ktiles) {
-        const size_t lds_bytes = (2 * kAttnRows * (DP + 4) + 2 * kAttnRows + window) * sizeof(float);
+        const size_t lds_bytes = 2 * row_bytes(DP) + 2 * col_bytes(DP) + (2 * kAttnRows + (a.rate.threshold ? kAttnThreads : 0) + window) * sizeof(float);
         const dim3 grid((unsigned)(heads * ktiles));
         ATTN_DISPATCH(attn_bwd_kv_kernel, a, lse, delta, go, gk, gv, ktiles);
         CGT_LAUNCH_CHECK("attention backward (keys)");
