@@ -14,12 +14,15 @@
 // keys gk and gv, so no sum is shared between workgroups and results do not depend on the order
 // they run in.
 //
-// Matrix products run at float32 accuracy on the bf16 matrix cores: every operand is cut into three
-// bf16 terms, x = h + m + l (each the rounded rest of the one before: 24 bits and the sign), and the six products
-// hh, hm, mh, mm, hl, lh are accumulated in float32; the three left out are below 2^-26 of |x y|.
-// Six v_mfma_f32_32x32x16_bf16 do in 6 x 32 cycles what eight v_mfma_f32_32x32x2_f32 do in 8 x 64, and the
-// vector units work beside them (fp32 matrix instructions keep them busy).  The range is float32's
-// own; an infinite q, k, v or go makes NaN of what it reaches.
+// Matrix products run at float32 accuracy on the fp16 matrix cores: an operand, times a power of two
+// that brings the largest of its head's values to 2^14, is cut into two fp16 terms, x = h + l (l is the
+// rounded rest: 22 bits and the sign), and the products l h, h l, h h are accumulated in float32.  Three
+// v_mfma_f32_32x32x16_f16 do in 3 x 32 cycles what eight v_mfma_f32_32x32x2_f32 do in 8 x 64, and the
+// vector units work beside them (fp32 matrix instructions keep them busy).  Measured on products of
+// 128 (64) normal values: error 1.1e-7 (1.0e-7) of the results' rms, 2.0e-7 (1.4e-7) with the fp32
+// instructions.  Values keep all 22 bits down to 2^-17 of the largest of their head, and an
+// absolute 2^-39 of it below; the largest values of a head are found by a kernel that runs first.
+// An infinite q, k, v or go makes NaN of what it reaches.
 //
 // A wavefront owns 32 columns (queries in the forward and the first backward kernel, keys in the
 // second) and forms the *transposed* score tile, rows = the other side: lane l then holds, for
@@ -113,69 +116,53 @@ __device__ __forceinline__ void store_scaled(float* row, int c, int D, const v16
     store4(row, c, D, valid ? v[4 * g] * f : 0.0f, valid ? v[4 * g + 1] * f : 0.0f, valid ? v[4 * g + 2] * f : 0.0f, valid ? v[4 * g + 3] * f : 0.0f);
 }
 
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef unsigned v4u32 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ unsigned to_bf16x2(float lo, float hi) {
-    const v2f v = {lo, hi};
-    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, v2bf));
+// The power of two that brings `top` to [2^14, 2^15), and its reciprocal; 1 for 0.  Capped at 2^100, so that
+// the reciprocal of two together stays a float.
+__device__ __forceinline__ float power_scale(float top) {
+    const unsigned e = __float_as_uint(top) >> 23 & 255u, field = min(268u - e, 227u);
+    return top == 0.0f ? 1.0f : __uint_as_float(field << 23);
 }
-__device__ __forceinline__ float bf16_lo(unsigned v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float bf16_hi(unsigned v) { return __uint_as_float(v & 0xffff0000u); }
+__device__ __forceinline__ float reciprocal_power(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// The three bf16 terms of two floats, packed (first in the low half).
+// The two fp16 terms of two floats, packed (first in the low half).
 struct Terms {
-    unsigned t[3];
+    unsigned t[2];
 };
 __device__ __forceinline__ Terms split2(float x, float y) {
-    Terms r;
-    r.t[0] = to_bf16x2(x, y);
-    x -= bf16_lo(r.t[0]);
-    y -= bf16_hi(r.t[0]);
-    r.t[1] = to_bf16x2(x, y);
-    x -= bf16_lo(r.t[1]);
-    y -= bf16_hi(r.t[1]);
-    r.t[2] = to_bf16x2(x, y);
-    return r;
+    const v2f v = {x, y};
+    const v2h h = __builtin_convertvector(v, v2h);
+    const v2f rest = {__builtin_fmaf((float)h.x, -1.0f, x), __builtin_fmaf((float)h.y, -1.0f, y)};
+    return {{__builtin_bit_cast(unsigned, h), __builtin_bit_cast(unsigned, __builtin_convertvector(rest, v2h))}};
 }
-// An operand of one 16-wide step: 8 values of the lane, three terms.
+// An operand of one 16-wide step: 8 values of the lane, two terms.
 struct Frag {
-    v8bf t[3];
+    v8h t[2];
 };
 __device__ __forceinline__ Frag split8(const float (&x)[8]) {
-    v4u32 w[3];
+    v4u32 w[2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const Terms t = split2(x[2 * i], x[2 * i + 1]);
-#pragma unroll
-        for (int n = 0; n < 3; ++n) w[n][i] = t.t[n];
+        w[0][i] = t.t[0];
+        w[1][i] = t.t[1];
     }
-    Frag f;
-#pragma unroll
-    for (int n = 0; n < 3; ++n) f.t[n] = __builtin_bit_cast(v8bf, w[n]);
-    return f;
+    return {{__builtin_bit_cast(v8h, w[0]), __builtin_bit_cast(v8h, w[1])}};
 }
-// acc += a * b by the six products: the five that are at most 2^-8 of the first in `low`.  A matrix
-// instruction cuts what it adds to the accumulator at the accumulator's last bit, always downwards;
-// kept apart, the small products lose nothing to that.  Measured on 32 x 32 products of 64 (128) normal values: error
-// 4.9e-8 (6.5e-8) of the results' rms with two accumulators, mean 1e-10; 1.1e-7 (1.6e-7), mean -7e-9 (-9e-9) with one;
-// 1.4e-7 (2.0e-7) for the fp32 matrix instructions.
-__device__ __forceinline__ v16f mul_low(v16f low, const Frag& a, const Frag& b) {
-    low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[2], b.t[0], low, 0, 0, 0);
-    low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[2], low, 0, 0, 0);
-    low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[1], low, 0, 0, 0);
-    low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[0], low, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[1], low, 0, 0, 0);
-}
-__device__ __forceinline__ v16f mul_high(v16f acc, const Frag& a, const Frag& b) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[0], acc, 0, 0, 0);
+// acc += a * b
+__device__ __forceinline__ v16f mul_step(v16f acc, const Frag& a, const Frag& b) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.t[1], b.t[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.t[0], b.t[1], acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.t[0], b.t[0], acc, 0, 0, 0);
 }
 
 // A tile of 32 rows of DP columns, shared by the workgroup.  A thread loads four neighbouring rows of
-// DP / 32 columns (rows at or beyond `end` are zero and not read), cuts them into terms and writes
-// them to LDS in one or both of two layouts, three planes (terms) each:
+// DP / 32 columns (rows at or beyond `end` are zero and not read), scales them, cuts them into terms and
+// writes them to LDS in one or both of two layouts, two planes (terms) each:
 //   by rows:    [row][DP + 8]  the A operand whose rows are the tile's
 //   by columns: [column][40]   the A operand whose rows are the tile's columns; the 32 rows in the
 //                              order of the score tile's registers (see above)
@@ -183,8 +170,8 @@ __device__ __forceinline__ v16f mul_high(v16f acc, const Frag& a, const Frag& b)
 template <int DP>
 struct Tile {
     static constexpr int E = DP / 32, kRowPitch = DP + 8, kColPitch = 40;
-    static constexpr int kRowPlane = kAttnRows * kRowPitch, kColPlane = DP * kColPitch;      // in bf16
-    static constexpr int kRowBytes = 3 * kRowPlane * 2, kColBytes = 3 * kColPlane * 2;
+    static constexpr int kRowPlane = kAttnRows * kRowPitch, kColPlane = DP * kColPitch;      // in fp16
+    static constexpr int kRowBytes = 2 * kRowPlane * 2, kColBytes = 2 * kColPlane * 2;
     float v[4][E];
 
     // Rows row0 .. row0 + 31.  At least one row has to lie before `end`; the others are read from the last that
@@ -225,24 +212,18 @@ struct Tile {
 #pragma unroll
             for (int e = 0; e < E; ++e) v[r][e] = r0 + r < end ? v[r][e] : 0.0f;
     }
-    __device__ __forceinline__ void scale(float f) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[r][e] *= f;
-    }
     template <bool ROWS, bool COLS>
-    __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols) const {
+    __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols, float scale) const {
         const int c = (threadIdx.x & 31) * E, rb = threadIdx.x >> 5;
         const int pos = 16 * (rb >> 2) + 8 * (rb & 1) + 4 * ((rb >> 1) & 1);
         Terms t[E][2];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            t[e][0] = split2(v[0][e], v[1][e]);
-            t[e][1] = split2(v[2][e], v[3][e]);
+            t[e][0] = split2(v[0][e] * scale, v[1][e] * scale);
+            t[e][1] = split2(v[2][e] * scale, v[3][e] * scale);
         }
 #pragma unroll
-        for (int n = 0; n < 3; ++n) {
+        for (int n = 0; n < 2; ++n) {
             if (COLS) {
 #pragma unroll
                 for (int e = 0; e < E; ++e)
@@ -268,39 +249,54 @@ struct Tile {
     }
 };
 
-// The lane's column as a B operand: d = 16 s + 8 half + 0..7 in step s.
+// The lane's column as a B operand: d = 16 s + 8 half + 0..7 in step s; odd steps negated (see product_rows).
 template <int DP>
 struct Column {
     Frag s[DP / 16];
-    __device__ __forceinline__ void load(const float* row, bool valid, int D, float scale) {
+    float v[DP / 2];
+    __device__ __forceinline__ void load(const float* row, bool valid, int D) {
         const int half = (threadIdx.x & 63) >> 5;
 #pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+            const float4 x = valid ? load4(row, 16 * (i >> 1) + 8 * half + 4 * (i & 1), D) : make_float4(0, 0, 0, 0);
+            v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+        }
+    }
+    // largest magnitude of the whole column (both halves)
+    __device__ __forceinline__ float top() const {
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DP / 2; ++i) t = fmaxf(t, fabsf(v[i]));
+        return fmaxf(t, __shfl_xor(t, 32));
+    }
+    __device__ __forceinline__ void split(float scale) {
+#pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            const float4 x = valid ? load4(row, 16 * i + 8 * half, D) : make_float4(0, 0, 0, 0);
-            const float4 y = valid ? load4(row, 16 * i + 8 * half + 4, D) : make_float4(0, 0, 0, 0);
-            const float v[8] = {x.x * scale, x.y * scale, x.z * scale, x.w * scale, y.x * scale, y.y * scale, y.z * scale, y.w * scale};
-            s[i] = split8(v);
+            const float f = i & 1 ? -scale : scale;
+            const float x[8] = {v[8 * i] * f, v[8 * i + 1] * f, v[8 * i + 2] * f, v[8 * i + 3] * f,
+                                v[8 * i + 4] * f, v[8 * i + 5] * f, v[8 * i + 6] * f, v[8 * i + 7] * f};
+            s[i] = split8(x);
         }
     }
 };
 
-// acc[row][col] += sum_d tile[row][d] * column[d]
+// sum_d tile[row][d] * column[d].  A matrix instruction aligns the products it adds and cuts their
+// last bits, always downwards.  The shift is some 1e-8 of the result, but the same sign everywhere, and the
+// gradient of the bias sums millions of nearly cancelling terms: so even and odd steps are summed
+// apart, the odd ones negated, and their difference has no such shift.
 template <int DP>
-__device__ __forceinline__ v16f product_rows(v16f acc, const unsigned short* rows, const Column<DP>& col) {
+__device__ __forceinline__ v16f product_rows(const unsigned short* rows, const Column<DP>& col) {
     const int lane = threadIdx.x & 63;
     const unsigned short* at = rows + (lane & 31) * Tile<DP>::kRowPitch + 8 * (lane >> 5);
-    v16f low = {};
+    v16f sum[2] = {};
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
         Frag f;
 #pragma unroll
-        for (int n = 0; n < 3; ++n) f.t[n] = *reinterpret_cast<const v8bf*>(at + n * Tile<DP>::kRowPlane + 16 * i);
-        low = mul_low(low, f, col.s[i]);
-        acc = mul_high(acc, f, col.s[i]);
+        for (int n = 0; n < 2; ++n) f.t[n] = *reinterpret_cast<const v8h*>(at + n * Tile<DP>::kRowPlane + 16 * i);
+        sum[i & 1] = mul_step(sum[i & 1], f, col.s[i]);
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] += low[r];
-    return acc;
+    return sum[0] - sum[1];
 }
 // acc[d][col] += sum_row tile[row][d] * p[row][col]
 template <int DP>
@@ -315,28 +311,34 @@ __device__ __forceinline__ void product_cols(v16f (&acc)[DP / 32], const unsigne
         for (int d = 0; d < DP / 32; ++d) {
             Frag f;
 #pragma unroll
-            for (int n = 0; n < 3; ++n) f.t[n] = *reinterpret_cast<const v8bf*>(at + n * Tile<DP>::kColPlane + 32 * d * Tile<DP>::kColPitch + 16 * i);
-            acc[d] = mul_high(mul_low(acc[d], f, b), f, b);
+            for (int n = 0; n < 2; ++n) f.t[n] = *reinterpret_cast<const v8h*>(at + n * Tile<DP>::kColPlane + 32 * d * Tile<DP>::kColPitch + 16 * i);
+            acc[d] = mul_step(acc[d], f, b);
         }
     }
 }
 
-// The bias of a score tile of origin rel0; sign 1: rows are keys, -1: rows are queries.
+__device__ __forceinline__ int tile_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (r & 3); }
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+constexpr float kLn2 = 0.6931471805599453f;
+// exp(x) of a non-positive difference of scores; below 2^-126 it is 0.  exp_scaled: 2^14 exp(x).
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+__device__ __forceinline__ float exp_scaled(float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, 14.0f)); }
+
+// s * unscale + bias for a score tile of origin rel0; sign 1: rows are keys, -1: rows are queries.
 template <bool BIAS>
-__device__ __forceinline__ v16f tile_bias(const BucketRule& rule, const float* win, int rel0, bool far, int sign) {
-    v16f s = {};
-    if (BIAS) {
-        if (far) {
-            const float v = win[rel0 < 0 ? 0 : bias_window(rule) - 1];
+__device__ __forceinline__ void scores(v16f& s, float unscale, const BucketRule& rule, const float* win, int rel0, int sign) {
+    if (!BIAS) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = v;
-        } else {
-            const float* at = win + bias_reach(rule) + rel0 + sign * (4 * ((threadIdx.x & 63) >> 5) - (int)(threadIdx.x & 31));
+        for (int r = 0; r < 16; ++r) s[r] *= unscale;
+    } else if (far_tile(rule, rel0)) {
+        const float v = win[rel0 < 0 ? 0 : bias_window(rule) - 1];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = at[sign * (8 * (r >> 2) + (r & 3))];
-        }
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], unscale, v);
+    } else {
+        const float* at = win + bias_reach(rule) + rel0 + sign * (4 * ((threadIdx.x & 63) >> 5) - (int)(threadIdx.x & 31));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], unscale, at[sign * (8 * (r >> 2) + (r & 3))]);
     }
-    return s;
 }
 // Between LDS writes and reads of one wavefront, by different lanes.
 __device__ __forceinline__ void wave_lds_fence() {
@@ -345,33 +347,103 @@ __device__ __forceinline__ void wave_lds_fence() {
 }
 constexpr int kSquarePitch = 36, kSquare = 32 * kSquarePitch;
 
-// exp(x) of a non-positive difference of scores; below 2^-126 it is 0.
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-__device__ __forceinline__ int tile_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (r & 3); }
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
-
 struct Where {
     int b, h, tile;
 };
 // Workgroups of one head follow each other on one XCD (ids go round the eight of them), so that its
-// keys and values are read into one L2.
-__device__ __forceinline__ Where where(const Attn& a, int tiles) {
-    const int heads = a.B * a.H, id = blockIdx.x;
-    int head, tile;
-    if (heads % kNumXCD == 0) {
-        const int slot = id / kNumXCD;
-        head = id % kNumXCD + kNumXCD * (slot / tiles);
-        tile = slot % tiles;
-    } else {
-        head = id / tiles;
-        tile = id % tiles;
-    }
+// keys and values are read into one L2.  Under a causal mask the tiles of a head differ in work, and
+// the ones that come last decide the time: there all heads' heaviest tiles come first (`last_heavy`:
+// the last tile of a head is its heaviest, otherwise the first).
+__device__ __forceinline__ Where where(const Attn& a, int tiles, bool last_heavy) {
+    const int heads = a.B * a.H, group = heads % kNumXCD == 0 ? kNumXCD : 1;
+    const int slot = blockIdx.x / group, per = heads / group;
+    int head = a.causal ? slot % per : slot / tiles, tile = a.causal ? slot / per : slot % tiles;
+    head = head * group + blockIdx.x % group;
+    if (a.causal && last_heavy) tile = tiles - 1 - tile;
     return {head / a.H, head % a.H, tile};
 }
 __device__ __forceinline__ int length_of(const int* lengths, int b, int T) {
     if (!lengths) return T;
     const int n = lengths[b];
     return n < 0 ? 0 : n > T ? T : n;
+}
+
+// ---- the largest values of a head
+
+// What the scales of a head rest on, for one of its arrays: the largest magnitude of a value and the
+// largest norm of a row, over the rows within the length (values that are no numbers left out), for a run of
+// rows each; [array][head][run].
+struct RangeArrays {
+    const float* base[4];
+    int keys[4];      // 1: laid out and limited as k, 0: as q
+};
+__global__ __launch_bounds__(kAttnThreads) void attn_range_kernel(Attn a, RangeArrays arrays, int runs, float2* out) {
+    __shared__ float2 join[4];
+    const int head = blockIdx.x / runs, at = blockIdx.x % runs, b = head / a.H, h = head % a.H, n = blockIdx.y, keys = arrays.keys[n];
+    const int T = keys ? a.Tk : a.Tq, end = length_of(keys ? a.k_lengths : a.q_lengths, b, T);
+    const int run = (T + runs - 1) / runs, first = at * run, last = min(end, first + run);
+    const long stride = keys ? a.k_t : a.q_t;
+    const float* base = arrays.base[n] + (keys ? b * a.k_b + h * a.k_h : b * a.q_b + h * a.q_h);
+    const int lanes = a.D <= 32 ? 8 : a.D <= 64 ? 16 : 32, c = threadIdx.x % lanes * 4, step = kAttnThreads / lanes;
+    float top = 0.0f, norm = 0.0f;
+    for (int r0 = first + threadIdx.x / lanes; r0 < last; r0 += 4 * step) {
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = load4(base + min(r0 + u * step, last - 1) * stride, c, a.D);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+            float sq = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float m = fabsf(x[e]) <= 3.4028235e38f ? fabsf(x[e]) : 0.0f;
+                top = fmaxf(top, m);
+                sq += m * m;
+            }
+            for (int d = 1; d < lanes; d <<= 1) sq += __shfl_xor(sq, d);
+            norm = fmaxf(norm, sq);
+        }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, d));
+        norm = fmaxf(norm, __shfl_xor(norm, d));
+    }
+    if ((threadIdx.x & 63) == 0) join[threadIdx.x >> 6] = make_float2(top, norm);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 4; ++i) {
+            top = fmaxf(top, join[i].x);
+            norm = fmaxf(norm, join[i].y);
+        }
+        out[(long)n * gridDim.x + blockIdx.x] = make_float2(top, sqrtf(norm));
+    }
+}
+struct Ranges {
+    const float2* at;
+    int runs;
+};
+__device__ __forceinline__ float2 head_range(const Attn& a, const Ranges& r, int array, const Where& w) {
+    const float2* p = r.at + ((long)array * a.B * a.H + w.b * a.H + w.h) * r.runs;
+    float2 m = p[0];
+    for (int i = 1; i < r.runs; ++i) m = make_float2(fmaxf(m.x, p[i].x), fmaxf(m.y, p[i].y));
+    return m;
+}
+
+// The scales of the backward pass, from the ranges of k, v, q and go (in that order).  ds = p (dp - go . o) is at
+// most twice the largest |go| |v| (o is a mean of the v; dropout's factor counts for both): its scale
+// brings that bound below 2^15.
+struct HeadScales {
+    float k, v, q, g, ds;
+    __device__ __forceinline__ float score(const Attn& a) const { return a.scale * reciprocal_power(k) * reciprocal_power(q); }
+    __device__ __forceinline__ float dp(const Attn& a) const {
+        return reciprocal_power(v) * reciprocal_power(g) * (a.rate.threshold ? a.rate.scale : 1.0f);
+    }
+};
+__device__ __forceinline__ HeadScales head_scales(const Attn& a, const Ranges& ranges, const Where& w) {
+    const float2 k = head_range(a, ranges, 0, w), v = head_range(a, ranges, 1, w), q = head_range(a, ranges, 2, w), g = head_range(a, ranges, 3, w);
+    const float bound = 2.0f * v.y * g.y * (a.rate.threshold ? a.rate.scale : 1.0f);
+    return {power_scale(k.x), power_scale(v.x), power_scale(q.x), power_scale(g.x), power_scale(bound)};
 }
 
 // Which of a tile's 16 elements of a lane are hidden; rows are keys, the column is a query.
@@ -382,11 +454,11 @@ __device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_
 // ---------------------------------------------------------------- forward
 
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 3) void attn_fwd_kernel(Attn a, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kernel(Attn a, Ranges ranges, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *kt = lds, *vt = kt + Tile<DP>::kRowBytes / 2;
     float* win = reinterpret_cast<float*>(vt + Tile<DP>::kColBytes / 2);
-    const Where w = where(a, tiles * splits);
+    const Where w = where(a, tiles * splits, true);
     const int split = w.tile % splits, q0 = w.tile / splits * kAttnCols;
     const int lane = threadIdx.x & 63, qw = q0 + (threadIdx.x >> 6) * 32, query = qw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
@@ -402,8 +474,12 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 3) void attn_fwd_kern
     const int first = split * run;
     last = min(last, first + run);
 
+    const float kscale = power_scale(head_range(a, ranges, 0, w).x), vscale = power_scale(head_range(a, ranges, 1, w).x);
     Column<DP> qcol;
-    qcol.load(a.q + qrow, query < q_end, a.D, a.scale);
+    qcol.load(a.q + qrow, query < q_end, a.D);
+    const float qscale = power_scale(qcol.top());
+    qcol.split(qscale);
+    const float unscale = a.scale * reciprocal_power(kscale) * reciprocal_power(qscale);      // of a score
     RngState rng = {};
     unsigned long long group0 = 0;
     if (DROP) {
@@ -421,8 +497,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 3) void attn_fwd_kern
         kr.clear(j0, last);
         vr.clear(j0, last);
         __syncthreads();
-        kr.template store<true, false>(kt, nullptr);
-        vr.template store<false, true>(nullptr, vt);
+        kr.template store<true, false>(kt, nullptr, kscale);
+        vr.template store<false, true>(nullptr, vt, vscale);
         __syncthreads();
         if (j0 + kAttnRows < last) {
             kr.load(kbase, a.k_t, j0 + kAttnRows, last, a.D);
@@ -430,8 +506,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 3) void attn_fwd_kern
         }
         if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;      // nothing here for this wavefront
         const int rel0 = j0 - qw - a.q_offset;
-        v16f s = tile_bias<BIAS>(a.rule, win, rel0, BIAS && far_tile(a.rule, rel0), 1);
-        s = product_rows<DP>(s, kt, qcol);
+        v16f s = product_rows<DP>(kt, qcol);
+        scores<BIAS>(s, unscale, a.rule, win, rel0, 1);
         if (j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset)) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -454,7 +530,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 3) void attn_fwd_kern
         float part_l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = exp_of(s[r] - ref);
+            s[r] = exp_scaled(s[r] - ref);
             part_l[r & 3] += s[r];
         }
         l += (part_l[0] + part_l[1]) + (part_l[2] + part_l[3]);
@@ -470,13 +546,12 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 3) void attn_fwd_kern
         product_cols<DP>(acc, vt, s);
     }
     if (query >= a.Tq) return;
-    l += other_half(l);
-    if (DROP) {
+    l = (l + other_half(l)) * 0x1p-14f;
+    const float back = 0x1p-14f * reciprocal_power(vscale) * (DROP ? a.rate.scale : 1.0f);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] *= a.rate.scale;
-    }
+        for (int r = 0; r < 16; ++r) acc[d][r] *= back;
     const int half4 = 4 * (lane >> 5);
     const long stat = ((long)w.b * a.H + w.h) * a.Tq + query;
     if (splits > 1) {
@@ -555,7 +630,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
     extern __shared__ float win[];
     __shared__ float4 join_o[NQ][4][LANES];
     __shared__ float2 join_ml[NQ][4];
-    const Where w = where(a, splits);
+    const Where w = where(a, splits, true);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % LANES * 4, group = lane / LANES, split = w.tile;
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
     int last = k_end;
@@ -666,7 +741,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
 
 // gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_kernel(Attn a, const float* o, const float* lse, const float* go, float* gq, float* delta,
+__global__ __launch_bounds__(kAttnThreads, 2) void attn_bwd_q_kernel(Attn a, Ranges ranges, const float* o, const float* lse, const float* go, float* gq, float* delta,
                                                                  float* part_table, int tiles) {
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *kt = lds, *kc = kt + Tile<DP>::kRowBytes / 2, *vt = kc + Tile<DP>::kColBytes / 2;
@@ -674,7 +749,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
     float* win = square + (BIAS ? 4 * kSquare : 0);
     const int window = BIAS ? bias_window(a.rule) : 0;
     float* diag = win + window;      // [wavefront][window]: sums of ds by relative position
-    const Where w = where(a, tiles);
+    const Where w = where(a, tiles, true);
     const int q0 = w.tile * kAttnCols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qw = q0 + wave * 32, query = qw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
     const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
@@ -698,10 +773,15 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         }
     }
     dl += other_half(dl);
+    const HeadScales sc = head_scales(a, ranges, w);
     Column<DP> qcol, gcol;
-    qcol.load(a.q + qrow, valid, a.D, a.scale);
-    gcol.load(go + qrow, valid, a.D, DROP ? a.rate.scale : 1.0f);
+    qcol.load(a.q + qrow, valid, a.D);
+    qcol.split(sc.q);
+    gcol.load(go + qrow, valid, a.D);
+    gcol.split(sc.g);
+    const float unscale = sc.score(a), dscale = sc.dp(a) * sc.ds;      // ds is formed times sc.ds
     if (query < a.Tq && lane < 32) delta[stat] = dl;
+    dl *= sc.ds;
     float row_lse = valid ? lse[stat] : INFINITY;
     if (row_lse == -INFINITY) row_lse = INFINITY;      // a row that saw nothing: every probability is 0
     RngState rng = {};
@@ -721,8 +801,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         kr.clear(j0, last);
         vr.clear(j0, last);
         __syncthreads();
-        kr.template store<true, true>(kt, kc);
-        vr.template store<true, false>(vt, nullptr);
+        kr.template store<true, true>(kt, kc, sc.k);
+        vr.template store<true, false>(vt, nullptr, sc.v);
         __syncthreads();
         if (j0 + kAttnRows < last) {
             kr.load(kbase, a.k_t, j0 + kAttnRows, last, a.D);
@@ -730,10 +810,9 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         }
         if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;
         const int rel0 = j0 - qw - a.q_offset;
-        const bool far = BIAS && far_tile(a.rule, rel0);
-        v16f s = tile_bias<BIAS>(a.rule, win, rel0, far, 1), dp = {};
-        s = product_rows<DP>(s, kt, qcol);
-        dp = product_rows<DP>(dp, vt, gcol);
+        v16f s = product_rows<DP>(kt, qcol);
+        v16f dp = product_rows<DP>(vt, gcol);
+        scores<BIAS>(s, unscale, a.rule, win, rel0, 1);
         const bool edge = j0 + kAttnRows > k_end || qw + 32 > q_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset);
         if (DROP) {
 #pragma unroll
@@ -747,10 +826,10 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float p = exp_of(s[r] - row_lse);
-            s[r] = edge && (!valid || hidden(a, j0 + tile_row(r), query, k_end)) ? 0.0f : p * (dp[r] - dl);
+            s[r] = edge && (!valid || hidden(a, j0 + tile_row(r), query, k_end)) ? 0.0f : p * __builtin_fmaf(dp[r], dscale, -dl);
         }
         if (BIAS) {
-            if (far) {      // one bucket has the whole tile
+            if (far_tile(a.rule, rel0)) {      // one bucket has the whole tile
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sum[r & 3] += s[r];
@@ -790,7 +869,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                store_scaled(gq + qrow, 32 * d + 8 * g + 4 * (lane >> 5), a.D, acc[d], g, valid, a.scale);
+                store_scaled(gq + qrow, 32 * d + 8 * g + 4 * (lane >> 5), a.D, acc[d], g, valid, a.scale * reciprocal_power(sc.k) * reciprocal_power(sc.ds));
     }
     if (BIAS) {
         // by bucket: the window's sums of the four wavefronts and the far tiles' in the window's ends
@@ -814,7 +893,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         for (int c = threadIdx.x; c < a.rule.buckets; c += kAttnThreads) {
             float sum = 0.0f;
             for (int s = 0; s < window; ++s) sum += bucket[s] == c ? win[s] : 0.0f;
-            part_table[(((long)w.b * tiles + w.tile) * a.H + w.h) * a.rule.buckets + c] = sum;
+            part_table[(((long)w.b * tiles + w.tile) * a.H + w.h) * a.rule.buckets + c] = sum * reciprocal_power(sc.ds);
         }
     }
 }
@@ -837,13 +916,13 @@ __global__ __launch_bounds__(kAttnThreads) void attn_table_kernel(const float* p
 // ---------------------------------------------------------------- backward: keys
 
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, const float* lse, const float* delta, const float* go, float* gk, float* gv, int tiles) {
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, Ranges ranges, const float* lse, const float* delta, const float* go, float* gk, float* gv, int tiles) {
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *qt = lds, *gt = qt + Tile<DP>::kRowBytes / 2, *qc = gt + Tile<DP>::kRowBytes / 2, *gc = qc + Tile<DP>::kColBytes / 2;
     float* stats = reinterpret_cast<float*>(gc + Tile<DP>::kColBytes / 2);
     unsigned* bits = reinterpret_cast<unsigned*>(stats + 2 * kAttnRows);      // [wavefront][half][query]: 16 keep bits each
     float* win = stats + 2 * kAttnRows + (DROP ? kAttnThreads : 0);
-    const Where w = where(a, tiles);
+    const Where w = where(a, tiles, false);
     const int k0 = w.tile * kAttnCols, lane = threadIdx.x & 63, kw = k0 + (threadIdx.x >> 6) * 32, key = kw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
     const float* qbase = a.q + w.b * a.q_b + w.h * a.q_h;
@@ -855,9 +934,13 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
     if (a.causal) first = max(0, k0 - a.q_offset) / kAttnRows * kAttnRows;
     if (k0 >= k_end) last = 0;
     const bool valid = key < k_end;
+    const HeadScales sc = head_scales(a, ranges, w);
+    const float unscale = sc.score(a), dscale = sc.dp(a) * sc.ds * 0x1p-14f, lscale = sc.ds * 0x1p-14f;      // p carries 2^14
     Column<DP> kcol, vcol;
-    kcol.load(a.k + krow, valid, a.D, a.scale);
-    vcol.load(a.v + krow, valid, a.D, 1.0f);
+    kcol.load(a.k + krow, valid, a.D);
+    kcol.split(sc.k);
+    vcol.load(a.v + krow, valid, a.D);
+    vcol.split(sc.v);
     const long stat0 = ((long)w.b * a.H + w.h) * a.Tq;
     RngState rng = {};
     if (DROP) rng = load_rng(a.rng, a.channel);
@@ -870,15 +953,14 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
     for (int i0 = first; i0 < last; i0 += kAttnRows) {
         qr.clear(i0, last);
         gr.clear(i0, last);
-        if (DROP) gr.scale(a.rate.scale);
         __syncthreads();
-        qr.template store<true, true>(qt, qc);
-        gr.template store<true, true>(gt, gc);
+        qr.template store<true, true>(qt, qc, sc.q);
+        gr.template store<true, true>(gt, gc, sc.g);
         if (threadIdx.x < kAttnRows) {
             const int i = i0 + threadIdx.x;
             const float v = i < last ? lse[stat0 + i] : INFINITY;
             stats[threadIdx.x] = v == -INFINITY ? INFINITY : v;
-            stats[kAttnRows + threadIdx.x] = i < last ? delta[stat0 + i] : 0.0f;
+            stats[kAttnRows + threadIdx.x] = i < last ? delta[stat0 + i] * lscale : 0.0f;
         }
         __syncthreads();
         if (i0 + kAttnRows < last) {
@@ -887,7 +969,6 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
         }
         if (kw >= k_end || (a.causal && kw > i0 + 31 + a.q_offset)) continue;
         const int rel0 = kw - i0 - a.q_offset;
-        v16f s = tile_bias<BIAS>(a.rule, win, rel0, BIAS && far_tile(a.rule, rel0), -1), dp = {};
         unsigned word[16];
         if (DROP) {
             // The generator's groups run along the keys of a query.  Lane l forms the numbers of query l % 32 and
@@ -909,17 +990,18 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
 #pragma unroll
             for (int r = 0; r < 16; ++r) word[r] = mine[32 * (c >> 2 & 1) + tile_row(r)] >> bit & 1u;
         }
-        s = product_rows<DP>(s, qt, kcol);
-        dp = product_rows<DP>(dp, gt, vcol);
+        v16f s = product_rows<DP>(qt, kcol);
+        v16f dp = product_rows<DP>(gt, vcol);
+        scores<BIAS>(s, unscale, a.rule, win, rel0, -1);
         const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + a.q_offset);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int row = tile_row(r);
-            float p = exp_of(s[r] - stats[row]);
+            float p = exp_scaled(s[r] - stats[row]);
             if (edge && hidden(a, key, i0 + row, k_end)) p = 0.0f;      // rows beyond the queries: p is 0 by their lse
             const bool keep = !DROP || word[r];
             s[r] = keep ? p : 0.0f;
-            dp[r] = p * ((keep ? dp[r] : 0.0f) - stats[kAttnRows + row]);
+            dp[r] = p * __builtin_fmaf(keep ? dp[r] : 0.0f, dscale, -stats[kAttnRows + row]);
         }
         product_cols<DP>(accv, gc, s);
         product_cols<DP>(acck, qc, dp);
@@ -930,8 +1012,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int c = 32 * d + 8 * g + 4 * (lane >> 5);
-            store_scaled(gk + krow, c, a.D, acck[d], g, valid, a.scale);
-            store_scaled(gv + krow, c, a.D, accv[d], g, valid, 1.0f);
+            store_scaled(gk + krow, c, a.D, acck[d], g, valid, a.scale * reciprocal_power(sc.q) * reciprocal_power(sc.ds));
+            store_scaled(gv + krow, c, a.D, accv[d], g, valid, 0x1p-14f * reciprocal_power(sc.g) * (DROP ? a.rate.scale : 1.0f));
         }
 }
 
@@ -973,6 +1055,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
         KERNEL<<<grid, kAttnThreads, lds_bytes, st>>>(__VA_ARGS__);                         \
     } while (0)
 
+// Runs of rows whose largest values are found by workgroups of their own: 256 rows or more, 16 at most.
+static int range_runs(long Tq, long Tk) { return (int)std::max(1L, std::min(cdiv(std::max(Tq, Tk), 256), 16L)); }
 static size_t row_bytes(int DP) { return DP == 32 ? Tile<32>::kRowBytes : DP == 64 ? Tile<64>::kRowBytes : Tile<128>::kRowBytes; }
 static size_t col_bytes(int DP) { return DP == 32 ? Tile<32>::kColBytes : DP == 64 ? Tile<64>::kColBytes : Tile<128>::kColBytes; }
 static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
@@ -1054,20 +1138,29 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
     // Too few workgroups to fill the chip: the keys are cut too, into runs of 128 at least.
     const int want = token ? 8 * kNumCU : 2 * kNumCU;
     const int splits = whole >= want / 2 ? 1 : (int)std::max(1L, std::min({cdiv(want, whole), Tk / 128, 64L}));
-    CGT_ARG_CHECK(whole * splits < (1L << 31), "attention: too many workgroups");
+    CGT_ARG_CHECK(whole * splits < (1L << 31) && heads * range_runs(Tq, Tk) < (1L << 31), "attention: too many workgroups");
+    // workspace: the heads' ranges, then the pieces of a split key axis
+    const int runs = range_runs(Tq, Tk);
+    const size_t rows = splits > 1 ? (size_t)heads * Tq * splits : 0, range_floats = token ? 0 : (size_t)heads * runs * 2 * 2;
     float* part = nullptr;
     float2* ml = nullptr;
-    if (splits > 1) {
-        const size_t rows = (size_t)heads * Tq * splits;
-        part = stream_workspace(stream, kWsAttention, rows * (D + 2) * sizeof(float), "attention");
-        if (!part) return CGT_AMD_ERR_NOMEM;
-        ml = reinterpret_cast<float2*>(part);      // first, for its alignment
-        part += 2 * rows;
+    Ranges ranges = {nullptr, runs};
+    if (rows + range_floats) {
+        float* ws = stream_workspace(stream, kWsAttention, (range_floats + rows * (D + 2)) * sizeof(float), "attention");
+        if (!ws) return CGT_AMD_ERR_NOMEM;
+        ranges.at = reinterpret_cast<const float2*>(ws);
+        ml = reinterpret_cast<float2*>(ws + range_floats);
+        part = ws + range_floats + 2 * rows;
+    }
+    if (!token && Tk > 0) {
+        const RangeArrays arrays = {{k, v}, {1, 1}};
+        attn_range_kernel<<<dim3((unsigned)(heads * runs), 2), kAttnThreads, 0, st>>>(a, arrays, runs, const_cast<float2*>(ranges.at));
+        CGT_LAUNCH_CHECK("attention ranges");
     }
     const size_t lds_bytes = (token ? 0 : row_bytes(DP) + col_bytes(DP)) + (table ? bias_window(a.rule) * sizeof(float) : 0);
     const dim3 grid((unsigned)(whole * splits));
     if (token) ATTN_TOKEN(a, o, lse, part, ml, splits);
-    else ATTN_DISPATCH(attn_fwd_kernel, a, o, lse, part, ml, tiles, splits);
+    else ATTN_DISPATCH(attn_fwd_kernel, a, ranges, o, lse, part, ml, tiles, splits);
     CGT_LAUNCH_CHECK("attention forward");
     if (splits > 1) {
         attn_join_kernel<<<dim3((unsigned)cdiv(heads * Tq, 4)), kAttnThreads, 0, st>>>(a, o, lse, part, ml, splits);
@@ -1098,17 +1191,22 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
     a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths;
     hipStream_t st = as_stream(stream);
     const int DP = padded_dim(a.D), qtiles = (int)cdiv(Tq, kAttnCols), ktiles = (int)cdiv(Tk, kAttnCols);
-    CGT_ARG_CHECK(heads * qtiles < (1L << 31) && heads * ktiles < (1L << 31), "attention backward: too many workgroups");
+    const int runs = range_runs(Tq, Tk);
+    CGT_ARG_CHECK(heads * qtiles < (1L << 31) && heads * ktiles < (1L << 31) && heads * runs < (1L << 31), "attention backward: too many workgroups");
     const long parts = B * qtiles;
-    const size_t need = (size_t)(heads * Tq + (table ? parts * H * buckets : 0)) * sizeof(float);
-    float* delta = stream_workspace(stream, kWsAttention, need, "attention backward");
-    if (!delta) return CGT_AMD_ERR_NOMEM;
-    float* part = delta + heads * Tq;
+    const size_t range_floats = (size_t)heads * runs * 4 * 2, need = range_floats + (size_t)(heads * Tq + (table ? parts * H * buckets : 0));
+    float* ws = stream_workspace(stream, kWsAttention, need * sizeof(float), "attention backward");
+    if (!ws) return CGT_AMD_ERR_NOMEM;
+    float *delta = ws + range_floats, *part = delta + heads * Tq;
+    const Ranges ranges = {reinterpret_cast<const float2*>(ws), runs};
+    const RangeArrays arrays = {{k, v, q, go}, {1, 1, 0, 0}};
+    attn_range_kernel<<<dim3((unsigned)(heads * runs), 4), kAttnThreads, 0, st>>>(a, arrays, runs, reinterpret_cast<float2*>(ws));
+    CGT_LAUNCH_CHECK("attention backward (ranges)");
     const int window = table ? bias_window(a.rule) : 0;
     {
         const size_t lds_bytes = 2 * row_bytes(DP) + col_bytes(DP) + (table ? 4 * kSquare + 5 * window : 0) * sizeof(float);
         const dim3 grid((unsigned)(heads * qtiles));
-        ATTN_DISPATCH(attn_bwd_q_kernel, a, o, lse, go, gq, delta, part, qtiles);
+        ATTN_DISPATCH(attn_bwd_q_kernel, a, ranges, o, lse, go, gq, delta, part, qtiles);
         CGT_LAUNCH_CHECK("attention backward (queries)");
     }
     if (table) {
@@ -1118,7 +1216,7 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
     if (ktiles) {
         const size_t lds_bytes = 2 * row_bytes(DP) + 2 * col_bytes(DP) + (2 * kAttnRows + (a.rate.threshold ? kAttnThreads : 0) + window) * sizeof(float);
         const dim3 grid((unsigned)(heads * ktiles));
-        ATTN_DISPATCH(attn_bwd_kv_kernel, a, lse, delta, go, gk, gv, ktiles);
+        ATTN_DISPATCH(attn_bwd_kv_kernel, a, ranges, lse, delta, go, gk, gv, ktiles);
         CGT_LAUNCH_CHECK("attention backward (keys)");
     }
     return CGT_AMD_OK;
