@@ -88,9 +88,10 @@ __host__ __device__ inline int bucket_of(const BucketRule& r, int rel) {
 __host__ __device__ inline int bias_reach(const BucketRule& r) { return r.max_distance + 62; }
 __host__ __device__ inline int bias_window(const BucketRule& r) { return 2 * bias_reach(r) + 1; }
 __device__ __forceinline__ bool far_tile(const BucketRule& r, int rel0) { return rel0 >= r.max_distance + 31 || rel0 <= -r.max_distance - 31; }
+__device__ __forceinline__ float to_log2(float x);
 __device__ __forceinline__ void fill_bias(const Attn& a, int head, float* win) {
     const int n = bias_window(a.rule), reach = bias_reach(a.rule);
-    for (int s = threadIdx.x; s < n; s += kAttnThreads) win[s] = a.table[(long)bucket_of(a.rule, s - reach) * a.H + head];
+    for (int s = threadIdx.x; s < n; s += kAttnThreads) win[s] = to_log2(a.table[(long)bucket_of(a.rule, s - reach) * a.H + head]);
 }
 
 // Four floats of a row of D at column c; zero beyond the row's end.
@@ -129,15 +130,22 @@ __device__ __forceinline__ float power_scale(float top) {
 }
 __device__ __forceinline__ float reciprocal_power(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// The two fp16 terms of two floats, packed (first in the low half).
+// The two fp16 terms of two floats times a power of two, packed (first in the low half).
 struct Terms {
     unsigned t[2];
 };
+__device__ __forceinline__ Terms split2(float x, float y, float scale) {
+    const v2h h = {(_Float16)__builtin_fmaf(x, scale, 0.0f), (_Float16)__builtin_fmaf(y, scale, 0.0f)};
+    const v2h l = {(_Float16)__builtin_fmaf(x, scale, -(float)h.x), (_Float16)__builtin_fmaf(y, scale, -(float)h.y)};
+    return {{__builtin_bit_cast(unsigned, h), __builtin_bit_cast(unsigned, l)}};
+}
 __device__ __forceinline__ Terms split2(float x, float y) {
     const v2f v = {x, y};
     const v2h h = __builtin_convertvector(v, v2h);
-    const v2f rest = {__builtin_fmaf((float)h.x, -1.0f, x), __builtin_fmaf((float)h.y, -1.0f, y)};
-    return {{__builtin_bit_cast(unsigned, h), __builtin_bit_cast(unsigned, __builtin_convertvector(rest, v2h))}};
+    float one = 1.0f;
+    asm("" : "+s"(one));      // a 1 that the compiler does not see: subtraction and rounding stay one instruction
+    const v2h l = {(_Float16)__builtin_fmaf(x, one, -(float)h.x), (_Float16)__builtin_fmaf(y, one, -(float)h.y)};
+    return {{__builtin_bit_cast(unsigned, h), __builtin_bit_cast(unsigned, l)}};
 }
 // An operand of one 16-wide step: 8 values of the lane, two terms.
 struct Frag {
@@ -174,43 +182,45 @@ struct Tile {
     static constexpr int kRowBytes = 2 * kRowPlane * 2, kColBytes = 2 * kColPlane * 2;
     float v[4][E];
 
-    // Rows row0 .. row0 + 31.  At least one row has to lie before `end`; the others are read from the last that
-    // does (so that all loads are issued together) and set to zero by clear().
-    __device__ __forceinline__ void load(const float* base, long stride, int row0, int end, int D) {
-        const int c = (threadIdx.x & 31) * E, r0 = row0 + (threadIdx.x >> 5) * 4;
-        const float* row[4];
+    // What does not change from tile to tile: the lane's offsets (bytes) from a tile's first row.
+    struct Offsets {
+        unsigned at[4];
+        bool fit;
+        __device__ __forceinline__ Offsets(long stride, int D) : fit(D == DP && stride < (1L << 24)) {
+            const int c = (threadIdx.x & 31) * E, r0 = (threadIdx.x >> 5) * 4;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) row[r] = base + min(r0 + r, end - 1) * stride;
-        if (D == DP) {
+            for (int r = 0; r < 4; ++r) at[r] = (unsigned)((r0 + r) * (int)stride + c) * 4u;
+        }
+    };
+    // Rows row0 .. row0 + 31, zero at or beyond `end` and in columns beyond a head's own (both are read from the last
+    // row or column inside, so that all loads are issued together; `end` is positive).
+    __device__ __forceinline__ void load(const Offsets& off, const float* base, long stride, int row0, int end, int D) {
+        if (off.fit && row0 + kAttnRows <= end) {      // a whole tile: one wave-uniform origin
+            const char* tile = reinterpret_cast<const char*>(base + row0 * stride);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if constexpr (E == 4) {
-                    const float4p q = *reinterpret_cast<const float4p*>(row[r] + c);
+                    const float4p q = *reinterpret_cast<const float4p*>(tile + off.at[r]);
                     v[r][0] = q.x, v[r][1] = q.y, v[r][2] = q.z, v[r][3] = q.w;
                 } else if constexpr (E == 2) {
-                    const float2p q = *reinterpret_cast<const float2p*>(row[r] + c);
+                    const float2p q = *reinterpret_cast<const float2p*>(tile + off.at[r]);
                     v[r][0] = q.x, v[r][1] = q.y;
                 } else {
-                    v[r][0] = row[r][c];
+                    v[r][0] = *reinterpret_cast<const float*>(tile + off.at[r]);
                 }
             }
-        } else {        // heads narrower than DP: columns beyond theirs are zero
+        } else {
+            const int c = (threadIdx.x & 31) * E, r0 = (threadIdx.x >> 5) * 4;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r) {
+                const float* row = base + min(row0 + r0 + r, end - 1) * stride;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float x = row[r][min(c + e, D - 1)];
-                    v[r][e] = c + e < D ? x : 0.0f;
+                    const float x = row[min(c + e, D - 1)];
+                    v[r][e] = row0 + r0 + r < end && c + e < D ? x : 0.0f;
                 }
+            }
         }
-    }
-    __device__ __forceinline__ void clear(int row0, int end) {
-        if (row0 + kAttnRows <= end) return;
-        const int r0 = row0 + (threadIdx.x >> 5) * 4;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[r][e] = r0 + r < end ? v[r][e] : 0.0f;
     }
     template <bool ROWS, bool COLS>
     __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols, float scale) const {
@@ -219,8 +229,8 @@ struct Tile {
         Terms t[E][2];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            t[e][0] = split2(v[0][e] * scale, v[1][e] * scale);
-            t[e][1] = split2(v[2][e] * scale, v[3][e] * scale);
+            t[e][0] = split2(v[0][e], v[1][e], scale);
+            t[e][1] = split2(v[2][e], v[3][e], scale);
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -249,7 +259,7 @@ struct Tile {
     }
 };
 
-// The lane's column as a B operand: d = 16 s + 8 half + 0..7 in step s; odd steps negated (see product_rows).
+// The lane's column as a B operand: d = 16 s + 8 half + 0..7 in step s.
 template <int DP>
 struct Column {
     Frag s[DP / 16];
@@ -269,10 +279,11 @@ struct Column {
         for (int i = 0; i < DP / 2; ++i) t = fmaxf(t, fabsf(v[i]));
         return fmaxf(t, __shfl_xor(t, 32));
     }
-    __device__ __forceinline__ void split(float scale) {
+    // odd: the sign of the odd steps (see product_rows)
+    __device__ __forceinline__ void split(float scale, float odd) {
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            const float f = i & 1 ? -scale : scale;
+            const float f = i & 1 ? odd * scale : scale;
             const float x[8] = {v[8 * i] * f, v[8 * i + 1] * f, v[8 * i + 2] * f, v[8 * i + 3] * f,
                                 v[8 * i + 4] * f, v[8 * i + 5] * f, v[8 * i + 6] * f, v[8 * i + 7] * f};
             s[i] = split8(x);
@@ -281,22 +292,23 @@ struct Column {
 };
 
 // sum_d tile[row][d] * column[d].  A matrix instruction aligns the products it adds and cuts their
-// last bits, always downwards.  The shift is some 1e-8 of the result, but the same sign everywhere, and the
-// gradient of the bias sums millions of nearly cancelling terms: so even and odd steps are summed
-// apart, the odd ones negated, and their difference has no such shift.
-template <int DP>
+// last bits, always downwards.  That shift is some 1e-8 of the result, nothing in itself, but it has the
+// same sign everywhere, and the gradient of the bias sums millions of nearly cancelling ds: APART
+// sums even and odd steps apart, the column's odd ones negated; in their difference the shifts cancel.
+template <int DP, bool APART>
 __device__ __forceinline__ v16f product_rows(const unsigned short* rows, const Column<DP>& col) {
     const int lane = threadIdx.x & 63;
     const unsigned short* at = rows + (lane & 31) * Tile<DP>::kRowPitch + 8 * (lane >> 5);
-    v16f sum[2] = {};
+    v16f sum = {}, odd = {};
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
         Frag f;
 #pragma unroll
         for (int n = 0; n < 2; ++n) f.t[n] = *reinterpret_cast<const v8h*>(at + n * Tile<DP>::kRowPlane + 16 * i);
-        sum[i & 1] = mul_step(sum[i & 1], f, col.s[i]);
+        if (APART && (i & 1)) odd = mul_step(odd, f, col.s[i]);
+        else sum = mul_step(sum, f, col.s[i]);
     }
-    return sum[0] - sum[1];
+    return APART ? sum - odd : sum;
 }
 // acc[d][col] += sum_row tile[row][d] * p[row][col]
 template <int DP>
@@ -318,11 +330,18 @@ __device__ __forceinline__ void product_cols(v16f (&acc)[DP / 32], const unsigne
 }
 
 __device__ __forceinline__ int tile_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (r & 3); }
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
-constexpr float kLn2 = 0.6931471805599453f;
-// exp(x) of a non-positive difference of scores; below 2^-126 it is 0.  exp_scaled: 2^14 exp(x).
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-__device__ __forceinline__ float exp_scaled(float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, 14.0f)); }
+// v of lane ^ 32
+__device__ __forceinline__ float other_half(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+// Scores are kept in powers of two (times log2 e): the exponential is then one instruction.
+constexpr float kLn2 = 0.6931471805599453f, kLowest = -3.4028234663852886e38f;
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }      // below 2^-126 it is 0
+// x log2 e; finite values stay finite at the lower end (a bias of the lowest float)
+__device__ __forceinline__ float to_log2(float x) { return x < -1e38f && x >= kLowest ? fmaxf(x * kLog2e, kLowest) : x * kLog2e; }
+// log sum exp from the reference of a row's exponentials (in powers of two) and their sum
+__device__ __forceinline__ float log_sum(float ref, float sum) { return ref < -1e38f ? ref : ref * kLn2 + logf(sum); }
 
 // s * unscale + bias for a score tile of origin rel0; sign 1: rows are keys, -1: rows are queries.
 template <bool BIAS>
@@ -345,21 +364,24 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-constexpr int kSquarePitch = 36, kSquare = 32 * kSquarePitch;
+constexpr int kSquare = 32 * 32;
+__device__ __forceinline__ int square_at(int d, int row) { return d * 32 + (row ^ (d & 7) << 2); }
 
 struct Where {
     int b, h, tile;
 };
 // Workgroups of one head follow each other on one XCD (ids go round the eight of them), so that its
 // keys and values are read into one L2.  Under a causal mask the tiles of a head differ in work, and
-// the ones that come last decide the time: there all heads' heaviest tiles come first (`last_heavy`:
-// the last tile of a head is its heaviest, otherwise the first).
-__device__ __forceinline__ Where where(const Attn& a, int tiles, bool last_heavy) {
+// the ones that come last decide the time: there all heads' heaviest tiles come first (its last
+// ones for blocks of queries, its first for blocks of keys).
+enum TileOrder { kByHead, kHeavyLast, kHeavyFirst };      // where a head's heaviest tiles are
+__device__ __forceinline__ Where where(const Attn& a, int tiles, TileOrder order) {
     const int heads = a.B * a.H, group = heads % kNumXCD == 0 ? kNumXCD : 1;
     const int slot = blockIdx.x / group, per = heads / group;
-    int head = a.causal ? slot % per : slot / tiles, tile = a.causal ? slot / per : slot % tiles;
+    const bool by_tile = a.causal && order != kByHead;
+    int head = by_tile ? slot % per : slot / tiles, tile = by_tile ? slot / per : slot % tiles;
     head = head * group + blockIdx.x % group;
-    if (a.causal && last_heavy) tile = tiles - 1 - tile;
+    if (by_tile && order == kHeavyLast) tile = tiles - 1 - tile;
     return {head / a.H, head % a.H, tile};
 }
 __device__ __forceinline__ int length_of(const int* lengths, int b, int T) {
@@ -368,40 +390,61 @@ __device__ __forceinline__ int length_of(const int* lengths, int b, int T) {
     return n < 0 ? 0 : n > T ? T : n;
 }
 
+// Sum over aligned groups of N lanes (8, 16 or 32); every lane gets it.
+template <int N>
+__device__ __forceinline__ float group_sum(float x) {
+    auto add = [](float v, auto ctrl) {
+        return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    x = add(x, std::integral_constant<int, 0xB1>());       // lane ^ 1
+    x = add(x, std::integral_constant<int, 0x4E>());       // lane ^ 2
+    x = add(x, std::integral_constant<int, 0x141>());      // mirrored within 8: the other quad
+    if (N >= 16) x = add(x, std::integral_constant<int, 0x140>());      // mirrored within 16: the other eight
+    if (N >= 32) x += __shfl_xor(x, 16);
+    return x;
+}
+
 // ---- the largest values of a head
 
-// What the scales of a head rest on, for one of its arrays: the largest magnitude of a value and the
-// largest norm of a row, over the rows within the length (values that are no numbers left out), for a run of
-// rows each; [array][head][run].
+// What a head's workgroups have in common, worked out once.  For each of its arrays, what the scales rest on:
+// the largest magnitude of a value and (if asked for) the largest norm of a row, over the rows within the
+// length, values that are no numbers left out, for a run of rows each: [array][head][run].  And the
+// bias by relative position, [head of H][window], in the grid's last row.
 struct RangeArrays {
     const float* base[4];
     int keys[4];      // 1: laid out and limited as k, 0: as q
+    int norm[4];
 };
-__global__ __launch_bounds__(kAttnThreads) void attn_range_kernel(Attn a, RangeArrays arrays, int runs, float2* out) {
+template <int DP>
+__global__ __launch_bounds__(kAttnThreads) void attn_range_kernel(Attn a, RangeArrays arrays, int n_arrays, int runs, float2* out, float* window) {
+    constexpr int LANES = DP / 4, STEP = kAttnThreads / LANES, DEEP = 8;
     __shared__ float2 join[4];
-    const int head = blockIdx.x / runs, at = blockIdx.x % runs, b = head / a.H, h = head % a.H, n = blockIdx.y, keys = arrays.keys[n];
+    const int n = blockIdx.y;
+    if (n == n_arrays) {
+        const int size = bias_window(a.rule), total = size * a.H;
+        for (int i = blockIdx.x * kAttnThreads + threadIdx.x; i < total; i += gridDim.x * kAttnThreads)
+            window[i] = to_log2(a.table[(long)bucket_of(a.rule, i % size - bias_reach(a.rule)) * a.H + i / size]);
+        return;
+    }
+    const int head = blockIdx.x / runs, at = blockIdx.x % runs, b = head / a.H, h = head % a.H, keys = arrays.keys[n], with_norm = arrays.norm[n];
     const int T = keys ? a.Tk : a.Tq, end = length_of(keys ? a.k_lengths : a.q_lengths, b, T);
-    const int run = (T + runs - 1) / runs, first = at * run, last = min(end, first + run);
+    const int run = (T + runs - 1) / runs, first = at * run, last = min(end, first + run), c = threadIdx.x % LANES * 4;
     const long stride = keys ? a.k_t : a.q_t;
     const float* base = arrays.base[n] + (keys ? b * a.k_b + h * a.k_h : b * a.q_b + h * a.q_h);
-    const int lanes = a.D <= 32 ? 8 : a.D <= 64 ? 16 : 32, c = threadIdx.x % lanes * 4, step = kAttnThreads / lanes;
     float top = 0.0f, norm = 0.0f;
-    for (int r0 = first + threadIdx.x / lanes; r0 < last; r0 += 4 * step) {
-        float4 v[4];
+    for (int r0 = first + threadIdx.x / LANES; r0 < last; r0 += DEEP * STEP) {
+        float4 v[DEEP];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = load4(base + min(r0 + u * step, last - 1) * stride, c, a.D);
+        for (int u = 0; u < DEEP; ++u) v[u] = load4(base + min(r0 + u * STEP, last - 1) * stride, c, a.D);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-            float sq = 0.0f;
+        for (int u = 0; u < DEEP; ++u) {
+            float x[4] = {fabsf(v[u].x), fabsf(v[u].y), fabsf(v[u].z), fabsf(v[u].w)};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float m = fabsf(x[e]) <= 3.4028235e38f ? fabsf(x[e]) : 0.0f;
-                top = fmaxf(top, m);
-                sq += m * m;
+                x[e] = x[e] <= -kLowest ? x[e] : 0.0f;
+                top = fmaxf(top, x[e]);
             }
-            for (int d = 1; d < lanes; d <<= 1) sq += __shfl_xor(sq, d);
-            norm = fmaxf(norm, sq);
+            if (with_norm) norm = fmaxf(norm, group_sum<LANES>((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])));
         }
     }
 #pragma unroll
@@ -422,7 +465,12 @@ __global__ __launch_bounds__(kAttnThreads) void attn_range_kernel(Attn a, RangeA
 struct Ranges {
     const float2* at;
     int runs;
+    const float* window;
 };
+__device__ __forceinline__ void copy_bias(const Attn& a, const Ranges& r, int head, float* win) {
+    const int n = bias_window(a.rule);
+    for (int s = threadIdx.x; s < n; s += kAttnThreads) win[s] = r.window[(long)head * n + s];
+}
 __device__ __forceinline__ float2 head_range(const Attn& a, const Ranges& r, int array, const Where& w) {
     const float2* p = r.at + ((long)array * a.B * a.H + w.b * a.H + w.h) * r.runs;
     float2 m = p[0];
@@ -435,7 +483,7 @@ __device__ __forceinline__ float2 head_range(const Attn& a, const Ranges& r, int
 // brings that bound below 2^15.
 struct HeadScales {
     float k, v, q, g, ds;
-    __device__ __forceinline__ float score(const Attn& a) const { return a.scale * reciprocal_power(k) * reciprocal_power(q); }
+    __device__ __forceinline__ float score(const Attn& a) const { return a.scale * kLog2e * reciprocal_power(k) * reciprocal_power(q); }
     __device__ __forceinline__ float dp(const Attn& a) const {
         return reciprocal_power(v) * reciprocal_power(g) * (a.rate.threshold ? a.rate.scale : 1.0f);
     }
@@ -458,14 +506,14 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *kt = lds, *vt = kt + Tile<DP>::kRowBytes / 2;
     float* win = reinterpret_cast<float*>(vt + Tile<DP>::kColBytes / 2);
-    const Where w = where(a, tiles * splits, true);
+    const Where w = where(a, tiles * splits, kHeavyLast);
     const int split = w.tile % splits, q0 = w.tile / splits * kAttnCols;
     const int lane = threadIdx.x & 63, qw = q0 + (threadIdx.x >> 6) * 32, query = qw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
     const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
     const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
     const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
-    if (BIAS) fill_bias(a, w.h, win);
+    if (BIAS) copy_bias(a, ranges, w.h, win);
     // keys this workgroup walks: to the last one its last query sees, cut into `splits` runs of whole tiles
     int last = k_end;
     if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
@@ -478,8 +526,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     Column<DP> qcol;
     qcol.load(a.q + qrow, query < q_end, a.D);
     const float qscale = power_scale(qcol.top());
-    qcol.split(qscale);
-    const float unscale = a.scale * reciprocal_power(kscale) * reciprocal_power(qscale);      // of a score
+    qcol.split(qscale, 1.0f);
+    const float unscale = a.scale * kLog2e * reciprocal_power(kscale) * reciprocal_power(qscale);      // of a score
     RngState rng = {};
     unsigned long long group0 = 0;
     if (DROP) {
@@ -487,26 +535,25 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
         group0 = ((unsigned long long)(w.b * a.H + w.h) * a.Tq + query) * ((a.Tk + 15) / 16) * 2 + (lane >> 5);
     }
     v16f acc[DP / 32] = {};
-    float m = -INFINITY, l = 0.0f;
+    float ref = -INFINITY, l = 0.0f;      // the exponentials are 2^(s - ref + 7)
+    const typename Tile<DP>::Offsets off(a.k_t, a.D);
     Tile<DP> kr, vr;
     if (first < last) {
-        kr.load(kbase, a.k_t, first, last, a.D);
-        vr.load(vbase, a.k_t, first, last, a.D);
+        kr.load(off, kbase, a.k_t, first, last, a.D);
+        vr.load(off, vbase, a.k_t, first, last, a.D);
     }
     for (int j0 = first; j0 < last; j0 += kAttnRows) {
-        kr.clear(j0, last);
-        vr.clear(j0, last);
         __syncthreads();
         kr.template store<true, false>(kt, nullptr, kscale);
         vr.template store<false, true>(nullptr, vt, vscale);
         __syncthreads();
         if (j0 + kAttnRows < last) {
-            kr.load(kbase, a.k_t, j0 + kAttnRows, last, a.D);
-            vr.load(vbase, a.k_t, j0 + kAttnRows, last, a.D);
+            kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
+            vr.load(off, vbase, a.k_t, j0 + kAttnRows, last, a.D);
         }
         if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;      // nothing here for this wavefront
         const int rel0 = j0 - qw - a.q_offset;
-        v16f s = product_rows<DP>(kt, qcol);
+        v16f s = product_rows<DP, false>(kt, qcol);
         scores<BIAS>(s, unscale, a.rule, win, rel0, 1);
         if (j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset)) {
 #pragma unroll
@@ -516,21 +563,24 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
         float top = s[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-        top = fmaxf(m, fmaxf(top, other_half(top)));
-        const float ref = top == -INFINITY ? 0.0f : top;      // a row that has seen nothing yet
-        if (__any(top > m)) {
-            const float f = exp_of(m - ref);
+        top = fmaxf(top, other_half(top));
+        // The reference follows the running maximum only where that is 2^7 above it: the exponentials stay below 2^14,
+        // and the results so far are seldom rescaled.
+        const bool rise = top > ref + 7.0f;
+        if (__any(rise)) {
+            const float to = rise ? top : ref, f = to == -INFINITY ? 0.0f : pow2(ref - to);
+            ref = to;
             l *= f;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= f;
         }
-        m = top;
+        const float from = ref == -INFINITY ? 0.0f : ref - 7.0f;      // (a row that has seen nothing yet)
         float part_l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = exp_scaled(s[r] - ref);
+            s[r] = pow2(s[r] - from);
             part_l[r & 3] += s[r];
         }
         l += (part_l[0] + part_l[1]) + (part_l[2] + part_l[3]);
@@ -546,8 +596,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
         product_cols<DP>(acc, vt, s);
     }
     if (query >= a.Tq) return;
-    l = (l + other_half(l)) * 0x1p-14f;
-    const float back = 0x1p-14f * reciprocal_power(vscale) * (DROP ? a.rate.scale : 1.0f);
+    l = (l + other_half(l)) * 0x1p-7f;
+    const float back = 0x1p-7f * reciprocal_power(vscale) * (DROP ? a.rate.scale : 1.0f);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -561,7 +611,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
 #pragma unroll
             for (int g = 0; g < 4; ++g)
                 store4(part + row * a.D, 32 * d + 8 * g + half4, a.D, acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
-        if (half4 == 0) part_ml[row] = make_float2(m, l);
+        if (half4 == 0) part_ml[row] = make_float2(ref, l);
         return;
     }
     const bool saw = query < q_end && l != 0.0f;      // a row that saw no key is zero, whatever the values hold
@@ -570,53 +620,37 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) store_scaled(o + qrow, 32 * d + 8 * g + half4, a.D, acc[d], g, saw, inv);
-    if (half4 == 0) lse[stat] = saw ? m + logf(l) : -INFINITY;
+    if (half4 == 0) lse[stat] = saw ? log_sum(ref, l) : -INFINITY;
 }
 
-// o and lse from the pieces of a split key axis, joined in order.  One wavefront per row.
+// o and lse from the pieces of a split key axis, joined in order.  A group of DP / 4 lanes takes a row.
+template <int DP>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(Attn a, float* o, float* lse, const float* part, const float2* part_ml, int splits) {
-    const long rows = (long)a.B * a.H * a.Tq, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int LANES = DP / 4;
+    const long rows = (long)a.B * a.H * a.Tq, row = (long)blockIdx.x * (kAttnThreads / LANES) + threadIdx.x / LANES;
     if (row >= rows) return;
-    const int lane = threadIdx.x & 63, query = (int)(row % a.Tq);
-    const long head = row / a.Tq;
-    const int b = (int)(head / a.H), h = (int)(head % a.H);
+    const int c = threadIdx.x % LANES * 4, head = (int)(row / a.Tq), query = (int)(row - (long)head * a.Tq);
+    const int b = head / a.H, h = head % a.H;
     const bool valid = query < length_of(a.q_lengths, b, a.Tq);
     float m = -INFINITY, l = 0.0f;
     for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[s * rows + row].x);
     const float ref = m == -INFINITY ? 0.0f : m;
-    float acc[2] = {0.0f, 0.0f};
+    float4 acc = make_float4(0, 0, 0, 0);
     for (int s = 0; s < splits; ++s) {
         const float2 ml = part_ml[s * rows + row];
-        const float f = exp_of(ml.x - ref);
+        const float f = pow2(ml.x - ref);
+        const float4 v = load4(part + (s * rows + row) * a.D, c, a.D);
         l += ml.y * f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-            if (lane + 64 * c < a.D) acc[c] += part[(s * rows + row) * a.D + lane + 64 * c] * f;
+        acc = make_float4(acc.x + v.x * f, acc.y + v.y * f, acc.z + v.z * f, acc.w + v.w * f);
     }
     const bool saw = valid && l != 0.0f;
     const float inv = 1.0f / l;
-    float* out = o + b * a.q_b + h * a.q_h + query * a.q_t;
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-        if (lane + 64 * c < a.D) out[lane + 64 * c] = saw ? acc[c] * inv : 0.0f;
-    if (lane == 0) lse[row] = saw ? m + logf(l) : -INFINITY;
+    store4(o + b * a.q_b + h * a.q_h + query * a.q_t, c, a.D, saw ? acc.x * inv : 0.0f, saw ? acc.y * inv : 0.0f, saw ? acc.z * inv : 0.0f,
+           saw ? acc.w * inv : 0.0f);
+    if (c == 0) lse[row] = saw ? log_sum(m, l) : -INFINITY;
 }
 
 // ---------------------------------------------------------------- forward: a few queries against many keys
-
-// Sum over aligned groups of N lanes (8, 16 or 32); every lane gets it.
-template <int N>
-__device__ __forceinline__ float group_sum(float x) {
-    auto add = [](float v, auto ctrl) {
-        return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true));
-    };
-    x = add(x, std::integral_constant<int, 0xB1>());       // lane ^ 1
-    x = add(x, std::integral_constant<int, 0x4E>());       // lane ^ 2
-    x = add(x, std::integral_constant<int, 0x141>());      // mirrored within 8: the other quad
-    if (N >= 16) x = add(x, std::integral_constant<int, 0x140>());      // mirrored within 16: the other eight
-    if (N >= 32) x += __shfl_xor(x, 16);
-    return x;
-}
 
 // One workgroup per head and run of keys; up to NQ queries share what is read.  DP / 4 lanes hold a
 // key's columns, so a wavefront's load covers 256 / DP neighbouring keys, and kTokenUnroll of those
@@ -630,7 +664,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
     extern __shared__ float win[];
     __shared__ float4 join_o[NQ][4][LANES];
     __shared__ float2 join_ml[NQ][4];
-    const Where w = where(a, splits, true);
+    const Where w = where(a, splits, kByHead);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % LANES * 4, group = lane / LANES, split = w.tile;
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
     int last = k_end;
@@ -644,12 +678,13 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
     __syncthreads();
     const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
     const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
+    const float qs = a.scale * kLog2e;
     float4 q[NQ], acc[NQ];
     float m[NQ], l[NQ];
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
         q[i] = i < q_end ? load4(a.q + w.b * a.q_b + w.h * a.q_h + i * a.q_t, c, a.D) : make_float4(0, 0, 0, 0);
-        q[i] = make_float4(q[i].x * a.scale, q[i].y * a.scale, q[i].z * a.scale, q[i].w * a.scale);
+        q[i] = make_float4(q[i].x * qs, q[i].y * qs, q[i].z * qs, q[i].w * qs);
         acc[i] = make_float4(0, 0, 0, 0);
         m[i] = -INFINITY;
         l[i] = 0.0f;
@@ -677,13 +712,13 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
                 if (j >= last || (a.causal && j > i + a.q_offset)) s[u] = -INFINITY;
                 top = fmaxf(top, s[u]);
             }
-            const float ref = top == -INFINITY ? 0.0f : top, f = exp_of(m[i] - ref);
+            const float ref = top == -INFINITY ? 0.0f : top, f = pow2(m[i] - ref);
             m[i] = top;
             l[i] *= f;
             acc[i] = make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f);
 #pragma unroll
             for (int u = 0; u < kTokenUnroll; ++u) {
-                const float p = exp_of(s[u] - ref);
+                const float p = pow2(s[u] - ref);
                 l[i] += p;
                 acc[i] = make_float4(acc[i].x + p * vv[u].x, acc[i].y + p * vv[u].y, acc[i].z + p * vv[u].z, acc[i].w + p * vv[u].w);
             }
@@ -694,7 +729,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
         float top = m[i];
 #pragma unroll
         for (int d = LANES; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        const float f = exp_of(m[i] - (top == -INFINITY ? 0.0f : top));
+        const float f = pow2(m[i] - (top == -INFINITY ? 0.0f : top));
         l[i] *= f;
         acc[i] = make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f);
 #pragma unroll
@@ -717,7 +752,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
         const float ref = top == -INFINITY ? 0.0f : top;
         float4 r = make_float4(0, 0, 0, 0);
         for (int o4 = 0; o4 < 4; ++o4) {
-            const float f = exp_of(join_ml[i][o4].x - ref);
+            const float f = pow2(join_ml[i][o4].x - ref);
             const float4 v = join_o[i][o4][col];
             sum += join_ml[i][o4].y * f;
             r = make_float4(r.x + v.x * f, r.y + v.y * f, r.z + v.z * f, r.w + v.w * f);
@@ -732,7 +767,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
             const float inv = 1.0f / sum;
             store4(o + w.b * a.q_b + w.h * a.q_h + i * a.q_t, col * 4, a.D, saw ? r.x * inv : 0.0f, saw ? r.y * inv : 0.0f, saw ? r.z * inv : 0.0f,
                    saw ? r.w * inv : 0.0f);
-            if (col == 0) lse[stat] = saw ? top + logf(sum) : -INFINITY;
+            if (col == 0) lse[stat] = saw ? log_sum(top, sum) : -INFINITY;
         }
     }
 }
@@ -741,27 +776,29 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
 
 // gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads, 2) void attn_bwd_q_kernel(Attn a, Ranges ranges, const float* o, const float* lse, const float* go, float* gq, float* delta,
-                                                                 float* part_table, int tiles) {
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_kernel(Attn a, Ranges ranges, const float* o, const float* lse, const float* go, float* gq,
+    float* part, float* delta, float* part_table, int tiles, int splits) {
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *kt = lds, *kc = kt + Tile<DP>::kRowBytes / 2, *vt = kc + Tile<DP>::kColBytes / 2;
-    float* square = reinterpret_cast<float*>(vt + Tile<DP>::kRowBytes / 2);      // [wavefront][32][36]
+    float* square = reinterpret_cast<float*>(vt + Tile<DP>::kRowBytes / 2);      // [wavefront][32][32]
     float* win = square + (BIAS ? 4 * kSquare : 0);
     const int window = BIAS ? bias_window(a.rule) : 0;
     float* diag = win + window;      // [wavefront][window]: sums of ds by relative position
-    const Where w = where(a, tiles, true);
-    const int q0 = w.tile * kAttnCols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qw = q0 + wave * 32, query = qw + (lane & 31);
+    const Where w = where(a, tiles * splits, kHeavyLast);
+    const int split = w.tile % splits, q0 = w.tile / splits * kAttnCols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qw = q0 + wave * 32, query = qw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
     const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
     const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
     const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
     if (BIAS) {
-        fill_bias(a, w.h, win);
+        copy_bias(a, ranges, w.h, win);
         for (int s = threadIdx.x; s < 4 * window; s += kAttnThreads) diag[s] = 0.0f;
     }
     int last = k_end;
     if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
     if (q0 >= q_end) last = 0;
+    const int run = (last + kAttnRows * splits - 1) / (kAttnRows * splits) * kAttnRows, first = split * run;
+    last = min(last, first + run);
     const bool valid = query < q_end;
     const long stat = ((long)w.b * a.H + w.h) * a.Tq + query;
     float dl = 0.0f;
@@ -776,13 +813,13 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_bwd_q_kernel(Attn a, Ran
     const HeadScales sc = head_scales(a, ranges, w);
     Column<DP> qcol, gcol;
     qcol.load(a.q + qrow, valid, a.D);
-    qcol.split(sc.q);
+    qcol.split(sc.q, 1.0f);
     gcol.load(go + qrow, valid, a.D);
-    gcol.split(sc.g);
+    gcol.split(sc.g, -1.0f);
     const float unscale = sc.score(a), dscale = sc.dp(a) * sc.ds;      // ds is formed times sc.ds
-    if (query < a.Tq && lane < 32) delta[stat] = dl;
+    if (query < a.Tq && lane < 32 && split == 0) delta[stat] = dl;
     dl *= sc.ds;
-    float row_lse = valid ? lse[stat] : INFINITY;
+    float row_lse = valid ? to_log2(lse[stat]) : INFINITY;
     if (row_lse == -INFINITY) row_lse = INFINITY;      // a row that saw nothing: every probability is 0
     RngState rng = {};
     unsigned long long group0 = 0;
@@ -792,26 +829,25 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_bwd_q_kernel(Attn a, Ran
     }
     float far_before = 0.0f, far_after = 0.0f;
     v16f acc[DP / 32] = {};
+    const typename Tile<DP>::Offsets off(a.k_t, a.D);
     Tile<DP> kr, vr;
-    if (last > 0) {
-        kr.load(kbase, a.k_t, 0, last, a.D);
-        vr.load(vbase, a.k_t, 0, last, a.D);
+    if (first < last) {
+        kr.load(off, kbase, a.k_t, first, last, a.D);
+        vr.load(off, vbase, a.k_t, first, last, a.D);
     }
-    for (int j0 = 0; j0 < last; j0 += kAttnRows) {
-        kr.clear(j0, last);
-        vr.clear(j0, last);
+    for (int j0 = first; j0 < last; j0 += kAttnRows) {
         __syncthreads();
         kr.template store<true, true>(kt, kc, sc.k);
         vr.template store<true, false>(vt, nullptr, sc.v);
         __syncthreads();
         if (j0 + kAttnRows < last) {
-            kr.load(kbase, a.k_t, j0 + kAttnRows, last, a.D);
-            vr.load(vbase, a.k_t, j0 + kAttnRows, last, a.D);
+            kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
+            vr.load(off, vbase, a.k_t, j0 + kAttnRows, last, a.D);
         }
         if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;
         const int rel0 = j0 - qw - a.q_offset;
-        v16f s = product_rows<DP>(kt, qcol);
-        v16f dp = product_rows<DP>(vt, gcol);
+        v16f s = product_rows<DP, false>(kt, qcol);
+        v16f dp = product_rows<DP, true>(vt, gcol);
         scores<BIAS>(s, unscale, a.rule, win, rel0, 1);
         const bool edge = j0 + kAttnRows > k_end || qw + 32 > q_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset);
         if (DROP) {
@@ -825,7 +861,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_bwd_q_kernel(Attn a, Ran
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float p = exp_of(s[r] - row_lse);
+            const float p = pow2(s[r] - row_lse);
             s[r] = edge && (!valid || hidden(a, j0 + tile_row(r), query, k_end)) ? 0.0f : p * __builtin_fmaf(dp[r], dscale, -dl);
         }
         if (BIAS) {
@@ -836,18 +872,18 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_bwd_q_kernel(Attn a, Ran
                 (rel0 < 0 ? far_before : far_after) += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             } else {
                 // Sums along the tile's 63 diagonals: element (row, column) goes to row (row - column) mod 32 of a
-                // 32 x 36 square, where lane l finds half of diagonals l and l - 32.  (Atomic additions in LDS
+                // 32 x 32 square (its 16-byte units permuted by row), where lane l finds half of diagonals l and l - 32.  (Atomic additions in LDS
                 // take about 180 cycles an instruction: 2900 for this tile, all wavefronts together.)
                 float* sq = square + wave * kSquare;
                 wave_lds_fence();
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sq[((tile_row(r) - lane) & 31) * kSquarePitch + tile_row(r)] = s[r];
+                for (int r = 0; r < 16; ++r) sq[square_at((tile_row(r) - lane) & 31, tile_row(r))] = s[r];
                 wave_lds_fence();
                 const int d = lane & 31, row0 = 16 * (lane >> 5);
                 float same = 0.0f, less = 0.0f;       // diagonals d and d - 32
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float4 v = *reinterpret_cast<const float4*>(sq + d * kSquarePitch + row0 + 4 * i);
+                    const float4 v = *reinterpret_cast<const float4*>(sq + square_at(d, row0 + 4 * i));
                     const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
@@ -865,11 +901,12 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_bwd_q_kernel(Attn a, Ran
         product_cols<DP>(acc, kc, s);
     }
     if (query < a.Tq) {
+        float* out = splits > 1 ? part + ((long)split * a.B * a.H * a.Tq + stat) * a.D : gq + qrow;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                store_scaled(gq + qrow, 32 * d + 8 * g + 4 * (lane >> 5), a.D, acc[d], g, valid, a.scale * reciprocal_power(sc.k) * reciprocal_power(sc.ds));
+                store_scaled(out, 32 * d + 8 * g + 4 * (lane >> 5), a.D, acc[d], g, valid, a.scale * reciprocal_power(sc.k) * reciprocal_power(sc.ds));
     }
     if (BIAS) {
         // by bucket: the window's sums of the four wavefronts and the far tiles' in the window's ends
@@ -890,10 +927,13 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_bwd_q_kernel(Attn a, Ran
             bucket[s] = bucket_of(a.rule, s - reach);
         }
         __syncthreads();
-        for (int c = threadIdx.x; c < a.rule.buckets; c += kAttnThreads) {
+        // 8 neighbouring lanes share a bucket's sum (buckets <= 256: eight rounds of 32 at most)
+        for (int c = threadIdx.x >> 3; c < a.rule.buckets; c += kAttnThreads / 8) {
             float sum = 0.0f;
-            for (int s = 0; s < window; ++s) sum += bucket[s] == c ? win[s] : 0.0f;
-            part_table[(((long)w.b * tiles + w.tile) * a.H + w.h) * a.rule.buckets + c] = sum * reciprocal_power(sc.ds);
+            for (int s = threadIdx.x & 7; s < window; s += 8) sum += bucket[s] == c ? win[s] : 0.0f;
+            sum = group_sum<8>(sum);
+            if ((threadIdx.x & 7) == 0)
+                part_table[(((long)w.b * tiles * splits + w.tile) * a.H + w.h) * a.rule.buckets + c] = sum * reciprocal_power(sc.ds);
         }
     }
 }
@@ -916,56 +956,59 @@ __global__ __launch_bounds__(kAttnThreads) void attn_table_kernel(const float* p
 // ---------------------------------------------------------------- backward: keys
 
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, Ranges ranges, const float* lse, const float* delta, const float* go, float* gk, float* gv, int tiles) {
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, Ranges ranges, const float* lse, const float* delta, const float* go, float* gk,
+    float* gv, float* part, int tiles, int splits) {
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *qt = lds, *gt = qt + Tile<DP>::kRowBytes / 2, *qc = gt + Tile<DP>::kRowBytes / 2, *gc = qc + Tile<DP>::kColBytes / 2;
     float* stats = reinterpret_cast<float*>(gc + Tile<DP>::kColBytes / 2);
     unsigned* bits = reinterpret_cast<unsigned*>(stats + 2 * kAttnRows);      // [wavefront][half][query]: 16 keep bits each
     float* win = stats + 2 * kAttnRows + (DROP ? kAttnThreads : 0);
-    const Where w = where(a, tiles, false);
-    const int k0 = w.tile * kAttnCols, lane = threadIdx.x & 63, kw = k0 + (threadIdx.x >> 6) * 32, key = kw + (lane & 31);
+    const Where w = where(a, tiles * splits, kHeavyFirst);
+    const int split = w.tile % splits, k0 = w.tile / splits * kAttnCols, lane = threadIdx.x & 63, kw = k0 + (threadIdx.x >> 6) * 32, key = kw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
     const float* qbase = a.q + w.b * a.q_b + w.h * a.q_h;
     const float* gbase = go + w.b * a.q_b + w.h * a.q_h;
     const long krow = w.b * a.k_b + w.h * a.k_h + key * a.k_t;
-    if (BIAS) fill_bias(a, w.h, win);
+    if (BIAS) copy_bias(a, ranges, w.h, win);
     // queries this workgroup walks: from the first that sees its first key
     int first = 0, last = q_end;
     if (a.causal) first = max(0, k0 - a.q_offset) / kAttnRows * kAttnRows;
     if (k0 >= k_end) last = 0;
+    const int run = (max(0, last - first) + kAttnRows * splits - 1) / (kAttnRows * splits) * kAttnRows;
+    first += split * run;
+    last = min(last, first + run);
     const bool valid = key < k_end;
     const HeadScales sc = head_scales(a, ranges, w);
-    const float unscale = sc.score(a), dscale = sc.dp(a) * sc.ds * 0x1p-14f, lscale = sc.ds * 0x1p-14f;      // p carries 2^14
+    const float unscale = sc.score(a), dscale = sc.dp(a) * sc.ds * 0x1p-14f, lscale = sc.ds * 0x1p-14f;
     Column<DP> kcol, vcol;
     kcol.load(a.k + krow, valid, a.D);
-    kcol.split(sc.k);
+    kcol.split(sc.k, 1.0f);
     vcol.load(a.v + krow, valid, a.D);
-    vcol.split(sc.v);
+    vcol.split(sc.v, -1.0f);
     const long stat0 = ((long)w.b * a.H + w.h) * a.Tq;
     RngState rng = {};
     if (DROP) rng = load_rng(a.rng, a.channel);
     v16f acck[DP / 32] = {}, accv[DP / 32] = {};
+    const typename Tile<DP>::Offsets off(a.q_t, a.D);
     Tile<DP> qr, gr;
     if (first < last) {
-        qr.load(qbase, a.q_t, first, last, a.D);
-        gr.load(gbase, a.q_t, first, last, a.D);
+        qr.load(off, qbase, a.q_t, first, last, a.D);
+        gr.load(off, gbase, a.q_t, first, last, a.D);
     }
     for (int i0 = first; i0 < last; i0 += kAttnRows) {
-        qr.clear(i0, last);
-        gr.clear(i0, last);
         __syncthreads();
         qr.template store<true, true>(qt, qc, sc.q);
         gr.template store<true, true>(gt, gc, sc.g);
         if (threadIdx.x < kAttnRows) {
             const int i = i0 + threadIdx.x;
             const float v = i < last ? lse[stat0 + i] : INFINITY;
-            stats[threadIdx.x] = v == -INFINITY ? INFINITY : v;
+            stats[threadIdx.x] = v == -INFINITY ? INFINITY : to_log2(v) - 14.0f;      // p carries 2^14
             stats[kAttnRows + threadIdx.x] = i < last ? delta[stat0 + i] * lscale : 0.0f;
         }
         __syncthreads();
         if (i0 + kAttnRows < last) {
-            qr.load(qbase, a.q_t, i0 + kAttnRows, last, a.D);
-            gr.load(gbase, a.q_t, i0 + kAttnRows, last, a.D);
+            qr.load(off, qbase, a.q_t, i0 + kAttnRows, last, a.D);
+            gr.load(off, gbase, a.q_t, i0 + kAttnRows, last, a.D);
         }
         if (kw >= k_end || (a.causal && kw > i0 + 31 + a.q_offset)) continue;
         const int rel0 = kw - i0 - a.q_offset;
@@ -990,14 +1033,14 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
 #pragma unroll
             for (int r = 0; r < 16; ++r) word[r] = mine[32 * (c >> 2 & 1) + tile_row(r)] >> bit & 1u;
         }
-        v16f s = product_rows<DP>(qt, kcol);
-        v16f dp = product_rows<DP>(gt, vcol);
+        v16f s = product_rows<DP, false>(qt, kcol);
+        v16f dp = product_rows<DP, true>(gt, vcol);
         scores<BIAS>(s, unscale, a.rule, win, rel0, -1);
         const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + a.q_offset);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int row = tile_row(r);
-            float p = exp_scaled(s[r] - stats[row]);
+            float p = pow2(s[r] - stats[row]);
             if (edge && hidden(a, key, i0 + row, k_end)) p = 0.0f;      // rows beyond the queries: p is 0 by their lse
             const bool keep = !DROP || word[r];
             s[r] = keep ? p : 0.0f;
@@ -1007,58 +1050,78 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
         product_cols<DP>(acck, qc, dp);
     }
     if (key >= a.Tk) return;
+    // partial sums: [split][array][head][key][D]
+    const long heads = (long)a.B * a.H, at = (2L * split * heads + w.b * a.H + w.h) * a.Tk + key;
+    float *out_k = splits > 1 ? part + at * a.D : gk + krow, *out_v = splits > 1 ? part + (at + heads * a.Tk) * a.D : gv + krow;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int c = 32 * d + 8 * g + 4 * (lane >> 5);
-            store_scaled(gk + krow, c, a.D, acck[d], g, valid, a.scale * reciprocal_power(sc.q) * reciprocal_power(sc.ds));
-            store_scaled(gv + krow, c, a.D, accv[d], g, valid, 0x1p-14f * reciprocal_power(sc.g) * (DROP ? a.rate.scale : 1.0f));
+            store_scaled(out_k, c, a.D, acck[d], g, valid, a.scale * reciprocal_power(sc.q) * reciprocal_power(sc.ds));
+            store_scaled(out_v, c, a.D, accv[d], g, valid, 0x1p-14f * reciprocal_power(sc.g) * (DROP ? a.rate.scale : 1.0f));
         }
+}
+
+// Adds up the partial gradients of a split axis, in order: part is [split][arrays][head][row][D]; a group of
+// DP / 4 lanes takes a row.
+template <int DP>
+__global__ __launch_bounds__(kAttnThreads) void attn_sum_kernel(Attn a, const float* part, float* out0, float* out1, int T, int splits, long s_b, long s_h, long s_t) {
+    constexpr int LANES = DP / 4;
+    const long rows = (long)a.B * a.H * T, row = (long)blockIdx.x * (kAttnThreads / LANES) + threadIdx.x / LANES, step = rows * a.D * gridDim.y;
+    const int c = threadIdx.x % LANES * 4;
+    if (row >= rows) return;
+    const float* p = part + (blockIdx.y * rows + row) * a.D;
+    float4 s = load4(p, c, a.D);
+    for (int k = 1; k < splits; ++k) {
+        const float4 v = load4(p + k * step, c, a.D);
+        s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    const int head = (int)(row / T), t = (int)(row - (long)head * T);
+    store4((blockIdx.y ? out1 : out0) + head / a.H * s_b + head % a.H * s_h + t * s_t, c, a.D, s.x, s.y, s.z, s.w);
 }
 
 // ---------------------------------------------------------------- launchers
 
-// Chooses the instantiation: head width rounded up, bias, dropout.
-#define ATTN_DISPATCH(KERNEL, ...)                                                          \
-    do {                                                                                    \
-        const bool bias_ = a.table != nullptr, drop_ = a.rate.threshold != 0;               \
-        if (a.D <= 32) ATTN_FLAGS(KERNEL, 32, __VA_ARGS__);                                 \
-        else if (a.D <= 64) ATTN_FLAGS(KERNEL, 64, __VA_ARGS__);                            \
-        else ATTN_FLAGS(KERNEL, 128, __VA_ARGS__);                                          \
-    } while (0)
-#define ATTN_FLAGS(KERNEL, DP, ...)                                                         \
-    do {                                                                                    \
-        if (bias_ && drop_) ATTN_LAUNCH((KERNEL<DP, true, true>), __VA_ARGS__);             \
-        else if (bias_) ATTN_LAUNCH((KERNEL<DP, true, false>), __VA_ARGS__);                \
-        else if (drop_) ATTN_LAUNCH((KERNEL<DP, false, true>), __VA_ARGS__);                \
-        else ATTN_LAUNCH((KERNEL<DP, false, false>), __VA_ARGS__);                          \
-    } while (0)
-// The same for a few queries: one or up to four of them.
-#define ATTN_TOKEN(...)                                                                     \
-    do {                                                                                    \
-        if (a.D <= 32) ATTN_TOKEN_FLAGS(32, __VA_ARGS__);                                   \
-        else if (a.D <= 64) ATTN_TOKEN_FLAGS(64, __VA_ARGS__);                              \
-        else ATTN_TOKEN_FLAGS(128, __VA_ARGS__);                                            \
-    } while (0)
-#define ATTN_TOKEN_FLAGS(DP, ...)                                                           \
-    do {                                                                                    \
-        if (table && a.Tq == 1) ATTN_LAUNCH((attn_token_kernel<DP, 1, true>), __VA_ARGS__); \
-        else if (table) ATTN_LAUNCH((attn_token_kernel<DP, 4, true>), __VA_ARGS__);         \
-        else if (a.Tq == 1) ATTN_LAUNCH((attn_token_kernel<DP, 1, false>), __VA_ARGS__);    \
-        else ATTN_LAUNCH((attn_token_kernel<DP, 4, false>), __VA_ARGS__);                   \
-    } while (0)
-#define ATTN_LAUNCH(KERNEL, ...)                                                            \
-    do {                                                                                    \
-        if (lds_bytes > 65536)                                                              \
-            CGT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes)); \
-        KERNEL<<<grid, kAttnThreads, lds_bytes, st>>>(__VA_ARGS__);                         \
-    } while (0)
+// Calls f(head width rounded up), and f(that, bias, dropout), with types for arguments.
+template <class F>
+static int attn_width(const Attn& a, F f) {
+    if (a.D <= 32) return f(std::integral_constant<int, 32>());
+    if (a.D <= 64) return f(std::integral_constant<int, 64>());
+    return f(std::integral_constant<int, 128>());
+}
+template <class F>
+static int attn_dispatch(const Attn& a, F f) {
+    return attn_width(a, [&](auto width) {
+        const bool bias = a.table != nullptr, drop = a.rate.threshold != 0;
+        if (bias) return drop ? f(width, std::true_type(), std::true_type()) : f(width, std::true_type(), std::false_type());
+        return drop ? f(width, std::false_type(), std::true_type()) : f(width, std::false_type(), std::false_type());
+    });
+}
+template <class... P, class... A>
+static int attn_launch(const char* name, void (*kernel)(P...), long grid, int grid_y, int threads, size_t lds_bytes, hipStream_t st, A... args) {
+    if (lds_bytes > 65536)
+        CGT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes));
+    kernel<<<dim3((unsigned)grid, (unsigned)grid_y), threads, lds_bytes, st>>>(args...);
+    CGT_LAUNCH_CHECK(name);
+    return CGT_AMD_OK;
+}
 
+static int launch_ranges(const Attn& a, const RangeArrays& arrays, int n_arrays, int runs, float2* out, float* window, hipStream_t st) {
+    return attn_width(a, [&](auto width) {
+        return attn_launch("attention ranges", attn_range_kernel<decltype(width)::value>, (long)a.B * a.H * runs, n_arrays + (a.table ? 1 : 0), kAttnThreads, 0,
+                           st, a, arrays, n_arrays, runs, out, window);
+    });
+}
 // Runs of rows whose largest values are found by workgroups of their own: 256 rows or more, 16 at most.
 static int range_runs(long Tq, long Tk) { return (int)std::max(1L, std::min(cdiv(std::max(Tq, Tk), 256), 16L)); }
-static size_t row_bytes(int DP) { return DP == 32 ? Tile<32>::kRowBytes : DP == 64 ? Tile<64>::kRowBytes : Tile<128>::kRowBytes; }
-static size_t col_bytes(int DP) { return DP == 32 ? Tile<32>::kColBytes : DP == 64 ? Tile<64>::kColBytes : Tile<128>::kColBytes; }
+// Into how many runs the walked axis (`rows` long) is cut, so that `whole` workgroups become enough to fill
+// every CU `resident` times (twice as often where a causal mask makes them uneven); runs of `shortest` rows at least.
+static int axis_splits(long whole, long rows, int resident, int causal, long shortest) {
+    if (whole <= 0) return 1;
+    const long want = (long)kNumCU * resident * (causal ? 2 : 1);
+    return (int)std::max(1L, std::min({cdiv(want, whole), rows / shortest, 16L}));
+}
 static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // The rule of the buckets: per side (all of them, or half when positions after the query have their
@@ -1135,16 +1198,16 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
     const bool token = Tq <= 4 && a.rate.threshold == 0;
     const int DP = padded_dim(a.D), tiles = token ? 1 : (int)cdiv(Tq, kAttnCols);
     const long heads = B * H, whole = heads * tiles;
-    // Too few workgroups to fill the chip: the keys are cut too, into runs of 128 at least.
-    const int want = token ? 8 * kNumCU : 2 * kNumCU;
-    const int splits = whole >= want / 2 ? 1 : (int)std::max(1L, std::min({cdiv(want, whole), Tk / 128, 64L}));
+    // Too few workgroups to fill the chip: the keys are cut too.
+    const int splits = token ? (whole >= 4 * kNumCU ? 1 : (int)std::max(1L, std::min({cdiv(8L * kNumCU, whole), Tk / 128, 64L})))
+                             : axis_splits(whole, Tk, DP == 128 ? 2 : 3, a.causal, 512);
     CGT_ARG_CHECK(whole * splits < (1L << 31) && heads * range_runs(Tq, Tk) < (1L << 31), "attention: too many workgroups");
     // workspace: the heads' ranges, then the pieces of a split key axis
     const int runs = range_runs(Tq, Tk);
-    const size_t rows = splits > 1 ? (size_t)heads * Tq * splits : 0, range_floats = token ? 0 : (size_t)heads * runs * 2 * 2;
+    const size_t rows = splits > 1 ? (size_t)heads * Tq * splits : 0, range_floats = token ? 0 : (size_t)heads * runs * 2 * 2 + (table ? bias_window(a.rule) * H : 0) + 2 & ~(size_t)1;
     float* part = nullptr;
     float2* ml = nullptr;
-    Ranges ranges = {nullptr, runs};
+    Ranges ranges = {nullptr, runs, nullptr};
     if (rows + range_floats) {
         float* ws = stream_workspace(stream, kWsAttention, (range_floats + rows * (D + 2)) * sizeof(float), "attention");
         if (!ws) return CGT_AMD_ERR_NOMEM;
@@ -1152,19 +1215,33 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
         ml = reinterpret_cast<float2*>(ws + range_floats);
         part = ws + range_floats + 2 * rows;
     }
-    if (!token && Tk > 0) {
-        const RangeArrays arrays = {{k, v}, {1, 1}};
-        attn_range_kernel<<<dim3((unsigned)(heads * runs), 2), kAttnThreads, 0, st>>>(a, arrays, runs, const_cast<float2*>(ranges.at));
-        CGT_LAUNCH_CHECK("attention ranges");
+    if (!token) {      // (no keys: no rows are read, but the kernel still takes its scales and bias from there)
+        float* window = reinterpret_cast<float*>(const_cast<float2*>(ranges.at)) + heads * runs * 2 * 2;
+        ranges.window = window;
+        if (int rc = launch_ranges(a, {{k, v}, {1, 1}, {0, 0}}, 2, runs, const_cast<float2*>(ranges.at), window, st)) return rc;
     }
-    const size_t lds_bytes = (token ? 0 : row_bytes(DP) + col_bytes(DP)) + (table ? bias_window(a.rule) * sizeof(float) : 0);
-    const dim3 grid((unsigned)(whole * splits));
-    if (token) ATTN_TOKEN(a, o, lse, part, ml, splits);
-    else ATTN_DISPATCH(attn_fwd_kernel, a, ranges, o, lse, part, ml, tiles, splits);
-    CGT_LAUNCH_CHECK("attention forward");
+    const size_t window_bytes = table ? bias_window(a.rule) * sizeof(float) : 0;
+    const int rc = attn_dispatch(a, [&](auto width, auto bias, auto drop) {
+        constexpr int W = decltype(width)::value;
+        constexpr bool bias_ = decltype(bias)::value, drop_ = decltype(drop)::value;
+        if constexpr (!drop_) {
+            if (token)
+                return a.Tq == 1 ? attn_launch("attention (one query)", attn_token_kernel<W, 1, bias_>, whole * splits, 1, kAttnThreads, window_bytes, st,
+                                               a, o, lse, part, ml, splits)
+                                 : attn_launch("attention (few queries)", attn_token_kernel<W, 4, bias_>, whole * splits, 1, kAttnThreads, window_bytes, st,
+                                               a, o, lse, part, ml, splits);
+        }
+        const size_t lds_bytes = Tile<W>::kRowBytes + Tile<W>::kColBytes + window_bytes;
+        return attn_launch("attention forward", attn_fwd_kernel<W, bias_, drop_>, whole * splits, 1, kAttnThreads, lds_bytes, st, a, ranges, o, lse, part, ml,
+                           tiles, splits);
+    });
+    if (rc != CGT_AMD_OK) return rc;
     if (splits > 1) {
-        attn_join_kernel<<<dim3((unsigned)cdiv(heads * Tq, 4)), kAttnThreads, 0, st>>>(a, o, lse, part, ml, splits);
-        CGT_LAUNCH_CHECK("attention join");
+        const int rc = attn_width(a, [&](auto width) {
+            constexpr int W = decltype(width)::value;
+            return attn_launch("attention join", attn_join_kernel<W>, cdiv(heads * Tq, kAttnThreads / (W / 4)), 1, kAttnThreads, 0, st, a, o, lse, part, ml, splits);
+        });
+        if (rc != CGT_AMD_OK) return rc;
     }
     return CGT_AMD_OK;
 }
@@ -1193,31 +1270,55 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
     const int DP = padded_dim(a.D), qtiles = (int)cdiv(Tq, kAttnCols), ktiles = (int)cdiv(Tk, kAttnCols);
     const int runs = range_runs(Tq, Tk);
     CGT_ARG_CHECK(heads * qtiles < (1L << 31) && heads * ktiles < (1L << 31) && heads * runs < (1L << 31), "attention backward: too many workgroups");
-    const long parts = B * qtiles;
-    const size_t range_floats = (size_t)heads * runs * 4 * 2, need = range_floats + (size_t)(heads * Tq + (table ? parts * H * buckets : 0));
-    float* ws = stream_workspace(stream, kWsAttention, need * sizeof(float), "attention backward");
+    const int qsplits = axis_splits(heads * qtiles, Tk, DP == 128 ? 1 : 2, a.causal, 256), ksplits = axis_splits(heads * ktiles, Tq, DP == 128 ? 1 : 2, a.causal, 256);
+    // workspace: ranges, row products, the table's partial rows, partial gradients (of the queries, then of the keys)
+    const long parts = B * qtiles * qsplits;
+    const size_t window_floats = table ? (size_t)bias_window(a.rule) * H : 0, range_floats = (size_t)heads * runs * 4 * 2 + window_floats;
+    const size_t table_floats = table ? (size_t)(parts * H * buckets) : 0;
+    const size_t part_floats = std::max(qsplits > 1 ? (size_t)qsplits * heads * Tq * D : 0, ksplits > 1 ? (size_t)ksplits * 2 * heads * Tk * D : 0);
+    float* ws = stream_workspace(stream, kWsAttention, (range_floats + heads * Tq + table_floats + part_floats) * sizeof(float), "attention backward");
     if (!ws) return CGT_AMD_ERR_NOMEM;
-    float *delta = ws + range_floats, *part = delta + heads * Tq;
-    const Ranges ranges = {reinterpret_cast<const float2*>(ws), runs};
-    const RangeArrays arrays = {{k, v, q, go}, {1, 1, 0, 0}};
-    attn_range_kernel<<<dim3((unsigned)(heads * runs), 4), kAttnThreads, 0, st>>>(a, arrays, runs, reinterpret_cast<float2*>(ws));
-    CGT_LAUNCH_CHECK("attention backward (ranges)");
-    const int window = table ? bias_window(a.rule) : 0;
-    {
-        const size_t lds_bytes = 2 * row_bytes(DP) + col_bytes(DP) + (table ? 4 * kSquare + 5 * window : 0) * sizeof(float);
-        const dim3 grid((unsigned)(heads * qtiles));
-        ATTN_DISPATCH(attn_bwd_q_kernel, a, ranges, o, lse, go, gq, delta, part, qtiles);
-        CGT_LAUNCH_CHECK("attention backward (queries)");
+    float *delta = ws + range_floats, *part_table = delta + heads * Tq, *part = part_table + table_floats;
+    const Ranges ranges = {reinterpret_cast<const float2*>(ws), runs, ws + range_floats - window_floats};
+    int rc = launch_ranges(a, {{k, v, q, go}, {1, 1, 0, 0}, {0, 1, 0, 1}}, 4, runs, reinterpret_cast<float2*>(ws), ws + range_floats - window_floats, st);
+    if (rc != CGT_AMD_OK) return rc;
+    const size_t window_bytes = table ? bias_window(a.rule) * sizeof(float) : 0;
+    rc = attn_dispatch(a, [&](auto width, auto bias, auto drop) {
+        constexpr int W = decltype(width)::value;
+        constexpr bool bias_ = decltype(bias)::value, drop_ = decltype(drop)::value;
+        const size_t lds_bytes = 2 * Tile<W>::kRowBytes + Tile<W>::kColBytes + (bias_ ? 4 * kSquare * sizeof(float) : 0) + 5 * window_bytes;
+        return attn_launch("attention backward (queries)", attn_bwd_q_kernel<W, bias_, drop_>, heads * qtiles * qsplits, 1, kAttnThreads, lds_bytes, st, a, ranges,
+                           o, lse, go, gq, part, delta, part_table, qtiles, qsplits);
+    });
+    if (rc != CGT_AMD_OK) return rc;
+    auto add_up = [&](float* out0, float* out1, long T, int splits, long s_b, long s_h, long s_t) {
+        return attn_width(a, [&](auto width) {
+            constexpr int W = decltype(width)::value;
+            return attn_launch("attention backward (partial sums)", attn_sum_kernel<W>, cdiv(heads * T, kAttnThreads / (W / 4)), out1 ? 2 : 1, kAttnThreads, 0, st,
+                               a, part, out0, out1, (int)T, splits, s_b, s_h, s_t);
+        });
+    };
+    if (qsplits > 1) {
+        rc = add_up(gq, nullptr, Tq, qsplits, a.q_b, a.q_h, a.q_t);
+        if (rc != CGT_AMD_OK) return rc;
     }
     if (table) {
-        attn_table_kernel<<<dim3((unsigned)cdiv(H * buckets, 16)), kAttnThreads, 0, st>>>(part, (int)parts, a.H, a.rule.buckets, gtable);
+        attn_table_kernel<<<dim3((unsigned)cdiv(H * buckets, 16)), kAttnThreads, 0, st>>>(part_table, (int)parts, a.H, a.rule.buckets, gtable);
         CGT_LAUNCH_CHECK("attention backward (table)");
     }
     if (ktiles) {
-        const size_t lds_bytes = 2 * row_bytes(DP) + 2 * col_bytes(DP) + (2 * kAttnRows + (a.rate.threshold ? kAttnThreads : 0) + window) * sizeof(float);
-        const dim3 grid((unsigned)(heads * ktiles));
-        ATTN_DISPATCH(attn_bwd_kv_kernel, a, ranges, lse, delta, go, gk, gv, ktiles);
-        CGT_LAUNCH_CHECK("attention backward (keys)");
+        rc = attn_dispatch(a, [&](auto width, auto bias, auto drop) {
+            constexpr int W = decltype(width)::value;
+            constexpr bool bias_ = decltype(bias)::value, drop_ = decltype(drop)::value;
+            const size_t lds_bytes = 2 * Tile<W>::kRowBytes + 2 * Tile<W>::kColBytes + (2 * kAttnRows + (drop_ ? kAttnThreads : 0)) * sizeof(float) + window_bytes;
+            return attn_launch("attention backward (keys)", attn_bwd_kv_kernel<W, bias_, drop_>, heads * ktiles * ksplits, 1, kAttnThreads, lds_bytes, st, a, ranges,
+                               lse, delta, go, gk, gv, part, ktiles, ksplits);
+        });
+        if (rc != CGT_AMD_OK) return rc;
+        if (ksplits > 1) {
+            rc = add_up(gk, gv, Tk, ksplits, a.k_b, a.k_h, a.k_t);
+            if (rc != CGT_AMD_OK) return rc;
+        }
     }
     return CGT_AMD_OK;
 }
