@@ -15,20 +15,22 @@
 // they run in.
 //
 // Matrix products run at float32 accuracy on the fp16 matrix cores: an operand, times a power of two
-// that brings the largest of its head's values to 2^14, is cut into two fp16 terms, x = h + l (l is the
+// that brings the largest of its head's values to [2^14, 2^15), is cut into two fp16 terms, x = h + l (l is the
 // rounded rest: 22 bits and the sign), and the products l h, h l, h h are accumulated in float32.  Three
 // v_mfma_f32_32x32x16_f16 do in 3 x 32 cycles what eight v_mfma_f32_32x32x2_f32 do in 8 x 64, and the
 // vector units work beside them (fp32 matrix instructions keep them busy).  Measured on products of
 // 128 (64) normal values: error 1.1e-7 (1.0e-7) of the results' rms, 2.0e-7 (1.4e-7) with the fp32
 // instructions.  Values keep all 22 bits down to 2^-17 of the largest of their head, and an
 // absolute 2^-39 of it below; the largest values of a head are found by a kernel that runs first.
-// An infinite q, k, v or go makes NaN of what it reaches.
+// (Heads whose largest value is below 2^-100 lose digits as fp16's subnormals do.)  Nothing is read behind
+// the lengths.  A NaN or infinity in a row of q makes that row NaN, one in a row of k or v that the walk
+// meets all of its head: a key that a causal mask hides has probability 0, and 0 * NaN is NaN.
 //
 // A wavefront owns 32 columns (queries in the forward and the first backward kernel, keys in the
 // second) and forms the *transposed* score tile, rows = the other side: lane l then holds, for
 // column l % 32, rows 8 g + 4 (l / 32) + t in register 4 g + t.  With the k positions of the next
 // product's 16-wide step taken in the order (row 8 b + 4 half + t at position 8 half + 4 b + t)
-// the score tile, cut into its three terms, is that product's B operand as it stands, with no
+// the score tile, cut into its two terms, is that product's B operand as it stands, with no
 // exchange between lanes; the other operand is laid out in that order when it is put into LDS.
 #include "random.h"
 #include <algorithm>
@@ -421,9 +423,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_range_kernel(Attn a, RangeA
     __shared__ float2 join[4];
     const int n = blockIdx.y;
     if (n == n_arrays) {
-        const int size = bias_window(a.rule), total = size * a.H;
-        for (int i = blockIdx.x * kAttnThreads + threadIdx.x; i < total; i += gridDim.x * kAttnThreads)
-            window[i] = to_log2(a.table[(long)bucket_of(a.rule, i % size - bias_reach(a.rule)) * a.H + i / size]);
+        const int size = bias_window(a.rule);
+        const long total = (long)size * a.H;
+        for (long i = (long)blockIdx.x * kAttnThreads + threadIdx.x; i < total; i += (long)gridDim.x * kAttnThreads)
+            window[i] = to_log2(a.table[(long)bucket_of(a.rule, (int)(i % size) - bias_reach(a.rule)) * a.H + i / size]);
         return;
     }
     const int head = blockIdx.x / runs, at = blockIdx.x % runs, b = head / a.H, h = head % a.H, keys = arrays.keys[n], with_norm = arrays.norm[n];
@@ -459,7 +462,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_range_kernel(Attn a, RangeA
             top = fmaxf(top, join[i].x);
             norm = fmaxf(norm, join[i].y);
         }
-        out[(long)n * gridDim.x + blockIdx.x] = make_float2(top, sqrtf(norm));
+        // squares that left the range of floats: the norm is at most sqrt(D) times the largest value
+        out[(long)n * gridDim.x + blockIdx.x] = make_float2(top, norm > 1e-30f && norm < 1e37f ? sqrtf(norm) : top * sqrtf((float)a.D));
     }
 }
 struct Ranges {
@@ -623,25 +627,53 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     if (half4 == 0) lse[stat] = saw ? log_sum(ref, l) : -INFINITY;
 }
 
-// o and lse from the pieces of a split key axis, joined in order.  A group of DP / 4 lanes takes a row.
-template <int DP>
+// o and lse from the pieces of a split key axis.  DP / 4 lanes take a row's columns, TEAMS such groups a row: team t
+// sums pieces t, t + TEAMS, ... in order, then the teams' sums are added in order through LDS.  One team a row while
+// there are few pieces, the workgroup's 256 threads a row where one team would walk many, each a trip to memory.  Both
+// sides, of the whole call (64 columns): one token, 16 heads, 8192 keys in 64 pieces 41 us with one team, 19 with 16;
+// 4 x 128 queries, 32 pieces 35 / 31; 8 heads of 4096 queries in 3 pieces 148 / 174, of 1024 in 4 pieces 35 / 42.
+constexpr int kJoinTeams = 6;      // pieces from which a row gets the workgroup
+template <int DP, int TEAMS>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(Attn a, float* o, float* lse, const float* part, const float2* part_ml, int splits) {
-    constexpr int LANES = DP / 4;
-    const long rows = (long)a.B * a.H * a.Tq, row = (long)blockIdx.x * (kAttnThreads / LANES) + threadIdx.x / LANES;
-    if (row >= rows) return;
-    const int c = threadIdx.x % LANES * 4, head = (int)(row / a.Tq), query = (int)(row - (long)head * a.Tq);
+    constexpr int LANES = DP / 4, ROWS = kAttnThreads / (LANES * TEAMS);
+    __shared__ float4 sums[TEAMS > 1 ? TEAMS : 1][LANES];
+    __shared__ float weights[TEAMS];
+    const long rows = (long)a.B * a.H * a.Tq, row = (long)blockIdx.x * ROWS + threadIdx.x / (LANES * TEAMS);
+    if (row >= rows) return;      // (TEAMS > 1: a row a workgroup, so all of it or none)
+    const int team = threadIdx.x / LANES % TEAMS, c = threadIdx.x % LANES * 4, head = (int)(row / a.Tq), query = (int)(row - (long)head * a.Tq);
     const int b = head / a.H, h = head % a.H;
     const bool valid = query < length_of(a.q_lengths, b, a.Tq);
     float m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[s * rows + row].x);
+    if constexpr (TEAMS > 1) {
+        for (int s = threadIdx.x & 63; s < splits; s += kWave) m = fmaxf(m, part_ml[s * rows + row].x);
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    } else {
+        for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[s * rows + row].x);
+    }
     const float ref = m == -INFINITY ? 0.0f : m;
     float4 acc = make_float4(0, 0, 0, 0);
-    for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+    for (int s = team; s < splits; s += TEAMS) {
         const float2 ml = part_ml[s * rows + row];
         const float f = pow2(ml.x - ref);
         const float4 v = load4(part + (s * rows + row) * a.D, c, a.D);
         l += ml.y * f;
         acc = make_float4(acc.x + v.x * f, acc.y + v.y * f, acc.z + v.z * f, acc.w + v.w * f);
+    }
+    if constexpr (TEAMS > 1) {
+        sums[team][threadIdx.x % LANES] = acc;
+        if (c == 0) weights[team] = l;
+        __syncthreads();
+        if (team) return;
+        acc = make_float4(0, 0, 0, 0);
+        l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < TEAMS; ++t) {
+            const float4 v = sums[t][threadIdx.x % LANES];
+            l += weights[t];
+            acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+        }
     }
     const bool saw = valid && l != 0.0f;
     const float inv = 1.0f / l;
@@ -656,7 +688,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(Attn a, float* 
 // key's columns, so a wavefront's load covers 256 / DP neighbouring keys, and kTokenUnroll of those
 // are in flight at once.  Every group of lanes keeps a running maximum, sum and result of its own
 // keys; they are joined at the end, first in the wavefront, then through LDS, then (splits > 1) by
-// attn_join_kernel.  No matrix instructions: with a few rows the time is that of reading k and v.
+// attn_join_kernel.  No matrix instructions: up to four rows the time is that of reading k and v (one
+// token of 16 sequences of 16 heads against 8192 keys, 64 columns, 1.07 GB: 188 us, 5.7 TB/s; four tokens
+// 203 us), with eight the vector units bound it (268 us).
 constexpr int kTokenUnroll = 4;
 template <int DP, int NQ, bool BIAS>
 __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float* o, float* lse, float* part, float2* part_ml, int splits) {
@@ -1113,14 +1147,20 @@ static int launch_ranges(const Attn& a, const RangeArrays& arrays, int n_arrays,
                            st, a, arrays, n_arrays, runs, out, window);
     });
 }
-// Runs of rows whose largest values are found by workgroups of their own: 256 rows or more, 16 at most.
-static int range_runs(long Tq, long Tk) { return (int)std::max(1L, std::min(cdiv(std::max(Tq, Tk), 256), 16L)); }
+// Runs of rows whose largest values are found by workgroups of their own: 256 rows or more, 64 at most.  (16 at most:
+// 64 queries of 2 heads against 16384 keys 48 us, with 64 37.  Runs of 64 rows: 128 heads of 1024 rows 158 us forward
+// and 539 backward, with 256 154 and 520; 4 heads of 512 21 us, with 256 23.)
+static int range_runs(long Tq, long Tk) { return (int)std::max(1L, std::min(cdiv(std::max(Tq, Tk), 256), 64L)); }
 // Into how many runs the walked axis (`rows` long) is cut, so that `whole` workgroups become enough to fill
 // every CU `resident` times (twice as often where a causal mask makes them uneven); runs of `shortest` rows at least.
+// Up to a quarter of that where the workgroups are fewer than the CUs, until they are as many.  Both sides (64 columns):
+// cut / whole, forward 8 heads of 4096 146 / 187 us, of 1024 35 / 57, 4 heads of 512 22 / 33, 64 heads of 512 stay whole: 39,
+// 45 in three; backward 64 heads of 512 123 / 133, 8 of 4096 479 / 708, 8 of 1024 96 / 203 (causal 96 / 202, and 118 in
+// twice as many), 4 of 512 62 / 123; 16 heads of 2047 under a causal mask, 128 columns, 491 / 720.
 static int axis_splits(long whole, long rows, int resident, int causal, long shortest) {
     if (whole <= 0) return 1;
     const long want = (long)kNumCU * resident * (causal ? 2 : 1);
-    return (int)std::max(1L, std::min({cdiv(want, whole), rows / shortest, 16L}));
+    return (int)std::max({1L, std::min({cdiv(want, whole), rows / shortest, 16L}), std::min({kNumCU / whole, rows / (shortest / 4), 64L})});
 }
 static int padded_dim(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
@@ -1155,7 +1195,7 @@ static int attn_setup(const char* what, Attn* a, long B, long H, long Tq, long T
     CGT_ARG_CHECK(B >= 0 && H >= 0 && Tq >= 0 && Tk >= 0, "%s: negative extent", what);
     CGT_ARG_CHECK(D >= 1 && D <= 128, "%s: heads of %ld columns (1 to 128)", what, D);
     CGT_ARG_CHECK(Tq < (1L << 29) && Tk < (1L << 29) && q_offset > -(1L << 29) && q_offset < (1L << 29), "%s: lengths and offset must be below 2^29", what);
-    CGT_ARG_CHECK(B * H < (1L << 22) && B < (1L << 22) && H < (1L << 22), "%s: too many heads", what);
+    CGT_ARG_CHECK(B < (1L << 22) && H < (1L << 22) && B * H < (1L << 22), "%s: too many heads", what);
     CGT_ARG_CHECK(layout == 0 || layout == 1, "%s: layout %d (0: heads before positions, 1: after them)", what, layout);
     CGT_ARG_CHECK(std::isfinite(scale), "%s: scale must be finite", what);
     if (!dropout_rate(p, what, &a->rate)) return CGT_AMD_ERR_ARG;
@@ -1194,8 +1234,11 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
     CGT_ARG_CHECK(q && o && lse && (Tk == 0 || (k && v)), "attention: null pointer");
     a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths;
     hipStream_t st = as_stream(stream);
-    // Up to four queries read k and v once on the vector units; more rows go through the matrix cores.
-    const bool token = Tq <= 4 && a.rate.threshold == 0;
+    // Up to eight queries read k and v once, on the vector units; more go through the matrix cores, whose
+    // scales take a walk over k and v of their own.  Both sides, vector / matrix: 16 heads of 16 sequences (64 columns)
+    // against 8192 keys, 1 query 188 / 370 us, 4 203 / 372, 8 268 / 373; against 512 keys 20 / 41, 24 / 41, 34 / 41;
+    // 128 columns, 8 queries 483 / 739; one sequence, 8192 keys, 1 query 19 / 48.
+    const bool token = Tq <= 8 && a.rate.threshold == 0;
     const int DP = padded_dim(a.D), tiles = token ? 1 : (int)cdiv(Tq, kAttnCols);
     const long heads = B * H, whole = heads * tiles;
     // Too few workgroups to fill the chip: the keys are cut too.
@@ -1228,7 +1271,9 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
             if (token)
                 return a.Tq == 1 ? attn_launch("attention (one query)", attn_token_kernel<W, 1, bias_>, whole * splits, 1, kAttnThreads, window_bytes, st,
                                                a, o, lse, part, ml, splits)
-                                 : attn_launch("attention (few queries)", attn_token_kernel<W, 4, bias_>, whole * splits, 1, kAttnThreads, window_bytes, st,
+                     : a.Tq <= 4 ? attn_launch("attention (few queries)", attn_token_kernel<W, 4, bias_>, whole * splits, 1, kAttnThreads, window_bytes, st,
+                                               a, o, lse, part, ml, splits)
+                                 : attn_launch("attention (few queries)", attn_token_kernel<W, 8, bias_>, whole * splits, 1, kAttnThreads, window_bytes, st,
                                                a, o, lse, part, ml, splits);
         }
         const size_t lds_bytes = Tile<W>::kRowBytes + Tile<W>::kColBytes + window_bytes;
@@ -1239,7 +1284,9 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
     if (splits > 1) {
         const int rc = attn_width(a, [&](auto width) {
             constexpr int W = decltype(width)::value;
-            return attn_launch("attention join", attn_join_kernel<W>, cdiv(heads * Tq, kAttnThreads / (W / 4)), 1, kAttnThreads, 0, st, a, o, lse, part, ml, splits);
+            constexpr int teams = kAttnThreads / (W / 4);
+            return splits >= kJoinTeams ? attn_launch("attention join", attn_join_kernel<W, teams>, heads * Tq, 1, kAttnThreads, 0, st, a, o, lse, part, ml, splits)
+                                        : attn_launch("attention join", attn_join_kernel<W, 1>, cdiv(heads * Tq, teams), 1, kAttnThreads, 0, st, a, o, lse, part, ml, splits);
         });
         if (rc != CGT_AMD_OK) return rc;
     }

@@ -366,7 +366,9 @@ int cgt_amd_dropout_add_layer_norm_bwd_f32(const float *h, const float *gamma, c
  * q_lengths, k_lengths (int32 [B], NULL: full; clamped to [0, T]) describe a
  * padded batch.  What lies behind them in q, k, v and go is not read; such rows
  * of o, gq, gk, gv are 0.  A query that sees no key (or only scores of -inf)
- * has o = 0 and lse = -inf and contributes to no gradient.
+ * has o = 0 and lse = -inf and contributes to no gradient.  A NaN or an infinity in
+ * a row of q makes NaN of that row's o; one in a key or value within the length
+ * of its head's, those of queries included that the causal rule hides it from.
  *
  * p is the dropout probability of the softmax's values, from the generator
  * described above (rng, channel; rng may be NULL if p rounds to 0): row

@@ -225,6 +225,40 @@ def test_large_scores(K):
     close(lse.get(), att.lse, tol["lse"], "lse")
 
 
+MORE = [
+    case(2, 2, 5, 700, 64, buckets=32, causal=True, q_offset=695, k_lengths=[700, 133]),      # up to eight queries: vector units
+    case(1, 3, 8, 1500, 128, buckets=16, layout="bthd", q_lengths=[6]),
+    case(2, 1, 7, 90, 33, buckets=8, shift=1),
+    case(1, 2, 8, 8, 96, causal=True),
+    case(1, 1, 2, 300, 20, buckets=8),                                                     # two pieces: a team a row
+    case(1, 2, 9, 1700, 64, buckets=32, causal=True, q_offset=1691),                        # nine: matrix cores, many pieces
+    case(1, 1, 200, 1100, 64, buckets=32, k_lengths=[1050]),                               # few workgroups: short runs
+    case(1, 2, 300, 300, 128, buckets=32, causal=True, p=0.2),
+]
+
+
+@pytest.mark.parametrize("c", MORE, ids=["%dx%dx%dx%dx%d-%d" % (c["B"], c["H"], c["Tq"], c["Tk"], c["D"], n) for n, c in enumerate(MORE)])
+def test_attention_with_cut_keys(K, c):
+    test_attention(K, c)
+
+
+@pytest.mark.parametrize("sq,sk,sv,sg", [(1e-15, 1e15, 1, 1), (1e12, 1e-12, 1e-20, 1e15), (1, 1, 1e15, 1e-25), (1, 1, 1, 1e-25), (1, 1, 1e-12, 1e20)])
+@pytest.mark.parametrize("Tq", [3, 70])
+def test_heads_of_any_magnitude(K, Tq, sq, sk, sv, sg):
+    # each array by a factor of its own: a power of two brings every head to the same range; squares leave float's
+    c = case(1, 2, Tq, 130, 64, buckets=32)
+    (q, k, v, table, go), _ = make(c)
+    q, k, v, go = ((a * f).astype(np.float32) for a, f in ((q, sq), (k, sk), (v, sv), (go, sg)))
+    att = T.Attention(q, k, v, table)
+    tol = tolerances(att, go)
+    o, lse = K.rel_attention_fwd(dev(q), dev(k), dev(v), dev(table))
+    close(o.get(), att.o, tol["o"], "o")
+    close(lse.get(), att.lse, tol["lse"], "lse")
+    got = K.rel_attention_bwd(dev(q), dev(k), dev(v), dev(table), o, lse, dev(go))
+    for name, a, want in zip(("gq", "gk", "gv", "gtable"), got, att.pullback(go)):
+        close(a.get(), want, tol[name], name)
+
+
 def test_values_that_are_no_numbers_stay_with_their_row_and_head(K):
     rs = np.random.RandomState(3)
     q, k, v = (rs.randn(2, 2, 50, 32).astype(np.float32) for _ in range(3))
