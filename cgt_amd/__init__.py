@@ -1,5 +1,7 @@
 """cgt_amd: the native CNN hot path of CGT (im2col/col2im, Mul22/BatchedMul22,
-max-pool with argmax, cross-channel LRN) on an MI355X, behind CGT's Op API.
+max-pool with argmax, cross-channel LRN) on an MI355X, behind CGT's Op API, and the
+operators of a transformer layer (layer norm, dropout, attention with a relative
+position bias: nn.layer_norm, nn.dropout, nn.relative_attention).
 
     import cgt_amd as cgt
     from cgt_amd import nn

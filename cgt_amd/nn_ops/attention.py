@@ -95,6 +95,8 @@ class RelativeAttention(core.Op):
         return (s, [s[0], s[3 - t], s[t]])
 
     def pullback(self, inputs, output, gout):
+        if gout[1] is not None or gout[0] is None:
+            raise core.MethodNotDefined("RelativeAttention: gradients go through o only, not through lse")
         o, lse = core.unpack(output)
         g = core.unpack(core.Result(RelativeAttentionBackward(self.info), list(inputs) + [o, lse, gout[0]]))
         return g + [None] * (len(inputs) - len(g))

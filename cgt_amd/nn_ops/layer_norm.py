@@ -52,6 +52,8 @@ class LayerNorm(core.Op):
     def pullback(self, inputs, output, gout):
         x, gamma, _beta = inputs
         _y, mean, rstd = core.unpack(output)
+        if any(g is not None for g in gout[1:]):
+            raise core.MethodNotDefined("LayerNorm: gradients go through y only, not through the statistics")
         return core.unpack(core.Result(LayerNormBackward(), [x, gamma, mean, rstd, gout[0]]))
 
     def get_native_compile_info(self, input_types, devtype):
@@ -133,6 +135,8 @@ class DropoutAddLayerNorm(core.Op):
     def pullback(self, inputs, output, gout):
         from .dropout import Dropout
         _y, h, mean, rstd = core.unpack(output)
+        if any(g is not None for g in gout[2:]):
+            raise core.MethodNotDefined("DropoutAddLayerNorm: gradients go through y and h, not through the statistics")
         gy, gh = gout[:2]
         rng = list(inputs[4:])
         if gy is None:          # only h was used: the residual add and the dropout alone

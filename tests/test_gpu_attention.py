@@ -367,6 +367,54 @@ def test_ops_and_gradients(K):
         nn.relative_attention(q, q, q, k_lengths=[1, 2])
 
 
+def test_no_gradients_through_what_is_kept_for_the_backward_pass(K):
+    from cgt_amd import core
+    from cgt_amd.nn_ops import attention, layer_norm
+    x = core.constant(np.ones((1, 2, 3, 8), np.float32))
+    info = attention.AttentionInfo(0.5, 0, 1, 128, 0, 0.0, 0, 0, 0, 0, 0)
+    _o, lse = core.unpack(core.Result(attention.RelativeAttention(info), [x, x, x]))
+    with pytest.raises(core.MethodNotDefined):
+        core.grad(core.sum(lse), [x])
+    w = core.constant(np.ones(8, np.float32))
+    for op, inputs, n in ((layer_norm.LayerNorm(1e-5), [x, w, w], 1), (layer_norm.DropoutAddLayerNorm(0.0, 1e-5, 0), [x, x, w, w], 2)):
+        with pytest.raises(core.MethodNotDefined):
+            core.grad(core.sum(core.unpack(core.Result(op, inputs))[n]), [x])
+
+
+def test_calls_from_two_threads_on_streams_of_their_own(K):
+    import threading
+    from cgt_amd import capi
+    cases = [case(1, 2, 150, 300, 64, buckets=32, causal=True, q_offset=150), case(2, 3, 4, 2100, 32, buckets=8),
+             case(1, 1, 520, 520, 128, buckets=16, p=0.2), case(3, 2, 30, 30, 40)]
+    data = [([None if a is None else dev(a) for a in make(c)[0]], arguments(c)) for c in cases]
+
+    def run(n, stream):
+        (q, k, v, table, go), more = data[n]
+        o, lse = K.rel_attention_fwd(q, k, v, table, stream=stream, **more)
+        g = K.rel_attention_bwd(q, k, v, table, o, lse, go, stream=stream, **more)
+        return [a for a in (o, lse) + tuple(g) if a is not None]
+    want = [[a.get() for a in run(n, None)] for n in range(len(cases))]
+    got, failed = [[], []], []
+
+    def work(t):
+        try:
+            s = capi.Stream()
+            for n in range(12):       # sizes rise and fall: workspaces grow under the calls in flight
+                got[t].append(((n + t) % 4, run((n + t) % 4, s.handle)))
+            s.synchronize()
+        except Exception as e:      # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for one in got:
+        for n, results in one:
+            assert all(np.array_equal(a.get(), b) for a, b in zip(results, want[n])), n
+
+
 class Block(object):
     """A transformer encoder block as a user writes it: attention and feed-forward sub-layers, each ended by
     dropout + residual + layer norm."""
