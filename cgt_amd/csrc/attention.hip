@@ -293,6 +293,17 @@ struct Column {
     }
 };
 
+// The operands of each step are read from LDS before the matrix instructions of the step in front of it (the backward
+// pass of 16 heads of 2047, 128 columns, one wavefront a SIMD: 661 -> 616 us; at 64 columns and below 1-2 %).
+template <int STEPS>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        if (i + 1 < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
+    }
+}
 // sum_d tile[row][d] * column[d].  A matrix instruction aligns the products it adds and cuts their
 // last bits, always downwards.  That shift is some 1e-8 of the result, nothing in itself, but it has the
 // same sign everywhere, and the gradient of the bias sums millions of nearly cancelling ds: APART
@@ -302,14 +313,21 @@ __device__ __forceinline__ v16f product_rows(const unsigned short* rows, const C
     const int lane = threadIdx.x & 63;
     const unsigned short* at = rows + (lane & 31) * Tile<DP>::kRowPitch + 8 * (lane >> 5);
     v16f sum = {}, odd = {};
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
+    const auto read = [&](int i) {
         Frag f;
 #pragma unroll
         for (int n = 0; n < 2; ++n) f.t[n] = *reinterpret_cast<const v8h*>(at + n * Tile<DP>::kRowPlane + 16 * i);
+        return f;
+    };
+    Frag next = read(0);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+        const Frag f = next;
+        if (i + 1 < DP / 16) next = read(i + 1);
         if (APART && (i & 1)) odd = mul_step(odd, f, col.s[i]);
         else sum = mul_step(sum, f, col.s[i]);
     }
+    reads_ahead<DP / 16>();
     return APART ? sum - odd : sum;
 }
 // acc[d][col] += sum_row tile[row][d] * p[row][col]
@@ -317,18 +335,26 @@ template <int DP>
 __device__ __forceinline__ void product_cols(v16f (&acc)[DP / 32], const unsigned short* cols, const v16f& p) {
     const int lane = threadIdx.x & 63;
     const unsigned short* at = cols + (lane & 31) * Tile<DP>::kColPitch + 8 * (lane >> 5);
+    const auto read = [&](int i, int d) {
+        Frag f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float v[8] = {p[8 * i], p[8 * i + 1], p[8 * i + 2], p[8 * i + 3], p[8 * i + 4], p[8 * i + 5], p[8 * i + 6], p[8 * i + 7]};
-        const Frag b = split8(v);
+        for (int n = 0; n < 2; ++n) f.t[n] = *reinterpret_cast<const v8h*>(at + n * Tile<DP>::kColPlane + 32 * d * Tile<DP>::kColPitch + 16 * i);
+        return f;
+    };
+    constexpr int N = DP / 32;
+    Frag next = read(0, 0), b = {};
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-            Frag f;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) f.t[n] = *reinterpret_cast<const v8h*>(at + n * Tile<DP>::kColPlane + 32 * d * Tile<DP>::kColPitch + 16 * i);
-            acc[d] = mul_step(acc[d], f, b);
+    for (int i = 0; i < 2 * N; ++i) {
+        if (i % N == 0) {
+            const float v[8] = {p[8 * (i / N)], p[8 * (i / N) + 1], p[8 * (i / N) + 2], p[8 * (i / N) + 3],
+                                p[8 * (i / N) + 4], p[8 * (i / N) + 5], p[8 * (i / N) + 6], p[8 * (i / N) + 7]};
+            b = split8(v);
         }
+        const Frag f = next;
+        if (i + 1 < 2 * N) next = read((i + 1) / N, (i + 1) % N);
+        acc[i % N] = mul_step(acc[i % N], f, b);
     }
+    reads_ahead<2 * N>();
 }
 
 __device__ __forceinline__ int tile_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (r & 3); }
@@ -345,9 +371,9 @@ __device__ __forceinline__ float to_log2(float x) { return x < -1e38f && x >= kL
 // log sum exp from the reference of a row's exponentials (in powers of two) and their sum
 __device__ __forceinline__ float log_sum(float ref, float sum) { return ref < -1e38f ? ref : ref * kLn2 + logf(sum); }
 
-// s * unscale + bias for a score tile of origin rel0; sign 1: rows are keys, -1: rows are queries.
+// Forward: s * unscale + bias for a score tile of origin rel0, rows = keys.
 template <bool BIAS>
-__device__ __forceinline__ void scores(v16f& s, float unscale, const BucketRule& rule, const float* win, int rel0, int sign) {
+__device__ __forceinline__ void scores(v16f& s, float unscale, const BucketRule& rule, const float* win, int rel0) {
     if (!BIAS) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] *= unscale;
@@ -356,10 +382,37 @@ __device__ __forceinline__ void scores(v16f& s, float unscale, const BucketRule&
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], unscale, v);
     } else {
-        const float* at = win + bias_reach(rule) + rel0 + sign * (4 * ((threadIdx.x & 63) >> 5) - (int)(threadIdx.x & 31));
+        const float* at = win + bias_reach(rule) + rel0 + 4 * ((threadIdx.x & 63) >> 5) - (int)(threadIdx.x & 31);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], unscale, at[sign * (8 * (r >> 2) + (r & 3))]);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], unscale, at[8 * (r >> 2) + (r & 3)]);
     }
+}
+// Backward: the bias of a score tile of origin rel0 (sign 1: rows are keys, -1: queries), -inf where hide(r) says so if
+// any element may be hidden.  It is read before the tile's products, which leaves no branch between them and what the
+// vector units do with their results, so that both can run at once: 16 heads of 2047, 128 columns 620 -> 544 us, 64 columns
+// 285 -> 266, 32 heads of 1000, 32 columns 128 -> 113.  (The forward pass loses by the registers it takes: 157 -> 159 us.)
+// For the same reason the backward kernels do not skip a wavefront's hidden tiles: at 128 columns the compiler carried the
+// running sums between the two register files around that branch (728 us with it, 667 without).
+// 64 columns with dropout read it after the products: 2 wavefronts a SIMD leave no registers for both the bias and the
+// generator (8 x 8 heads of 512, padded: 127 us before, 118 after).
+constexpr bool shifts_early(int DP, bool DROP) { return !(DROP && DP == 64); }
+template <bool BIAS, class Hide>
+__device__ __forceinline__ v16f shifts(const BucketRule& rule, const float* win, int rel0, int sign, bool edge, Hide hide) {
+    v16f b = {};
+    if (BIAS) {
+        if (far_tile(rule, rel0)) {
+            b = win[rel0 < 0 ? 0 : bias_window(rule) - 1];
+        } else {
+            const float* at = win + bias_reach(rule) + rel0 + sign * (4 * ((threadIdx.x & 63) >> 5) - (int)(threadIdx.x & 31));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) b[r] = at[sign * (8 * (r >> 2) + (r & 3))];
+        }
+    }
+    if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) b[r] = hide(r) ? -INFINITY : b[r];
+    }
+    return b;
 }
 // Between LDS writes and reads of one wavefront, by different lanes.
 __device__ __forceinline__ void wave_lds_fence() {
@@ -558,7 +611,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
         if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;      // nothing here for this wavefront
         const int rel0 = j0 - qw - a.q_offset;
         v16f s = product_rows<DP, false>(kt, qcol);
-        scores<BIAS>(s, unscale, a.rule, win, rel0, 1);
+        scores<BIAS>(s, unscale, a.rule, win, rel0);
         if (j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset)) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -808,7 +861,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
 
 // ---------------------------------------------------------------- backward: queries
 
-// gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.
+// gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.  Bound by the vector
+// instructions beside the matrix cores (10 a matrix instruction, 19 with dropout) and, at 128 columns, by one wavefront a
+// SIMD: its operands q and go (128 registers), gq (64) and the tiles on their way take more than half of the registers.
 template <int DP, bool BIAS, bool DROP>
 __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_kernel(Attn a, Ranges ranges, const float* o, const float* lse, const float* go, float* gq,
     float* part, float* delta, float* part_table, int tiles, int splits) {
@@ -878,12 +933,16 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
             kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
             vr.load(off, vbase, a.k_t, j0 + kAttnRows, last, a.D);
         }
-        if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;
         const int rel0 = j0 - qw - a.q_offset;
+        const bool edge = j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset);
+        const auto tile_shifts = [&] {
+            return shifts<BIAS>(a.rule, win, rel0, 1, edge, [&](int r) { return hidden(a, j0 + tile_row(r), query, k_end); });
+        };
+        v16f shift;
+        if constexpr (shifts_early(DP, DROP)) shift = tile_shifts();
         v16f s = product_rows<DP, false>(kt, qcol);
         v16f dp = product_rows<DP, true>(vt, gcol);
-        scores<BIAS>(s, unscale, a.rule, win, rel0, 1);
-        const bool edge = j0 + kAttnRows > k_end || qw + 32 > q_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset);
+        if constexpr (!shifts_early(DP, DROP)) shift = tile_shifts();
         if (DROP) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -895,8 +954,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float p = pow2(s[r] - row_lse);
-            s[r] = edge && (!valid || hidden(a, j0 + tile_row(r), query, k_end)) ? 0.0f : p * __builtin_fmaf(dp[r], dscale, -dl);
+            const float p = pow2(__builtin_fmaf(s[r], unscale, shift[r]) - row_lse);      // (0 for queries behind the last)
+            s[r] = p * __builtin_fmaf(dp[r], dscale, -dl);
         }
         if (BIAS) {
             if (far_tile(a.rule, rel0)) {      // one bucket has the whole tile
@@ -1044,7 +1103,6 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
             qr.load(off, qbase, a.q_t, i0 + kAttnRows, last, a.D);
             gr.load(off, gbase, a.q_t, i0 + kAttnRows, last, a.D);
         }
-        if (kw >= k_end || (a.causal && kw > i0 + 31 + a.q_offset)) continue;
         const int rel0 = kw - i0 - a.q_offset;
         unsigned word[16];
         if (DROP) {
@@ -1067,15 +1125,19 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
 #pragma unroll
             for (int r = 0; r < 16; ++r) word[r] = mine[32 * (c >> 2 & 1) + tile_row(r)] >> bit & 1u;
         }
+        const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + a.q_offset);
+        const auto tile_shifts = [&] {
+            return shifts<BIAS>(a.rule, win, rel0, -1, edge, [&](int r) { return hidden(a, key, i0 + tile_row(r), k_end); });
+        };
+        v16f shift;
+        if constexpr (shifts_early(DP, DROP)) shift = tile_shifts();
         v16f s = product_rows<DP, false>(qt, kcol);
         v16f dp = product_rows<DP, true>(gt, vcol);
-        scores<BIAS>(s, unscale, a.rule, win, rel0, -1);
-        const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + a.q_offset);
+        if constexpr (!shifts_early(DP, DROP)) shift = tile_shifts();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int row = tile_row(r);
-            float p = pow2(s[r] - stats[row]);
-            if (edge && hidden(a, key, i0 + row, k_end)) p = 0.0f;      // rows beyond the queries: p is 0 by their lse
+            const float p = pow2(__builtin_fmaf(s[r], unscale, shift[r]) - stats[row]);      // rows beyond the queries: 0 by their lse
             const bool keep = !DROP || word[r];
             s[r] = keep ? p : 0.0f;
             dp[r] = p * __builtin_fmaf(keep ? dp[r] : 0.0f, dscale, -stats[kAttnRows + row]);
