@@ -558,6 +558,10 @@ __device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_
 
 // ---------------------------------------------------------------- forward
 
+// o and lse of a block of 128 queries, or of a run of its keys.  Bound by the issue of 9.2 vector instructions (the exponential,
+// the split into two terms, the sum) a matrix instruction: 8x16 heads of 1024, 64 columns, padded: 113 us (and 12 for the
+// ranges), the matrix cores 0.34 busy; 21.7 GFLOP, 180 TFLOP/s of the formulas' products, where fp32 matrix
+// instructions reach 154 at most.
 template <int DP, bool BIAS, bool DROP>
 __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kernel(Attn a, Ranges ranges, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
     extern __shared__ __align__(16) unsigned short lds[];
@@ -862,8 +866,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
 // ---------------------------------------------------------------- backward: queries
 
 // gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.  Bound by the vector
-// instructions beside the matrix cores (10 a matrix instruction, 19 with dropout) and, at 128 columns, by one wavefront a
-// SIMD: its operands q and go (128 registers), gq (64) and the tiles on their way take more than half of the registers.
+// instructions beside the matrix cores (8 a matrix instruction at 128 columns, 18 at 64 with dropout) and, at 128 columns, by one
+// wavefront a SIMD: its operands q and go (128 registers), gq (64) and the tiles on their way take more than half of the registers.
 template <int DP, bool BIAS, bool DROP>
 __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_kernel(Attn a, Ranges ranges, const float* o, const float* lse, const float* go, float* gq,
     float* part, float* delta, float* part_table, int tiles, int splits) {
@@ -1048,6 +1052,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_table_kernel(const float* p
 
 // ---------------------------------------------------------------- backward: keys
 
+// gk and gv of a block of 128 keys.  Both sums stay in registers (128 of them at 128 columns) beside the columns of k and v
+// (another 128), hence one wavefront a SIMD there.  2x8 heads of 2047, 128 columns, causal: 194 us, the matrix cores 0.26 busy,
+// with 6 vector instructions a matrix instruction; 8x8 heads of 512, 64 columns, dropout, padded: 49 us.
 template <int DP, bool BIAS, bool DROP>
 __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, Ranges ranges, const float* lse, const float* delta, const float* go, float* gk,
     float* gv, float* part, int tiles, int splits) {
@@ -1217,8 +1224,8 @@ static int range_runs(long Tq, long Tk) { return (int)std::max(1L, std::min(cdiv
 // every CU `resident` times (twice as often where a causal mask makes them uneven); runs of `shortest` rows at least.
 // Up to a quarter of that where the workgroups are fewer than the CUs, until they are as many.  Both sides (64 columns):
 // cut / whole, forward 8 heads of 4096 146 / 187 us, of 1024 35 / 57, 4 heads of 512 22 / 33, 64 heads of 512 stay whole: 39,
-// 45 in three; backward 64 heads of 512 123 / 133, 8 of 4096 479 / 708, 8 of 1024 96 / 203 (causal 96 / 202, and 118 in
-// twice as many), 4 of 512 62 / 123; 16 heads of 2047 under a causal mask, 128 columns, 491 / 720.
+// 45 in three; backward (before its last step for speed) 64 heads of 512 123 / 133, 8 of 4096 479 / 708, 8 of 1024 96 / 203
+// (causal 96 / 202, and 118 in twice as many), 4 of 512 62 / 123; 16 heads of 2047 under a causal mask, 128 columns, 491 / 720.
 static int axis_splits(long whole, long rows, int resident, int causal, long shortest) {
     if (whole <= 0) return 1;
     const long want = (long)kNumCU * resident * (causal ? 2 : 1);
