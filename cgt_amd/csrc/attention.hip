@@ -886,6 +886,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
     if (BIAS) {
         copy_bias(a, ranges, w.h, win);
         for (int s = threadIdx.x; s < 4 * window; s += kAttnThreads) diag[s] = 0.0f;
+        __syncthreads();      // a workgroup without a key meets no other barrier before its wavefronts add to their sums
     }
     int last = k_end;
     if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
