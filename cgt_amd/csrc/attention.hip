@@ -14,23 +14,27 @@
 // keys gk and gv, so no sum is shared between workgroups and results do not depend on the order
 // they run in.
 //
-// Matrix products run at float32 accuracy on the fp16 matrix cores: an operand, times a power of two
-// that brings the largest of its head's values to [2^14, 2^15), is cut into two fp16 terms, x = h + l (l is the
-// rounded rest: 22 bits and the sign), and the products l h, h l, h h are accumulated in float32.  Three
-// v_mfma_f32_32x32x16_f16 do in 3 x 32 cycles what eight v_mfma_f32_32x32x2_f32 do in 8 x 64, and the
-// vector units work beside them (fp32 matrix instructions keep them busy).  Measured on products of
-// 128 (64) normal values: error 1.1e-7 (1.0e-7) of the results' rms, 2.0e-7 (1.4e-7) with the fp32
-// instructions.  Values keep all 22 bits down to 2^-17 of the largest of their head, and an
-// absolute 2^-39 of it below; the largest values of a head are found by a kernel that runs first.
-// (Heads whose largest value is below 2^-100 lose digits as fp16's subnormals do.)  Nothing is read behind
-// the lengths.  A NaN or infinity in a row of q makes that row NaN, one in a row of k or v that the walk
-// meets all of its head: a key that a causal mask hides has probability 0, and 0 * NaN is NaN.
+// Matrix products run at float32 accuracy on the fp16 matrix cores: an operand, times a power of two, is cut into two
+// fp16 terms, x = h + l (l is the rounded rest: 22 bits and the sign), and the products l h, h l, h h are accumulated in
+// float32.  Three v_mfma_f32_32x32x16_f16 do in 3 x 32 cycles what eight v_mfma_f32_32x32x2_f32 do in 8 x 64, and the vector
+// units work beside them (fp32 matrix instructions keep them busy).  Measured on products of 128 (64) normal values: error
+// 1.1e-7 (1.0e-7) of the results' rms, 2.0e-7 (1.4e-7) with the fp32 instructions.  The powers of two:
+//   a lane's own column has one, that brings its largest value to [2^14, 2^15);
+//   a tile of 32 rows in LDS has one, or one a row where its rows differ by more than 2^8 (attn_scale_kernel).  So a row's
+//     digits do not depend on the rows around it: values keep 22 bits down to 2^-9 of its largest and an absolute 2^-31 of
+//     that below, at least;
+//   what multiplies such a tile in the sums over keys or queries (p v, ds k, p go, ds q) takes over the rows' factors, so that
+//     it is of the size of the terms that are added, and gets the power of two that its largest term needs: of the tile in
+//     the backward pass, of the terms met so far in the forward pass, where the others are cut with an absolute error
+//     of 2^-37 of the largest at most.
+// Nothing is read behind the lengths.  A NaN or infinity in a row of q makes that row NaN, one in a row of k or v that the
+// walk meets all of its head: a key that a causal mask hides has probability 0, and 0 * NaN is NaN.
 //
 // A wavefront owns 32 columns (queries in the forward and the first backward kernel, keys in the
 // second) and forms the *transposed* score tile, rows = the other side: lane l then holds, for
 // column l % 32, rows 8 g + 4 (l / 32) + t in register 4 g + t.  With the k positions of the next
 // product's 16-wide step taken in the order (row 8 b + 4 half + t at position 8 half + 4 b + t)
-// the score tile, cut into its two terms, is that product's B operand as it stands, with no
+// the score tile, cut into its terms, is that product's B operand as it stands, with no
 // exchange between lanes; the other operand is laid out in that order when it is put into LDS.
 #include "random.h"
 #include <algorithm>
@@ -124,21 +128,20 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef unsigned v4u32 __attribute__((ext_vector_type(4)));
 
-// The power of two that brings `top` to [2^14, 2^15), and its reciprocal; 1 for 0.  Capped at 2^100, so that
-// the reciprocal of two together stays a float.
+// The power of two that brings `top` to [2^14, 2^15).  Capped at 2^126: values below 2^-112 lose digits.
 __device__ __forceinline__ float power_scale(float top) {
-    const unsigned e = __float_as_uint(top) >> 23 & 255u, field = min(268u - e, 227u);
-    return top == 0.0f ? 1.0f : __uint_as_float(field << 23);
+    const unsigned e = __float_as_uint(top) >> 23 & 255u;
+    return __uint_as_float(min(268u - e, 253u) << 23);
 }
 __device__ __forceinline__ float reciprocal_power(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// The two fp16 terms of two floats times a power of two, packed (first in the low half).
+// The two fp16 terms of two floats, each times a power of two, packed (first in the low half).
 struct Terms {
     unsigned t[2];
 };
-__device__ __forceinline__ Terms split2(float x, float y, float scale) {
-    const v2h h = {(_Float16)__builtin_fmaf(x, scale, 0.0f), (_Float16)__builtin_fmaf(y, scale, 0.0f)};
-    const v2h l = {(_Float16)__builtin_fmaf(x, scale, -(float)h.x), (_Float16)__builtin_fmaf(y, scale, -(float)h.y)};
+__device__ __forceinline__ Terms split2(float x, float y, float sx, float sy) {
+    const v2h h = {(_Float16)__builtin_fmaf(x, sx, 0.0f), (_Float16)__builtin_fmaf(y, sy, 0.0f)};
+    const v2h l = {(_Float16)__builtin_fmaf(x, sx, -(float)h.x), (_Float16)__builtin_fmaf(y, sy, -(float)h.y)};
     return {{__builtin_bit_cast(unsigned, h), __builtin_bit_cast(unsigned, l)}};
 }
 __device__ __forceinline__ Terms split2(float x, float y) {
@@ -170,6 +173,13 @@ __device__ __forceinline__ v16f mul_step(v16f acc, const Frag& a, const Frag& b)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.t[0], b.t[0], acc, 0, 0, 0);
 }
 
+// What a tile's rows are scaled by: one power of two, or 0 and one for each row where the rows are mixed (rare: see
+// attn_scale_kernel).  Where they are not, a tile costs one load that all lanes share.
+struct ScaleArray {
+    const float *tiles, *rows;      // a head's
+};
+__device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+
 // A tile of 32 rows of DP columns, shared by the workgroup.  A thread loads four neighbouring rows of
 // DP / 32 columns (rows at or beyond `end` are zero and not read), scales them, cuts them into terms and
 // writes them to LDS in one or both of two layouts, two planes (terms) each:
@@ -180,7 +190,7 @@ __device__ __forceinline__ v16f mul_step(v16f acc, const Frag& a, const Frag& b)
 template <int DP>
 struct Tile {
     static constexpr int E = DP / 32, kRowPitch = DP + 8, kColPitch = 40;
-    static constexpr int kRowPlane = kAttnRows * kRowPitch, kColPlane = DP * kColPitch;      // in fp16
+    static constexpr int kRowPlane = kAttnRows * kRowPitch, kColPlane = DP * kColPitch;      // in 16-bit values
     static constexpr int kRowBytes = 2 * kRowPlane * 2, kColBytes = 2 * kColPlane * 2;
     float v[4][E];
 
@@ -224,15 +234,31 @@ struct Tile {
             }
         }
     }
+    // `factors`: where a mixed tile (row0 its first row, `end` as in load) leaves the reciprocals of its rows' scales
     template <bool ROWS, bool COLS>
-    __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols, float scale) const {
+    __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols, float tile_scale, const float* row_scales, float* factors, int row0, int end) const {
+        if (__builtin_expect(tile_scale != 0.0f, 1)) {
+            const float scale[4] = {tile_scale, tile_scale, tile_scale, tile_scale};
+            store<ROWS, COLS>(rows, cols, scale);
+        } else {
+            float scale[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                scale[r] = row_scales[min(row0 + (int)(threadIdx.x >> 5) * 4 + r, end - 1)];
+                if ((threadIdx.x & 31) == 0) factors[(threadIdx.x >> 5) * 4 + r] = reciprocal_power(scale[r]);
+            }
+            store<ROWS, COLS>(rows, cols, scale);
+        }
+    }
+    template <bool ROWS, bool COLS>
+    __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols, const float (&scale)[4]) const {
         const int c = (threadIdx.x & 31) * E, rb = threadIdx.x >> 5;
         const int pos = 16 * (rb >> 2) + 8 * (rb & 1) + 4 * ((rb >> 1) & 1);
         Terms t[E][2];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            t[e][0] = split2(v[0][e], v[1][e], scale);
-            t[e][1] = split2(v[2][e], v[3][e], scale);
+            t[e][0] = split2(v[0][e], v[1][e], scale[0], scale[1]);
+            t[e][1] = split2(v[2][e], v[3][e], scale[2], scale[3]);
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -330,33 +356,6 @@ __device__ __forceinline__ v16f product_rows(const unsigned short* rows, const C
     reads_ahead<DP / 16>();
     return APART ? sum - odd : sum;
 }
-// acc[d][col] += sum_row tile[row][d] * p[row][col]
-template <int DP>
-__device__ __forceinline__ void product_cols(v16f (&acc)[DP / 32], const unsigned short* cols, const v16f& p) {
-    const int lane = threadIdx.x & 63;
-    const unsigned short* at = cols + (lane & 31) * Tile<DP>::kColPitch + 8 * (lane >> 5);
-    const auto read = [&](int i, int d) {
-        Frag f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) f.t[n] = *reinterpret_cast<const v8h*>(at + n * Tile<DP>::kColPlane + 32 * d * Tile<DP>::kColPitch + 16 * i);
-        return f;
-    };
-    constexpr int N = DP / 32;
-    Frag next = read(0, 0), b = {};
-#pragma unroll
-    for (int i = 0; i < 2 * N; ++i) {
-        if (i % N == 0) {
-            const float v[8] = {p[8 * (i / N)], p[8 * (i / N) + 1], p[8 * (i / N) + 2], p[8 * (i / N) + 3],
-                                p[8 * (i / N) + 4], p[8 * (i / N) + 5], p[8 * (i / N) + 6], p[8 * (i / N) + 7]};
-            b = split8(v);
-        }
-        const Frag f = next;
-        if (i + 1 < 2 * N) next = read((i + 1) / N, (i + 1) % N);
-        acc[i % N] = mul_step(acc[i % N], f, b);
-    }
-    reads_ahead<2 * N>();
-}
-
 __device__ __forceinline__ int tile_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (r & 3); }
 // v of lane ^ 32
 __device__ __forceinline__ float other_half(float v) {
@@ -370,6 +369,66 @@ __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x
 __device__ __forceinline__ float to_log2(float x) { return x < -1e38f && x >= kLowest ? fmaxf(x * kLog2e, kLowest) : x * kLog2e; }
 // log sum exp from the reference of a row's exponentials (in powers of two) and their sum
 __device__ __forceinline__ float log_sum(float ref, float sum) { return ref < -1e38f ? ref : ref * kLn2 + logf(sum); }
+
+// What undoes the scales of a tile's rows: one factor, or 32 in LDS where the rows are mixed.  A product of such a tile is
+// multiplied row by row, by a branch around 16 multiplications that the other tiles do without.
+struct TileRows {
+    const float* at;
+    float one;
+    bool mixed;
+    __device__ __forceinline__ TileRows(float tile_scale, const float* factors)
+        : at(factors), one(tile_scale != 0.0f ? reciprocal_power(tile_scale) : 1.0f), mixed(__builtin_expect(tile_scale == 0.0f, 0)) {}
+    // v, but for the factor `one`
+    __device__ __forceinline__ void undo(v16f& v) const {
+        if (__builtin_expect(mixed, 0)) {
+            const float* f = at + 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 x = *reinterpret_cast<const float4*>(f + 8 * g);
+                v[4 * g] *= x.x, v[4 * g + 1] *= x.y, v[4 * g + 2] *= x.z, v[4 * g + 3] *= x.w;
+            }
+        }
+    }
+};
+__device__ __forceinline__ float magnitude(const v16f& v) {
+    float top = fabsf(v[0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(v[r]));
+    return fmaxf(top, other_half(top));
+}
+// An operand of a tile by columns.
+template <int DP>
+__device__ __forceinline__ Frag read_cols(const unsigned short* cols, int block, int step) {
+    const int lane = threadIdx.x & 63;
+    const unsigned short* at = cols + (32 * block + (lane & 31)) * Tile<DP>::kColPitch + 8 * (lane >> 5) + 16 * step;
+    return {{*reinterpret_cast<const v8h*>(at), *reinterpret_cast<const v8h*>(at + Tile<DP>::kColPlane)}};
+}
+// The lane's column of 32 rows as a B operand of two steps.
+__device__ __forceinline__ void split16(Frag (&b)[2], const v16f& w) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float v[8] = {w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3], w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]};
+        b[i] = split8(v);
+    }
+}
+// acc[d][column] += sum over a tile's rows of x[row][d] * w[row][column].  `cols` has x by columns, each row times its
+// scale, `rows` the reciprocals, which go over to w.  A lane brings the largest of its column's terms to [2^14, 2^15)
+// and adds what the tile gives to acc on the vector units, with the power of two undone: tiles do not share a scale,
+// and acc is rounded where a matrix instruction would cut it.
+template <int DP>
+__device__ __forceinline__ void add_tile(v16f (&acc)[DP / 32], const unsigned short* cols, const TileRows& rows, v16f w) {
+    rows.undo(w);
+    const float scale = power_scale(magnitude(w)), back = reciprocal_power(scale) * rows.one;
+    Frag b[2];
+    split16(b, w * scale);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+        const v16f part = mul_step(mul_step(v16f{}, read_cols<DP>(cols, d, 0), b[0]), read_cols<DP>(cols, d, 1), b[1]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = __builtin_fmaf(part[r], back, acc[d][r]);
+        if (d & 1) __builtin_amdgcn_sched_barrier(0);
+    }
+}
 
 // Forward: s * unscale + bias for a score tile of origin rel0, rows = keys.
 template <bool BIAS>
@@ -459,98 +518,93 @@ __device__ __forceinline__ float group_sum(float x) {
     return x;
 }
 
-// ---- the largest values of a head
+// Largest over aligned groups of N lanes (8, 16 or 32) of values that are not negative; every lane gets it.
+template <int N>
+__device__ __forceinline__ float group_max(float x) {
+    auto top = [](float v, auto ctrl) {
+        return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true)));
+    };
+    x = top(x, std::integral_constant<int, 0xB1>());
+    x = top(x, std::integral_constant<int, 0x4E>());
+    x = top(x, std::integral_constant<int, 0x141>());
+    if (N >= 16) x = top(x, std::integral_constant<int, 0x140>());
+    if (N >= 32) x = fmaxf(x, __shfl_xor(x, 16));
+    return x;
+}
 
-// What a head's workgroups have in common, worked out once.  For each of its arrays, what the scales rest on:
-// the largest magnitude of a value and (if asked for) the largest norm of a row, over the rows within the
-// length, values that are no numbers left out, for a run of rows each: [array][head][run].  And the
-// bias by relative position, [head of H][window], in the grid's last row.
-struct RangeArrays {
+// ---- the rows' scales
+
+// What the workgroups of a call have in common, worked out once: the powers of two that the products of the arrays staged
+// through LDS are formed with, for each tile of 32 rows (within the length) and for each row; and the bias by relative
+// position, [head of H][window], in the grid's last row.  A tile's scale brings its largest magnitude (values that are no
+// numbers left out) to [2^14, 2^15), unless a row, not all zeros, is smaller by more than 2^8: there it is 0, and each row's brings
+// its own.  So the 22 bits of a row reach down to 2^-9 of its largest value at least, whatever other rows hold.
+struct ScaledArrays {
     const float* base[4];
     int keys[4];      // 1: laid out and limited as k, 0: as q
-    int norm[4];
+};
+// Where they are: of each array first the tiles', [head][tile], then the rows', [head][row].
+struct Scales {
+    const float *arrays, *window;
+    long start[4];
+    int heads;
+    __device__ __forceinline__ ScaleArray of(int array, int head, int T) const {
+        const int tiles = (T + kAttnRows - 1) / kAttnRows;
+        const float* at = arrays + start[array];
+        return {at + (long)head * tiles, at + (long)heads * tiles + (long)head * T};
+    }
 };
 template <int DP>
-__global__ __launch_bounds__(kAttnThreads) void attn_range_kernel(Attn a, RangeArrays arrays, int n_arrays, int runs, float2* out, float* window) {
+__global__ __launch_bounds__(kAttnThreads) void attn_scale_kernel(Attn a, ScaledArrays arrays, Scales scales, int n_arrays, int runs) {
     constexpr int LANES = DP / 4, STEP = kAttnThreads / LANES, DEEP = 8;
-    __shared__ float2 join[4];
+    __shared__ float tops[kAttnThreads];
     const int n = blockIdx.y;
     if (n == n_arrays) {
         const int size = bias_window(a.rule);
         const long total = (long)size * a.H;
         for (long i = (long)blockIdx.x * kAttnThreads + threadIdx.x; i < total; i += (long)gridDim.x * kAttnThreads)
-            window[i] = to_log2(a.table[(long)bucket_of(a.rule, (int)(i % size) - bias_reach(a.rule)) * a.H + i / size]);
+            const_cast<float*>(scales.window)[i] = to_log2(a.table[(long)bucket_of(a.rule, (int)(i % size) - bias_reach(a.rule)) * a.H + i / size]);
         return;
     }
-    const int head = blockIdx.x / runs, at = blockIdx.x % runs, b = head / a.H, h = head % a.H, keys = arrays.keys[n], with_norm = arrays.norm[n];
+    const int head = blockIdx.x / runs, at = blockIdx.x % runs, b = head / a.H, h = head % a.H, keys = arrays.keys[n];
     const int T = keys ? a.Tk : a.Tq, end = length_of(keys ? a.k_lengths : a.q_lengths, b, T);
-    const int run = (T + runs - 1) / runs, first = at * run, last = min(end, first + run), c = threadIdx.x % LANES * 4;
+    // a run is a multiple of the 256 rows that the workgroup has in hand at a time
+    const long run = ((long)T + runs * kAttnThreads - 1) / (runs * kAttnThreads) * kAttnThreads;
+    const int first = (int)min((long)end, at * run), last = (int)min((long)end, first + run), lane = threadIdx.x % LANES;
     const long stride = keys ? a.k_t : a.q_t;
     const float* base = arrays.base[n] + (keys ? b * a.k_b + h * a.k_h : b * a.q_b + h * a.q_h);
-    float top = 0.0f, norm = 0.0f;
-    for (int r0 = first + threadIdx.x / LANES; r0 < last; r0 += DEEP * STEP) {
-        float4 v[DEEP];
+    const ScaleArray to = scales.of(n, head, T);
+    for (int c0 = first; c0 < last; c0 += kAttnThreads) {
 #pragma unroll
-        for (int u = 0; u < DEEP; ++u) v[u] = load4(base + min(r0 + u * STEP, last - 1) * stride, c, a.D);
+        for (int u0 = 0; u0 < kAttnThreads / STEP; u0 += DEEP) {
+            const int r0 = c0 + u0 * STEP + threadIdx.x / LANES;
+            float4 v[DEEP];
 #pragma unroll
-        for (int u = 0; u < DEEP; ++u) {
-            float x[4] = {fabsf(v[u].x), fabsf(v[u].y), fabsf(v[u].z), fabsf(v[u].w)};
+            for (int u = 0; u < DEEP; ++u) v[u] = load4(base + min(r0 + u * STEP, last - 1) * stride, 4 * lane, a.D);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = x[e] <= -kLowest ? x[e] : 0.0f;
-                top = fmaxf(top, x[e]);
+            for (int u = 0; u < DEEP; ++u) {
+                const float x[4] = {fabsf(v[u].x), fabsf(v[u].y), fabsf(v[u].z), fabsf(v[u].w)};
+                float top = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, x[e] <= -kLowest ? x[e] : 0.0f);
+                top = group_max<LANES>(top);
+                if (lane == 0) tops[r0 + u * STEP - c0] = r0 + u * STEP < last ? top : 0.0f;
             }
-            if (with_norm) norm = fmaxf(norm, group_sum<LANES>((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])));
         }
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        top = fmaxf(top, __shfl_xor(top, d));
-        norm = fmaxf(norm, __shfl_xor(norm, d));
-    }
-    if ((threadIdx.x & 63) == 0) join[threadIdx.x >> 6] = make_float2(top, norm);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 4; ++i) {
-            top = fmaxf(top, join[i].x);
-            norm = fmaxf(norm, join[i].y);
+        __syncthreads();
+        const float top = tops[threadIdx.x], tile = group_max<kAttnRows>(top);
+        const bool mixed = group_max<kAttnRows>(top > 0.0f && top < 0x1p-8f * tile ? 1.0f : 0.0f) > 0.0f;
+        if (c0 + (int)threadIdx.x < last) {
+            const_cast<float*>(to.rows)[c0 + threadIdx.x] = power_scale(top);
+            if (threadIdx.x % kAttnRows == 0) const_cast<float*>(to.tiles)[(c0 + threadIdx.x) / kAttnRows] = mixed ? 0.0f : power_scale(tile);
         }
-        // squares that left the range of floats: the norm is at most sqrt(D) times the largest value
-        out[(long)n * gridDim.x + blockIdx.x] = make_float2(top, norm > 1e-30f && norm < 1e37f ? sqrtf(norm) : top * sqrtf((float)a.D));
+        __syncthreads();
     }
 }
-struct Ranges {
-    const float2* at;
-    int runs;
-    const float* window;
-};
-__device__ __forceinline__ void copy_bias(const Attn& a, const Ranges& r, int head, float* win) {
+__device__ __forceinline__ void copy_bias(const Attn& a, const float* window, int head, float* win) {
     const int n = bias_window(a.rule);
-    for (int s = threadIdx.x; s < n; s += kAttnThreads) win[s] = r.window[(long)head * n + s];
+    for (int s = threadIdx.x; s < n; s += kAttnThreads) win[s] = window[(long)head * n + s];
 }
-__device__ __forceinline__ float2 head_range(const Attn& a, const Ranges& r, int array, const Where& w) {
-    const float2* p = r.at + ((long)array * a.B * a.H + w.b * a.H + w.h) * r.runs;
-    float2 m = p[0];
-    for (int i = 1; i < r.runs; ++i) m = make_float2(fmaxf(m.x, p[i].x), fmaxf(m.y, p[i].y));
-    return m;
-}
-
-// The scales of the backward pass, from the ranges of k, v, q and go (in that order).  ds = p (dp - go . o) is at
-// most twice the largest |go| |v| (o is a mean of the v; dropout's factor counts for both): its scale
-// brings that bound below 2^15.
-struct HeadScales {
-    float k, v, q, g, ds;
-    __device__ __forceinline__ float score(const Attn& a) const { return a.scale * kLog2e * reciprocal_power(k) * reciprocal_power(q); }
-    __device__ __forceinline__ float dp(const Attn& a) const {
-        return reciprocal_power(v) * reciprocal_power(g) * (a.rate.threshold ? a.rate.scale : 1.0f);
-    }
-};
-__device__ __forceinline__ HeadScales head_scales(const Attn& a, const Ranges& ranges, const Where& w) {
-    const float2 k = head_range(a, ranges, 0, w), v = head_range(a, ranges, 1, w), q = head_range(a, ranges, 2, w), g = head_range(a, ranges, 3, w);
-    const float bound = 2.0f * v.y * g.y * (a.rate.threshold ? a.rate.scale : 1.0f);
-    return {power_scale(k.x), power_scale(v.x), power_scale(q.x), power_scale(g.x), power_scale(bound)};
-}
-
 // Which of a tile's 16 elements of a lane are hidden; rows are keys, the column is a query.
 __device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_end) {
     return key >= k_end || (a.causal && key > query + a.q_offset);
@@ -558,15 +612,15 @@ __device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_
 
 // ---------------------------------------------------------------- forward
 
-// o and lse of a block of 128 queries, or of a run of its keys.  Bound by the issue of 9.2 vector instructions (the exponential,
-// the split into two terms, the sum) a matrix instruction: 8x16 heads of 1024, 64 columns, padded: 113 us (and 12 for the
-// ranges), the matrix cores 0.34 busy; 21.7 GFLOP, 180 TFLOP/s of the formulas' products, where fp32 matrix
-// instructions reach 154 at most.
+// o and lse of a block of 128 queries, or of a run of its keys.  8x16 heads of 1024, 64 columns, padded, 21.7 GFLOP of the
+// formulas' products: 134 us (and 13 for the scales), where one power of two a head, without regard to what its rows hold,
+// took 117.
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kernel(Attn a, Ranges ranges, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kernel(Attn a, Scales scales, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *kt = lds, *vt = kt + Tile<DP>::kRowBytes / 2;
-    float* win = reinterpret_cast<float*>(vt + Tile<DP>::kColBytes / 2);
+    float* krows = reinterpret_cast<float*>(vt + Tile<DP>::kColBytes / 2);      // reciprocal scales of the tile's rows of k, of v
+    float *vrows = krows + kAttnRows, *win = vrows + kAttnRows;
     const Where w = where(a, tiles * splits, kHeavyLast);
     const int split = w.tile % splits, q0 = w.tile / splits * kAttnCols;
     const int lane = threadIdx.x & 63, qw = q0 + (threadIdx.x >> 6) * 32, query = qw + (lane & 31);
@@ -574,7 +628,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
     const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
     const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
-    if (BIAS) copy_bias(a, ranges, w.h, win);
+    if (BIAS) copy_bias(a, scales.window, w.h, win);
     // keys this workgroup walks: to the last one its last query sees, cut into `splits` runs of whole tiles
     int last = k_end;
     if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
@@ -583,12 +637,12 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     const int first = split * run;
     last = min(last, first + run);
 
-    const float kscale = power_scale(head_range(a, ranges, 0, w).x), vscale = power_scale(head_range(a, ranges, 1, w).x);
+    const ScaleArray kscales = scales.of(0, w.b * a.H + w.h, a.Tk), vscales = scales.of(1, w.b * a.H + w.h, a.Tk);
     Column<DP> qcol;
     qcol.load(a.q + qrow, query < q_end, a.D);
     const float qscale = power_scale(qcol.top());
     qcol.split(qscale, 1.0f);
-    const float unscale = a.scale * kLog2e * reciprocal_power(kscale) * reciprocal_power(qscale);      // of a score
+    const float unscale = a.scale * kLog2e * reciprocal_power(qscale);      // of a score, beside its key's
     RngState rng = {};
     unsigned long long group0 = 0;
     if (DROP) {
@@ -596,26 +650,48 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
         group0 = ((unsigned long long)(w.b * a.H + w.h) * a.Tq + query) * ((a.Tk + 15) / 16) * 2 + (lane >> 5);
     }
     v16f acc[DP / 32] = {};
-    float ref = -INFINITY, l = 0.0f;      // the exponentials are 2^(s - ref + 7)
+    float ref = -INFINITY, l = 0.0f;      // the exponentials are 2^(s - ref)
+    float e = 0.0f;                       // acc is the sum of p v times e; 0 while there was nothing to add
+    const auto rescale = [&](float f) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+    };
+    // e for terms p v of this size: the first to [2^12, 2^13), lowered where one outgrows that (as seldom)
+    const auto outgrows = [&](float largest) { return largest * e > 0x1p15f || (e == 0.0f && largest > 0.0f); };
+    const auto settle = [&](float largest) {
+        const float to = outgrows(largest) ? 0.25f * power_scale(largest) : e;
+        rescale(e == 0.0f ? 0.0f : to * reciprocal_power(e));
+        e = to;
+    };
     const typename Tile<DP>::Offsets off(a.k_t, a.D);
     Tile<DP> kr, vr;
+    float knext = 1.0f, vnext = 1.0f;      // the scales of the tiles on their way
     if (first < last) {
         kr.load(off, kbase, a.k_t, first, last, a.D);
         vr.load(off, vbase, a.k_t, first, last, a.D);
+        knext = kscales.tiles[first / kAttnRows];
+        vnext = vscales.tiles[first / kAttnRows];
     }
     for (int j0 = first; j0 < last; j0 += kAttnRows) {
+        const float kscale = uniform(knext), vscale = uniform(vnext);
         __syncthreads();
-        kr.template store<true, false>(kt, nullptr, kscale);
-        vr.template store<false, true>(nullptr, vt, vscale);
+        kr.template store<true, false>(kt, nullptr, kscale, kscales.rows, krows, j0, last);
+        vr.template store<false, true>(nullptr, vt, vscale, vscales.rows, vrows, j0, last);
         __syncthreads();
         if (j0 + kAttnRows < last) {
             kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
             vr.load(off, vbase, a.k_t, j0 + kAttnRows, last, a.D);
+            knext = kscales.tiles[j0 / kAttnRows + 1];
+            vnext = vscales.tiles[j0 / kAttnRows + 1];
         }
         if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;      // nothing here for this wavefront
         const int rel0 = j0 - qw - a.q_offset;
         v16f s = product_rows<DP, false>(kt, qcol);
-        scores<BIAS>(s, unscale, a.rule, win, rel0);
+        const TileRows key_rows(kscale, krows), value_rows(vscale, vrows);
+        key_rows.undo(s);
+        scores<BIAS>(s, unscale * key_rows.one, a.rule, win, rel0);
         if (j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset)) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -625,26 +701,32 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
         top = fmaxf(top, other_half(top));
-        // The reference follows the running maximum only where that is 2^7 above it: the exponentials stay below 2^14,
-        // and the results so far are seldom rescaled.
+        // The reference, a whole number, follows the running maximum only where that is 2^7 above it: the exponentials stay
+        // below 2^7, and the results so far are seldom rescaled.  The same for the scale of the terms p v, known from the
+        // maximum where the tile has one factor.
         const bool rise = top > ref + 7.0f;
-        if (__any(rise)) {
-            const float to = rise ? top : ref, f = to == -INFINITY ? 0.0f : pow2(ref - to);
+        const float to = rise ? ceilf(top) : ref, from = to == -INFINITY ? 0.0f : to;      // (0: a row that has seen nothing yet)
+        const float largest = value_rows.mixed ? 0.0f : pow2(top - from) * value_rows.one;
+        if (__any(rise || outgrows(largest))) {
+            const float f = to == -INFINITY ? 0.0f : pow2(ref - to);
             ref = to;
             l *= f;
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+            rescale(f);
+            settle(largest);
         }
-        const float from = ref == -INFINITY ? 0.0f : ref - 7.0f;      // (a row that has seen nothing yet)
+        // A tile with one factor: the terms' scale goes into the exponent, and comes out of the sum.  (Not where the sum would
+        // lose by it, nor where the difference of the two is no longer exact.)
+        float lift = value_rows.mixed || e == 0.0f ? 0.0f : (float)(__builtin_amdgcn_frexp_expf(e) + __builtin_amdgcn_frexp_expf(value_rows.one) - 2);
+        const bool apart = value_rows.mixed || __any(!(fabsf(lift) <= 40.0f && fabsf(from) < 0x1p22f));
+        if (__builtin_expect(apart, 0)) lift = 0.0f;
+        const float lifted = from - lift;
         float part_l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = pow2(s[r] - from);
+            s[r] = pow2(s[r] - lifted);
             part_l[r & 3] += s[r];
         }
-        l += (part_l[0] + part_l[1]) + (part_l[2] + part_l[3]);
+        l = __builtin_fmaf((part_l[0] + part_l[1]) + (part_l[2] + part_l[3]), pow2(-lift), l);
         if (DROP) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -654,15 +736,31 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
                 for (int e = 0; e < 8; ++e) s[8 * b + e] = random16(u, e) >= a.rate.threshold ? s[8 * b + e] : 0.0f;      // scaled at the end
             }
         }
-        product_cols<DP>(acc, vt, s);
+        if (__builtin_expect(apart, 0)) {
+            value_rows.undo(s);
+            const float found = magnitude(s) * value_rows.one;
+            if (__any(outgrows(found))) settle(found);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = s[r] * value_rows.one * e;
+        }
+        Frag b[2];
+        split16(b, s);
+        Frag next = read_cols<DP>(vt, 0, 0);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const Frag x = next;
+            if (i + 1 < DP / 16) next = read_cols<DP>(vt, (i + 1) % (DP / 32), (i + 1) / (DP / 32));
+            acc[i % (DP / 32)] = mul_step(acc[i % (DP / 32)], x, b[i / (DP / 32)]);
+        }
+        reads_ahead<DP / 16>();
     }
     if (query >= a.Tq) return;
-    l = (l + other_half(l)) * 0x1p-7f;
-    const float back = 0x1p-7f * reciprocal_power(vscale) * (DROP ? a.rate.scale : 1.0f);
+    l += other_half(l);
+    const float back = reciprocal_power(e);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[d][r] *= back;
+        for (int r = 0; r < 16; ++r) acc[d][r] = acc[d][r] * back * (DROP ? a.rate.scale : 1.0f);
     const int half4 = 4 * (lane >> 5);
     const long stat = ((long)w.b * a.H + w.h) * a.Tq + query;
     if (splits > 1) {
@@ -869,11 +967,12 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
 // instructions beside the matrix cores (8 a matrix instruction at 128 columns, 18 at 64 with dropout) and, at 128 columns, by one
 // wavefront a SIMD: its operands q and go (128 registers), gq (64) and the tiles on their way take more than half of the registers.
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_kernel(Attn a, Ranges ranges, const float* o, const float* lse, const float* go, float* gq,
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_kernel(Attn a, Scales scales, const float* o, const float* lse, const float* go, float* gq,
     float* part, float* delta, float* part_table, int tiles, int splits) {
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *kt = lds, *kc = kt + Tile<DP>::kRowBytes / 2, *vt = kc + Tile<DP>::kColBytes / 2;
-    float* square = reinterpret_cast<float*>(vt + Tile<DP>::kRowBytes / 2);      // [wavefront][32][32]
+    float* krows = reinterpret_cast<float*>(vt + Tile<DP>::kRowBytes / 2);      // reciprocal scales of the tile's rows of k, of v
+    float *vrows = krows + kAttnRows, *square = vrows + kAttnRows;              // square: [wavefront][32][32]
     float* win = square + (BIAS ? 4 * kSquare : 0);
     const int window = BIAS ? bias_window(a.rule) : 0;
     float* diag = win + window;      // [wavefront][window]: sums of ds by relative position
@@ -884,7 +983,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
     const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
     const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
     if (BIAS) {
-        copy_bias(a, ranges, w.h, win);
+        copy_bias(a, scales.window, w.h, win);
         for (int s = threadIdx.x; s < 4 * window; s += kAttnThreads) diag[s] = 0.0f;
         __syncthreads();      // a workgroup without a key meets no other barrier before its wavefronts add to their sums
     }
@@ -904,15 +1003,16 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         }
     }
     dl += other_half(dl);
-    const HeadScales sc = head_scales(a, ranges, w);
+    const ScaleArray kscales = scales.of(0, w.b * a.H + w.h, a.Tk), vscales = scales.of(1, w.b * a.H + w.h, a.Tk);
     Column<DP> qcol, gcol;
     qcol.load(a.q + qrow, valid, a.D);
-    qcol.split(sc.q, 1.0f);
+    const float qscale = power_scale(qcol.top());
+    qcol.split(qscale, 1.0f);
     gcol.load(go + qrow, valid, a.D);
-    gcol.split(sc.g, -1.0f);
-    const float unscale = sc.score(a), dscale = sc.dp(a) * sc.ds;      // ds is formed times sc.ds
+    const float gscale = power_scale(gcol.top());
+    gcol.split(gscale, -1.0f);
+    const float unscale = a.scale * kLog2e * reciprocal_power(qscale), dscale = reciprocal_power(gscale) * (DROP ? a.rate.scale : 1.0f);
     if (query < a.Tq && lane < 32 && split == 0) delta[stat] = dl;
-    dl *= sc.ds;
     float row_lse = valid ? to_log2(lse[stat]) : INFINITY;
     if (row_lse == -INFINITY) row_lse = INFINITY;      // a row that saw nothing: every probability is 0
     RngState rng = {};
@@ -925,18 +1025,24 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
     v16f acc[DP / 32] = {};
     const typename Tile<DP>::Offsets off(a.k_t, a.D);
     Tile<DP> kr, vr;
+    float knext = 1.0f, vnext = 1.0f;      // the scales of the tiles on their way
     if (first < last) {
         kr.load(off, kbase, a.k_t, first, last, a.D);
         vr.load(off, vbase, a.k_t, first, last, a.D);
+        knext = kscales.tiles[first / kAttnRows];
+        vnext = vscales.tiles[first / kAttnRows];
     }
     for (int j0 = first; j0 < last; j0 += kAttnRows) {
+        const float kscale = uniform(knext), vscale = uniform(vnext);
         __syncthreads();
-        kr.template store<true, true>(kt, kc, sc.k);
-        vr.template store<true, false>(vt, nullptr, sc.v);
+        kr.template store<true, true>(kt, kc, kscale, kscales.rows, krows, j0, last);
+        vr.template store<true, false>(vt, nullptr, vscale, vscales.rows, vrows, j0, last);
         __syncthreads();
         if (j0 + kAttnRows < last) {
             kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
             vr.load(off, vbase, a.k_t, j0 + kAttnRows, last, a.D);
+            knext = kscales.tiles[j0 / kAttnRows + 1];
+            vnext = vscales.tiles[j0 / kAttnRows + 1];
         }
         const int rel0 = j0 - qw - a.q_offset;
         const bool edge = j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset);
@@ -947,6 +1053,10 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         if constexpr (shifts_early(DP, DROP)) shift = tile_shifts();
         v16f s = product_rows<DP, false>(kt, qcol);
         v16f dp = product_rows<DP, true>(vt, gcol);
+        const TileRows key_rows(kscale, krows), value_rows(vscale, vrows);
+        key_rows.undo(s);
+        value_rows.undo(dp);
+        const float score_scale = unscale * key_rows.one, dp_scale = dscale * value_rows.one;
         if constexpr (!shifts_early(DP, DROP)) shift = tile_shifts();
         if (DROP) {
 #pragma unroll
@@ -959,8 +1069,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float p = pow2(__builtin_fmaf(s[r], unscale, shift[r]) - row_lse);      // (0 for queries behind the last)
-            s[r] = p * __builtin_fmaf(dp[r], dscale, -dl);
+            const float p = pow2(__builtin_fmaf(s[r], score_scale, shift[r]) - row_lse);      // (0 for queries behind the last)
+            s[r] = p * __builtin_fmaf(dp[r], dp_scale, -dl);
         }
         if (BIAS) {
             if (far_tile(a.rule, rel0)) {      // one bucket has the whole tile
@@ -996,7 +1106,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
                 if (lane != 32) *mine += lane < 32 ? same : less;      // (there is no diagonal -32)
             }
         }
-        product_cols<DP>(acc, kc, s);
+        add_tile<DP>(acc, kc, key_rows, s);
     }
     if (query < a.Tq) {
         float* out = splits > 1 ? part + ((long)split * a.B * a.H * a.Tq + stat) * a.D : gq + qrow;
@@ -1004,7 +1114,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                store_scaled(out, 32 * d + 8 * g + 4 * (lane >> 5), a.D, acc[d], g, valid, a.scale * reciprocal_power(sc.k) * reciprocal_power(sc.ds));
+                store_scaled(out, 32 * d + 8 * g + 4 * (lane >> 5), a.D, acc[d], g, valid, a.scale);
     }
     if (BIAS) {
         // by bucket: the window's sums of the four wavefronts and the far tiles' in the window's ends
@@ -1031,7 +1141,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
             for (int s = threadIdx.x & 7; s < window; s += 8) sum += bucket[s] == c ? win[s] : 0.0f;
             sum = group_sum<8>(sum);
             if ((threadIdx.x & 7) == 0)
-                part_table[(((long)w.b * tiles * splits + w.tile) * a.H + w.h) * a.rule.buckets + c] = sum * reciprocal_power(sc.ds);
+                part_table[(((long)w.b * tiles * splits + w.tile) * a.H + w.h) * a.rule.buckets + c] = sum;
         }
     }
 }
@@ -1057,20 +1167,21 @@ __global__ __launch_bounds__(kAttnThreads) void attn_table_kernel(const float* p
 // (another 128), hence one wavefront a SIMD there.  2x8 heads of 2047, 128 columns, causal: 194 us, the matrix cores 0.26 busy,
 // with 6 vector instructions a matrix instruction; 8x8 heads of 512, 64 columns, dropout, padded: 49 us.
 template <int DP, bool BIAS, bool DROP>
-__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, Ranges ranges, const float* lse, const float* delta, const float* go, float* gk,
+__global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, Scales scales, const float* lse, const float* delta, const float* go, float* gk,
     float* gv, float* part, int tiles, int splits) {
     extern __shared__ __align__(16) unsigned short lds[];
     unsigned short *qt = lds, *gt = qt + Tile<DP>::kRowBytes / 2, *qc = gt + Tile<DP>::kRowBytes / 2, *gc = qc + Tile<DP>::kColBytes / 2;
     float* stats = reinterpret_cast<float*>(gc + Tile<DP>::kColBytes / 2);
-    unsigned* bits = reinterpret_cast<unsigned*>(stats + 2 * kAttnRows);      // [wavefront][half][query]: 16 keep bits each
-    float* win = stats + 2 * kAttnRows + (DROP ? kAttnThreads : 0);
+    float *qrows = stats + 2 * kAttnRows, *grows = qrows + kAttnRows;         // reciprocal scales of the tile's rows of q, of go
+    unsigned* bits = reinterpret_cast<unsigned*>(grows + kAttnRows);          // [wavefront][half][query]: 16 keep bits each
+    float* win = grows + kAttnRows + (DROP ? kAttnThreads : 0);
     const Where w = where(a, tiles * splits, kHeavyFirst);
     const int split = w.tile % splits, k0 = w.tile / splits * kAttnCols, lane = threadIdx.x & 63, kw = k0 + (threadIdx.x >> 6) * 32, key = kw + (lane & 31);
     const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
     const float* qbase = a.q + w.b * a.q_b + w.h * a.q_h;
     const float* gbase = go + w.b * a.q_b + w.h * a.q_h;
     const long krow = w.b * a.k_b + w.h * a.k_h + key * a.k_t;
-    if (BIAS) copy_bias(a, ranges, w.h, win);
+    if (BIAS) copy_bias(a, scales.window, w.h, win);
     // queries this workgroup walks: from the first that sees its first key
     int first = 0, last = q_end;
     if (a.causal) first = max(0, k0 - a.q_offset) / kAttnRows * kAttnRows;
@@ -1079,40 +1190,49 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
     first += split * run;
     last = min(last, first + run);
     const bool valid = key < k_end;
-    const HeadScales sc = head_scales(a, ranges, w);
-    const float unscale = sc.score(a), dscale = sc.dp(a) * sc.ds * 0x1p-14f, lscale = sc.ds * 0x1p-14f;
     Column<DP> kcol, vcol;
     kcol.load(a.k + krow, valid, a.D);
-    kcol.split(sc.k, 1.0f);
+    const float kscale = power_scale(kcol.top());
+    kcol.split(kscale, 1.0f);
     vcol.load(a.v + krow, valid, a.D);
-    vcol.split(sc.v, -1.0f);
+    const float vscale = power_scale(vcol.top());
+    vcol.split(vscale, -1.0f);
+    const float unscale = a.scale * kLog2e * reciprocal_power(kscale), dscale = reciprocal_power(vscale) * (DROP ? a.rate.scale : 1.0f);
     const long stat0 = ((long)w.b * a.H + w.h) * a.Tq;
     RngState rng = {};
     if (DROP) rng = load_rng(a.rng, a.channel);
+    const int bit = 8 * ((lane & 31) >> 4) + 4 * ((lane & 31) >> 3 & 1) + (lane & 3);      // of the lane's key in `kept`, by query
+    const unsigned* kept = bits + (threadIdx.x >> 6) * kWave + 32 * (lane >> 2 & 1);
     v16f acck[DP / 32] = {}, accv[DP / 32] = {};
     const typename Tile<DP>::Offsets off(a.q_t, a.D);
+    const ScaleArray qscales = scales.of(2, w.b * a.H + w.h, a.Tq), gscales = scales.of(3, w.b * a.H + w.h, a.Tq);
     Tile<DP> qr, gr;
+    float qnext = 1.0f, gnext = 1.0f;
     if (first < last) {
         qr.load(off, qbase, a.q_t, first, last, a.D);
         gr.load(off, gbase, a.q_t, first, last, a.D);
+        qnext = qscales.tiles[first / kAttnRows];
+        gnext = gscales.tiles[first / kAttnRows];
     }
     for (int i0 = first; i0 < last; i0 += kAttnRows) {
+        const float qscale = uniform(qnext), gscale = uniform(gnext);
         __syncthreads();
-        qr.template store<true, true>(qt, qc, sc.q);
-        gr.template store<true, true>(gt, gc, sc.g);
+        qr.template store<true, true>(qt, qc, qscale, qscales.rows, qrows, i0, last);
+        gr.template store<true, true>(gt, gc, gscale, gscales.rows, grows, i0, last);
         if (threadIdx.x < kAttnRows) {
             const int i = i0 + threadIdx.x;
             const float v = i < last ? lse[stat0 + i] : INFINITY;
-            stats[threadIdx.x] = v == -INFINITY ? INFINITY : to_log2(v) - 14.0f;      // p carries 2^14
-            stats[kAttnRows + threadIdx.x] = i < last ? delta[stat0 + i] * lscale : 0.0f;
+            stats[threadIdx.x] = v == -INFINITY ? INFINITY : to_log2(v);
+            stats[kAttnRows + threadIdx.x] = i < last ? delta[stat0 + i] : 0.0f;
         }
         __syncthreads();
         if (i0 + kAttnRows < last) {
             qr.load(off, qbase, a.q_t, i0 + kAttnRows, last, a.D);
             gr.load(off, gbase, a.q_t, i0 + kAttnRows, last, a.D);
+            qnext = qscales.tiles[i0 / kAttnRows + 1];
+            gnext = gscales.tiles[i0 / kAttnRows + 1];
         }
         const int rel0 = kw - i0 - a.q_offset;
-        unsigned word[16];
         if (DROP) {
             // The generator's groups run along the keys of a query.  Lane l forms the numbers of query l % 32 and
             // its half's 16 keys of this tile, bit 8 b + e for number e of 16-key block b, and leaves the bits in LDS,
@@ -1129,9 +1249,6 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
             wave_lds_fence();
             mine[lane] = mask;
             wave_lds_fence();
-            const int c = lane & 31, bit = 8 * (c >> 4) + 4 * (c >> 3 & 1) + (c & 3);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) word[r] = mine[32 * (c >> 2 & 1) + tile_row(r)] >> bit & 1u;
         }
         const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + a.q_offset);
         const auto tile_shifts = [&] {
@@ -1141,17 +1258,21 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
         if constexpr (shifts_early(DP, DROP)) shift = tile_shifts();
         v16f s = product_rows<DP, false>(qt, kcol);
         v16f dp = product_rows<DP, true>(gt, vcol);
+        const TileRows query_rows(qscale, qrows), go_rows(gscale, grows);
+        query_rows.undo(s);
+        go_rows.undo(dp);
+        const float score_scale = unscale * query_rows.one, dp_scale = dscale * go_rows.one;
         if constexpr (!shifts_early(DP, DROP)) shift = tile_shifts();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int row = tile_row(r);
-            const float p = pow2(__builtin_fmaf(s[r], unscale, shift[r]) - stats[row]);      // rows beyond the queries: 0 by their lse
-            const bool keep = !DROP || word[r];
+            const float p = pow2(__builtin_fmaf(s[r], score_scale, shift[r]) - stats[row]);      // rows beyond the queries: 0 by their lse
+            const bool keep = !DROP || (kept[row] >> bit & 1u);
             s[r] = keep ? p : 0.0f;
-            dp[r] = p * __builtin_fmaf(keep ? dp[r] : 0.0f, dscale, -stats[kAttnRows + row]);
+            dp[r] = p * __builtin_fmaf(keep ? dp[r] : 0.0f, dp_scale, -stats[kAttnRows + row]);
         }
-        product_cols<DP>(accv, gc, s);
-        product_cols<DP>(acck, qc, dp);
+        add_tile<DP>(accv, gc, go_rows, s);
+        add_tile<DP>(acck, qc, query_rows, dp);
     }
     if (key >= a.Tk) return;
     // partial sums: [split][array][head][key][D]
@@ -1162,8 +1283,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int c = 32 * d + 8 * g + 4 * (lane >> 5);
-            store_scaled(out_k, c, a.D, acck[d], g, valid, a.scale * reciprocal_power(sc.q) * reciprocal_power(sc.ds));
-            store_scaled(out_v, c, a.D, accv[d], g, valid, 0x1p-14f * reciprocal_power(sc.g) * (DROP ? a.rate.scale : 1.0f));
+            store_scaled(out_k, c, a.D, acck[d], g, valid, a.scale);
+            store_scaled(out_v, c, a.D, accv[d], g, valid, DROP ? a.rate.scale : 1.0f);
         }
 }
 
@@ -1211,16 +1332,25 @@ static int attn_launch(const char* name, void (*kernel)(P...), long grid, int gr
     return CGT_AMD_OK;
 }
 
-static int launch_ranges(const Attn& a, const RangeArrays& arrays, int n_arrays, int runs, float2* out, float* window, hipStream_t st) {
+static size_t scale_floats(long heads, long T) { return (size_t)heads * (cdiv(T, kAttnRows) + T); }
+// Fills `scales` (of n arrays of Tk or Tq rows) and the bias window behind them, both at `ws`.
+static int launch_scales(const Attn& a, const ScaledArrays& arrays, int n_arrays, int runs, float* ws, Scales* scales, hipStream_t st) {
+    const long heads = (long)a.B * a.H;
+    long at = 0;
+    for (int n = 0; n < n_arrays; ++n) {
+        scales->start[n] = at;
+        at += (long)scale_floats(heads, arrays.keys[n] ? a.Tk : a.Tq);
+    }
+    scales->arrays = ws, scales->window = ws + at, scales->heads = (int)heads;
     return attn_width(a, [&](auto width) {
-        return attn_launch("attention ranges", attn_range_kernel<decltype(width)::value>, (long)a.B * a.H * runs, n_arrays + (a.table ? 1 : 0), kAttnThreads, 0,
-                           st, a, arrays, n_arrays, runs, out, window);
+        return attn_launch("attention scales", attn_scale_kernel<decltype(width)::value>, heads * runs, n_arrays + (a.table ? 1 : 0), kAttnThreads, 0,
+                           st, a, arrays, *scales, n_arrays, runs);
     });
 }
-// Runs of rows whose largest values are found by workgroups of their own: 256 rows or more, 64 at most.  (16 at most:
+// Runs of rows whose scales are found by workgroups of their own: 256 rows or more, 64 at most.  (16 at most:
 // 64 queries of 2 heads against 16384 keys 48 us, with 64 37.  Runs of 64 rows: 128 heads of 1024 rows 158 us forward
 // and 539 backward, with 256 154 and 520; 4 heads of 512 21 us, with 256 23.)
-static int range_runs(long Tq, long Tk) { return (int)std::max(1L, std::min(cdiv(std::max(Tq, Tk), 256), 64L)); }
+static int scale_runs(long Tq, long Tk) { return (int)std::max(1L, std::min(cdiv(std::max(Tq, Tk), 256), 64L)); }
 // Into how many runs the walked axis (`rows` long) is cut, so that `whole` workgroups become enough to fill
 // every CU `resident` times (twice as often where a causal mask makes them uneven); runs of `shortest` rows at least.
 // Up to a quarter of that where the workgroups are fewer than the CUs, until they are as many.  Both sides (64 columns):
@@ -1314,24 +1444,21 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
     // Too few workgroups to fill the chip: the keys are cut too.
     const int splits = token ? (whole >= 4 * kNumCU ? 1 : (int)std::max(1L, std::min({cdiv(8L * kNumCU, whole), Tk / 128, 64L})))
                              : axis_splits(whole, Tk, DP == 128 ? 2 : 3, a.causal, 512);
-    CGT_ARG_CHECK(whole * splits < (1L << 31) && heads * range_runs(Tq, Tk) < (1L << 31), "attention: too many workgroups");
-    // workspace: the heads' ranges, then the pieces of a split key axis
-    const int runs = range_runs(Tq, Tk);
-    const size_t rows = splits > 1 ? (size_t)heads * Tq * splits : 0, range_floats = token ? 0 : (size_t)heads * runs * 2 * 2 + (table ? bias_window(a.rule) * H : 0) + 2 & ~(size_t)1;
+    CGT_ARG_CHECK(whole * splits < (1L << 31) && heads * scale_runs(Tq, Tk) < (1L << 31), "attention: too many workgroups");
+    // workspace: the scales of k's and v's rows and the bias window, then the pieces of a split key axis
+    const size_t rows = splits > 1 ? (size_t)heads * Tq * splits : 0, window_floats = table && !token ? (size_t)bias_window(a.rule) * H : 0;
+    const size_t shared_floats = token ? 0 : (2 * scale_floats(heads, Tk) + window_floats + 1) & ~(size_t)1;
     float* part = nullptr;
     float2* ml = nullptr;
-    Ranges ranges = {nullptr, runs, nullptr};
-    if (rows + range_floats) {
-        float* ws = stream_workspace(stream, kWsAttention, (range_floats + rows * (D + 2)) * sizeof(float), "attention");
+    Scales scales = {};
+    if (rows + shared_floats) {
+        float* ws = stream_workspace(stream, kWsAttention, (shared_floats + rows * (D + 2)) * sizeof(float), "attention");
         if (!ws) return CGT_AMD_ERR_NOMEM;
-        ranges.at = reinterpret_cast<const float2*>(ws);
-        ml = reinterpret_cast<float2*>(ws + range_floats);
-        part = ws + range_floats + 2 * rows;
-    }
-    if (!token) {      // (no keys: no rows are read, but the kernel still takes its scales and bias from there)
-        float* window = reinterpret_cast<float*>(const_cast<float2*>(ranges.at)) + heads * runs * 2 * 2;
-        ranges.window = window;
-        if (int rc = launch_ranges(a, {{k, v}, {1, 1}, {0, 0}}, 2, runs, const_cast<float2*>(ranges.at), window, st)) return rc;
+        ml = reinterpret_cast<float2*>(ws + shared_floats);
+        part = ws + shared_floats + 2 * rows;
+        if (!token) {
+            if (int rc = launch_scales(a, {{k, v}, {1, 1}}, 2, scale_runs(Tk, Tk), ws, &scales, st)) return rc;
+        }
     }
     const size_t window_bytes = table ? bias_window(a.rule) * sizeof(float) : 0;
     const int rc = attn_dispatch(a, [&](auto width, auto bias, auto drop) {
@@ -1346,8 +1473,8 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
                                  : attn_launch("attention (few queries)", attn_token_kernel<W, 8, bias_>, whole * splits, 1, kAttnThreads, window_bytes, st,
                                                a, o, lse, part, ml, splits);
         }
-        const size_t lds_bytes = Tile<W>::kRowBytes + Tile<W>::kColBytes + window_bytes;
-        return attn_launch("attention forward", attn_fwd_kernel<W, bias_, drop_>, whole * splits, 1, kAttnThreads, lds_bytes, st, a, ranges, o, lse, part, ml,
+        const size_t lds_bytes = Tile<W>::kRowBytes + Tile<W>::kColBytes + 2 * kAttnRows * sizeof(float) + window_bytes;
+        return attn_launch("attention forward", attn_fwd_kernel<W, bias_, drop_>, whole * splits, 1, kAttnThreads, lds_bytes, st, a, scales, o, lse, part, ml,
                            tiles, splits);
     });
     if (rc != CGT_AMD_OK) return rc;
@@ -1385,26 +1512,27 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
     a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths;
     hipStream_t st = as_stream(stream);
     const int DP = padded_dim(a.D), qtiles = (int)cdiv(Tq, kAttnCols), ktiles = (int)cdiv(Tk, kAttnCols);
-    const int runs = range_runs(Tq, Tk);
+    const int runs = scale_runs(Tq, Tk);
     CGT_ARG_CHECK(heads * qtiles < (1L << 31) && heads * ktiles < (1L << 31) && heads * runs < (1L << 31), "attention backward: too many workgroups");
     const int qsplits = axis_splits(heads * qtiles, Tk, DP == 128 ? 1 : 2, a.causal, 256), ksplits = axis_splits(heads * ktiles, Tq, DP == 128 ? 1 : 2, a.causal, 256);
-    // workspace: ranges, row products, the table's partial rows, partial gradients (of the queries, then of the keys)
+    // workspace: the rows' scales, the bias window, row products, the table's partial rows, partial gradients (of the queries,
+    // then of the keys)
     const long parts = B * qtiles * qsplits;
-    const size_t window_floats = table ? (size_t)bias_window(a.rule) * H : 0, range_floats = (size_t)heads * runs * 4 * 2 + window_floats;
+    const size_t window_floats = table ? (size_t)bias_window(a.rule) * H : 0, range_floats = 2 * (scale_floats(heads, Tk) + scale_floats(heads, Tq)) + window_floats;
     const size_t table_floats = table ? (size_t)(parts * H * buckets) : 0;
     const size_t part_floats = std::max(qsplits > 1 ? (size_t)qsplits * heads * Tq * D : 0, ksplits > 1 ? (size_t)ksplits * 2 * heads * Tk * D : 0);
     float* ws = stream_workspace(stream, kWsAttention, (range_floats + heads * Tq + table_floats + part_floats) * sizeof(float), "attention backward");
     if (!ws) return CGT_AMD_ERR_NOMEM;
     float *delta = ws + range_floats, *part_table = delta + heads * Tq, *part = part_table + table_floats;
-    const Ranges ranges = {reinterpret_cast<const float2*>(ws), runs, ws + range_floats - window_floats};
-    int rc = launch_ranges(a, {{k, v, q, go}, {1, 1, 0, 0}, {0, 1, 0, 1}}, 4, runs, reinterpret_cast<float2*>(ws), ws + range_floats - window_floats, st);
+    Scales scales = {};
+    int rc = launch_scales(a, {{k, v, q, go}, {1, 1, 0, 0}}, 4, runs, ws, &scales, st);
     if (rc != CGT_AMD_OK) return rc;
     const size_t window_bytes = table ? bias_window(a.rule) * sizeof(float) : 0;
     rc = attn_dispatch(a, [&](auto width, auto bias, auto drop) {
         constexpr int W = decltype(width)::value;
         constexpr bool bias_ = decltype(bias)::value, drop_ = decltype(drop)::value;
-        const size_t lds_bytes = 2 * Tile<W>::kRowBytes + Tile<W>::kColBytes + (bias_ ? 4 * kSquare * sizeof(float) : 0) + 5 * window_bytes;
-        return attn_launch("attention backward (queries)", attn_bwd_q_kernel<W, bias_, drop_>, heads * qtiles * qsplits, 1, kAttnThreads, lds_bytes, st, a, ranges,
+        const size_t lds_bytes = 2 * Tile<W>::kRowBytes + Tile<W>::kColBytes + 2 * kAttnRows * sizeof(float) + (bias_ ? 4 * kSquare * sizeof(float) : 0) + 5 * window_bytes;
+        return attn_launch("attention backward (queries)", attn_bwd_q_kernel<W, bias_, drop_>, heads * qtiles * qsplits, 1, kAttnThreads, lds_bytes, st, a, scales,
                            o, lse, go, gq, part, delta, part_table, qtiles, qsplits);
     });
     if (rc != CGT_AMD_OK) return rc;
@@ -1427,8 +1555,8 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
         rc = attn_dispatch(a, [&](auto width, auto bias, auto drop) {
             constexpr int W = decltype(width)::value;
             constexpr bool bias_ = decltype(bias)::value, drop_ = decltype(drop)::value;
-            const size_t lds_bytes = 2 * Tile<W>::kRowBytes + 2 * Tile<W>::kColBytes + (2 * kAttnRows + (drop_ ? kAttnThreads : 0)) * sizeof(float) + window_bytes;
-            return attn_launch("attention backward (keys)", attn_bwd_kv_kernel<W, bias_, drop_>, heads * ktiles * ksplits, 1, kAttnThreads, lds_bytes, st, a, ranges,
+            const size_t lds_bytes = 2 * Tile<W>::kRowBytes + 2 * Tile<W>::kColBytes + (4 * kAttnRows + (drop_ ? kAttnThreads : 0)) * sizeof(float) + window_bytes;
+            return attn_launch("attention backward (keys)", attn_bwd_kv_kernel<W, bias_, drop_>, heads * ktiles * ksplits, 1, kAttnThreads, lds_bytes, st, a, scales,
                                lse, delta, go, gk, gv, part, ktiles, ksplits);
         });
         if (rc != CGT_AMD_OK) return rc;

@@ -34,3 +34,157 @@ def test_bias_gradient_where_workgroups_have_nothing_to_do(K):
     o, lse = K.rel_attention_fwd(args[0], none, none, args[3])
     gtable = K.rel_attention_bwd(args[0], none, none, args[3], o, lse, dev(go))[3]
     assert not gtable.get().any()
+
+
+# ---------------------------------------------------------------- rows of very different size within one head
+
+def plain32(q, k, v, table, go, causal=False, max_distance=128, bidirectional=None, keep=1.0):
+    """The composition of elementary operations in float32: (o, gq, gk, gv)."""
+    f = np.float32
+    Tq, Tk = q.shape[2], k.shape[2]
+    scale = f(q.shape[3] ** -0.5)
+    i, j = np.arange(Tq)[:, None], np.arange(Tk)[None, :]
+    s = np.matmul(q * scale, k.transpose(0, 1, 3, 2))
+    if table is not None:
+        rel = np.arange(1 - Tq, Tk)
+        by_rel = np.array([T.bucket(int(r), table.shape[0], max_distance, not causal if bidirectional is None else bidirectional) for r in rel])
+        s = s + table.T[:, by_rel][:, j - i + Tq - 1]
+    if causal:
+        s = np.where(j <= i, s, f(-np.inf))
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    w = (p * keep).astype(f)
+    o = np.matmul(w, v)
+    gp = np.matmul(go, v.transpose(0, 1, 3, 2)) * keep
+    ds = (p * (gp - (go * o).sum(-1, keepdims=True))).astype(f)
+    return o, np.matmul(ds, k) * scale, np.matmul(ds.transpose(0, 1, 3, 2), q) * scale, np.matmul(w.transpose(0, 1, 3, 2), go)
+
+
+def units(att, go):
+    """For o, gq, gk and gv: what one rounding in every operation leaves in an element, errors of different operations added as
+    a random walk.  Scores are off by a share of their largest products, of the largest score and of lse; that error of p,
+    and those of go . v and go . o, go through the sums."""
+    sq = np.square
+    q, k, v, p, w = att.q, att.k, att.vm, att.prob, att.prob * att.keep
+    root = lambda spec, *ops: np.sqrt(np.einsum(spec, *[sq(a) for a in ops]))      # noqa: E731
+    s = att.scale * root("bhid,bhjd->bhij", q, k)
+    es = U * (np.max(np.where(p > 0, s, 0.0), -1) + 2 * np.max(np.abs(np.where(p > 0, att.scores, 0.0)), -1) + 1)[..., None]     # of a row's scores
+    gp = att.keep * np.einsum("bhid,bhjd->bhij", go, v)
+    delta = (go * att.o).sum(-1, keepdims=True)
+    egp, edelta = U * att.keep * root("bhid,bhjd->bhij", go, v), U * np.sqrt(sq(go * att.o).sum(-1, keepdims=True))
+    eo = es * root("bhij,bhjd->bhid", w, v) + (es + U) * np.abs(att.o)
+    ds = p * (gp - delta)
+    # go . o carries what o is off by; it goes into all of a row's ds alike
+    row = edelta + np.sqrt((sq(go * eo)).sum(-1, keepdims=True))
+    eds = np.sqrt(sq(ds * es) + sq(p * egp) + sq(p * U * gp))
+    gq = att.scale * (root("bhij,bhjd->bhid", eds, k) + row * np.abs(np.einsum("bhij,bhjd->bhid", p, k)) + es * np.abs(np.einsum("bhij,bhjd->bhid", ds, k)))
+    gk = att.scale * root("bhij,bhid->bhjd", np.sqrt(sq(eds) + sq(p * row) + sq(ds * es)), q)
+    gv = root("bhij,bhid->bhjd", w * (es + U), go)
+    return eo, gq + U * np.abs(att.scale * np.einsum("bhij,bhjd->bhid", ds, k)), gk, gv
+
+
+def rows_close(got, want, plain, unit, name):
+    """Each row to float32 accuracy: within 8 times what float32 numpy is off by on that row, or (where it is lucky) a rounding
+    in every operation would leave.  The operands of a score have 22 bits, so a product is off by up to 4 U where a
+    rounding gives U, and a matrix instruction cuts its sum's last bits where numpy rounds them: 4 times 2."""
+    norm = lambda a: np.sqrt((np.asarray(a, np.float64) ** 2).sum(-1))      # noqa: E731
+    assert np.isfinite(got).all(), name
+    off, allowed = norm(got - want), 8 * np.maximum(norm(plain - want), norm(unit)) + 1e-37
+    worst = np.max(off / allowed)
+    at = np.unravel_index(np.argmax(off / allowed), off.shape)
+    size = np.maximum(norm(want)[at], 1e-300)
+    said = "%s, row %s: off by %.3g of it, float32 numpy by %.3g, a rounding an operation %.3g" % (
+        name, tuple(map(int, at)), off[at] / size, norm(plain - want)[at] / size, norm(unit)[at] / size)
+    print("%.2f" % worst, said)
+    assert worst <= 1, said
+
+
+def spread(rs, n, low):
+    """Factors from `low` to 1, one of them 1."""
+    f = np.exp(rs.uniform(np.log(low), 0.0, n))
+    f[rs.randint(n)] = 1.0
+    return f[:, None]
+
+
+SPREADS = {
+    "normal": dict(),
+    "small cotangents": dict(go=1e-6),
+    "one large cotangent": dict(go=(7, 1e4)),
+    "spread values": dict(v=1e-6),
+    "one large value": dict(v=(300, 1e2)),
+    "a huge value most queries do not see": dict(v=(690, 1e6), causal=True),
+    "spread queries": dict(q=1e-4),
+    "one large key": dict(k=(300, 30.0)),
+    "a huge key most queries do not see": dict(k=(690, 1e4), causal=True),
+    "garbage behind the causal horizon": dict(k=(690, 1e20), v=(690, 1e25), causal=True, Tq=600),
+    "tiny values and cotangents": dict(scales=(1, 1, 1e-15, 1e-15)),
+    "everything spread, dropout": dict(q=1e-3, k=1e-3, v=1e-5, go=1e-5, p=0.2),
+    "sharp": dict(scales=(12, 1, 1, 1)),
+    "a huge value among the first": dict(v=(3, 1e8), causal=True),
+    "a huge key among the first": dict(k=(3, 1e3), causal=True),
+    "blocks of values of very different size": dict(v=[1e-25, 1.0, 1e-12, 1e12], go=[1e-10, 1.0]),
+    "blocks of keys of very different size": dict(k=[1e-20, 1.0, 1e-6], q=[1.0, 1e-15]),
+    "rows of zeros": dict(k="zeros", v="zeros", q="zeros", go="zeros"),
+}
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("name", sorted(SPREADS))
+def test_rows_of_any_size_keep_float32_accuracy(K, name, D):
+    how = SPREADS[name]
+    rs = np.random.RandomState(len(name) + D)
+    H, Tq, Tk = 2, how.get("Tq", 700), 700
+    arrays = {n: rs.randn(1, H, t, D) for n, t in (("q", Tq), ("k", Tk), ("v", Tk), ("go", Tq))}
+    for n, f in zip(("q", "k", "v", "go"), how.get("scales", ())):
+        arrays[n] *= f
+    for n, a in arrays.items():
+        f = how.get(n)
+        if isinstance(f, tuple):
+            a[:, 1, f[0]] *= f[1]          # the second head; the first stays as it is
+        elif isinstance(f, list):          # runs of 96 rows
+            a[:, 1] *= np.array(f)[np.arange(a.shape[2]) // 96 % len(f)][:, None]
+        elif f == "zeros":                 # single ones, and whole tiles
+            a[:, 1] *= spread(rs, a.shape[2], 1e-4)
+            a[:, 1, 1::3] = 0.0
+            a[:, 1, 64:130] = 0.0
+        elif f:
+            a[:, 1] *= spread(rs, a.shape[2], f)
+    q, k, v, go = (arrays[n].astype(np.float32) for n in ("q", "k", "v", "go"))
+    table = (0.5 * rs.randn(32, H)).astype(np.float32)
+    causal, p = how.get("causal", False), how.get("p", 0.0)
+    keep = T.attention_keep(1, H, Tq, Tk, p, 31337, 2) if p else None
+    seen = slice(0, Tq if causal else Tk)      # (keys that no query sees do not count)
+    att = T.Attention(q, k[:, :, seen], v[:, :, seen], table, causal=causal, keep=keep)
+    att.scores = att.scale * np.matmul(att.q, att.k.transpose(0, 1, 3, 2)) + table.astype(np.float64)[att.bucket].transpose(2, 0, 1)
+    plain = plain32(q, k[:, :, seen], v[:, :, seen], table, go, causal, keep=1.0 if keep is None else keep.astype(np.float32))
+    more = dict(causal=causal)
+    if p:
+        more.update(p=p, rng=dev(np.array([31337, 2]), np.int64))
+    ins = [dev(a) for a in (q, k, v, table)]
+    o, lse = K.rel_attention_fwd(*ins, **more)
+    unit = units(att, go.astype(np.float64))
+    rows_close(o.get(), att.o, plain[0], unit[0], "o")
+    gq, gk, gv, gtable = K.rel_attention_bwd(*ins, o, lse, dev(go), **more)
+    want = att.pullback(go)
+    for a, w, p32, u, n in zip((gq.get(), gk.get()[:, :, seen], gv.get()[:, :, seen]), want, plain[1:], unit[1:], ("gq", "gk", "gv")):
+        rows_close(a, w, p32, u, n)
+    # the table's gradient is a sum over all pairs: a random walk of their roundings, and a share of each pair's own error
+    ds = att.prob * (np.matmul(go.astype(np.float64), att.v.transpose(0, 1, 3, 2)) * att.keep - (go * att.o).sum(-1, keepdims=True))
+    allowed = 64 * U * np.sqrt((ds ** 2).sum((0, 2, 3))) + 8 * U * np.abs(ds).sum((0, 2, 3))
+    assert np.all(np.abs(gtable.get() - want[3]).max(0) <= allowed)
+
+
+@pytest.mark.parametrize("Tq", [1, 5, 40])
+def test_forward_rows_of_any_size_against_long_keys(K, Tq):
+    # cut key axes and the join, at float32 accuracy
+    rs = np.random.RandomState(Tq)
+    H, Tk, D = 2, 6000, 64
+    q, k, v = rs.randn(1, H, Tq, D), rs.randn(1, H, Tk, D), rs.randn(1, H, Tk, D)
+    v[:, 1] *= spread(rs, Tk, 1e-5)
+    q, k, v = (a.astype(np.float32) for a in (q, k, v))
+    o, lse = K.rel_attention_fwd(dev(q), dev(k), dev(v))
+    att = T.Attention(q, k, v)
+    att.scores = att.scale * np.matmul(att.q, att.k.transpose(0, 1, 3, 2))
+    zero = np.zeros_like(q)
+    rows_close(o.get(), att.o, plain32(q, k, v, None, zero)[0], units(att, zero.astype(np.float64))[0], "o")
+    assert np.abs(lse.get() - att.lse).max() <= 16 * U * np.abs(att.lse).max()
