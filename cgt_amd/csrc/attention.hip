@@ -176,7 +176,7 @@ __device__ __forceinline__ v16f mul_step(v16f acc, const Frag& a, const Frag& b)
 // What a tile's rows are scaled by: one power of two, or 0 and one for each row where the rows are mixed (rare: see
 // attn_scale_kernel).  Where they are not, a tile costs one load that all lanes share.
 struct ScaleArray {
-    const float *tiles, *rows;      // a head's
+    const float *tiles, *rows, *weights;      // a head's; weights of rows (null: 1) that go into what undoes the scales of a mixed tile
 };
 __device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 
@@ -236,7 +236,7 @@ struct Tile {
     }
     // `factors`: where a mixed tile (row0 its first row, `end` as in load) leaves the reciprocals of its rows' scales
     template <bool ROWS, bool COLS>
-    __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols, float tile_scale, const float* row_scales, float* factors, int row0, int end) const {
+    __device__ __forceinline__ void store(unsigned short* rows, unsigned short* cols, float tile_scale, const ScaleArray& scales, float* factors, int row0, int end) const {
         if (__builtin_expect(tile_scale != 0.0f, 1)) {
             const float scale[4] = {tile_scale, tile_scale, tile_scale, tile_scale};
             store<ROWS, COLS>(rows, cols, scale);
@@ -244,8 +244,9 @@ struct Tile {
             float scale[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                scale[r] = row_scales[min(row0 + (int)(threadIdx.x >> 5) * 4 + r, end - 1)];
-                if ((threadIdx.x & 31) == 0) factors[(threadIdx.x >> 5) * 4 + r] = reciprocal_power(scale[r]);
+                const int row = min(row0 + (int)(threadIdx.x >> 5) * 4 + r, end - 1);
+                scale[r] = scales.rows[row];
+                if ((threadIdx.x & 31) == 0) factors[(threadIdx.x >> 5) * 4 + r] = reciprocal_power(scale[r]) * (scales.weights ? scales.weights[row] : 1.0f);
             }
             store<ROWS, COLS>(rows, cols, scale);
         }
@@ -367,8 +368,14 @@ constexpr float kLn2 = 0.6931471805599453f, kLowest = -3.4028234663852886e38f;
 __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }      // below 2^-126 it is 0
 // x log2 e; finite values stay finite at the lower end (a bias of the lowest float)
 __device__ __forceinline__ float to_log2(float x) { return x < -1e38f && x >= kLowest ? fmaxf(x * kLog2e, kLowest) : x * kLog2e; }
-// log sum exp from the reference of a row's exponentials (in powers of two) and their sum
-__device__ __forceinline__ float log_sum(float ref, float sum) { return ref < -1e38f ? ref : ref * kLn2 + logf(sum); }
+// log sum exp from the reference of a row's exponentials (in powers of two) and their sum; the lowest float stays what it is
+__device__ __forceinline__ float log_sum(float ref, float sum) { return ref == kLowest ? ref : ref * kLn2 + logf(sum); }
+// What the backward pass takes from a row's scores, p = 2^(s - this).  Infinity, that is p = 0, for a row that saw nothing,
+// and for one whose lse has no digits behind the point: next to 2^22 a rounding of it is a factor in p.  The lowest
+// float is exact: p is 1 for every key there, and the row's weight (attn_scale_kernel) has their number.
+__device__ __forceinline__ float row_reference(float lse) {
+    return lse == kLowest ? lse : fabsf(lse) >= 0x1p22f ? INFINITY : lse * kLog2e;
+}
 
 // What undoes the scales of a tile's rows: one factor, or 32 in LDS where the rows are mixed.  A product of such a tile is
 // multiplied row by row, by a branch around 16 multiplications that the other tiles do without.
@@ -539,22 +546,36 @@ __device__ __forceinline__ float group_max(float x) {
 // position, [head of H][window], in the grid's last row.  A tile's scale brings its largest magnitude (values that are no
 // numbers left out) to [2^14, 2^15), unless a row, not all zeros, is smaller by more than 2^8: there it is 0, and each row's brings
 // its own.  So the 22 bits of a row reach down to 2^-9 of its largest value at least, whatever other rows hold.
+//
+// With go comes lse.  A row whose lse is the lowest float has nothing but keys of that bias, p is 1 for each of them in the
+// backward kernels, and go and go . o get the reciprocal of their number as a weight (1 for all other rows).  Its tile
+// counts as mixed.
 struct ScaledArrays {
     const float* base[4];
     int keys[4];      // 1: laid out and limited as k, 0: as q
+    const float* lse;      // of the fourth
 };
 // Where they are: of each array first the tiles', [head][tile], then the rows', [head][row].
 struct Scales {
-    const float *arrays, *window;
+    const float *arrays, *window, *weights;      // weights of the rows of the fourth, [head][row]
     long start[4];
     int heads;
     __device__ __forceinline__ ScaleArray of(int array, int head, int T) const {
         const int tiles = (T + kAttnRows - 1) / kAttnRows;
         const float* at = arrays + start[array];
-        return {at + (long)head * tiles, at + (long)heads * tiles + (long)head * T};
+        return {at + (long)head * tiles, at + (long)heads * tiles + (long)head * T, array == 3 ? weights + (long)head * T : nullptr};
     }
 };
-template <int DP>
+// How many keys a query may see that are not switched off by a bias of -inf.
+__device__ __forceinline__ int keys_in_sight(const Attn& a, int b, int h, int query) {
+    int end = length_of(a.k_lengths, b, a.Tk), n = 0;
+    if (a.causal) end = min(end, query + a.q_offset + 1);
+    if (!a.table) return end;
+    for (int j = 0; j < end; ++j) n += a.table[(long)bucket_of(a.rule, j - query - a.q_offset) * a.H + h] >= kLowest ? 1 : 0;
+    return n;
+}
+// BACKWARD: with lse and weights.
+template <int DP, bool BACKWARD>
 __global__ __launch_bounds__(kAttnThreads) void attn_scale_kernel(Attn a, ScaledArrays arrays, Scales scales, int n_arrays, int runs) {
     constexpr int LANES = DP / 4, STEP = kAttnThreads / LANES, DEEP = 8;
     __shared__ float tops[kAttnThreads];
@@ -593,10 +614,13 @@ __global__ __launch_bounds__(kAttnThreads) void attn_scale_kernel(Attn a, Scaled
         }
         __syncthreads();
         const float top = tops[threadIdx.x], tile = group_max<kAttnRows>(top);
-        const bool mixed = group_max<kAttnRows>(top > 0.0f && top < 0x1p-8f * tile ? 1.0f : 0.0f) > 0.0f;
-        if (c0 + (int)threadIdx.x < last) {
-            const_cast<float*>(to.rows)[c0 + threadIdx.x] = power_scale(top);
-            if (threadIdx.x % kAttnRows == 0) const_cast<float*>(to.tiles)[(c0 + threadIdx.x) / kAttnRows] = mixed ? 0.0f : power_scale(tile);
+        const int row = c0 + threadIdx.x;
+        const bool lowest = BACKWARD && n == 3 && row < last && arrays.lse[(long)head * T + row] == kLowest;
+        const bool mixed = group_max<kAttnRows>(lowest || (top > 0.0f && top < 0x1p-8f * tile) ? 1.0f : 0.0f) > 0.0f;
+        if (BACKWARD && n == 3 && row < last) const_cast<float*>(to.weights)[row] = lowest ? 1.0f / (float)max(1, keys_in_sight(a, b, h, row)) : 1.0f;
+        if (row < last) {
+            const_cast<float*>(to.rows)[row] = power_scale(top);
+            if (threadIdx.x % kAttnRows == 0) const_cast<float*>(to.tiles)[row / kAttnRows] = mixed ? 0.0f : power_scale(tile);
         }
         __syncthreads();
     }
@@ -677,8 +701,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     for (int j0 = first; j0 < last; j0 += kAttnRows) {
         const float kscale = uniform(knext), vscale = uniform(vnext);
         __syncthreads();
-        kr.template store<true, false>(kt, nullptr, kscale, kscales.rows, krows, j0, last);
-        vr.template store<false, true>(nullptr, vt, vscale, vscales.rows, vrows, j0, last);
+        kr.template store<true, false>(kt, nullptr, kscale, kscales, krows, j0, last);
+        vr.template store<false, true>(nullptr, vt, vscale, vscales, vrows, j0, last);
         __syncthreads();
         if (j0 + kAttnRows < last) {
             kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
@@ -1011,10 +1035,13 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
     gcol.load(go + qrow, valid, a.D);
     const float gscale = power_scale(gcol.top());
     gcol.split(gscale, -1.0f);
-    const float unscale = a.scale * kLog2e * reciprocal_power(qscale), dscale = reciprocal_power(gscale) * (DROP ? a.rate.scale : 1.0f);
+    const float unscale = a.scale * kLog2e * reciprocal_power(qscale);
+    float dscale = reciprocal_power(gscale) * (DROP ? a.rate.scale : 1.0f);
+    const float weight = valid ? scales.weights[stat] : 1.0f;
+    dl *= weight;
+    dscale *= weight;
     if (query < a.Tq && lane < 32 && split == 0) delta[stat] = dl;
-    float row_lse = valid ? to_log2(lse[stat]) : INFINITY;
-    if (row_lse == -INFINITY) row_lse = INFINITY;      // a row that saw nothing: every probability is 0
+    const float row_lse = valid ? row_reference(lse[stat]) : INFINITY;
     RngState rng = {};
     unsigned long long group0 = 0;
     if (DROP) {
@@ -1035,8 +1062,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
     for (int j0 = first; j0 < last; j0 += kAttnRows) {
         const float kscale = uniform(knext), vscale = uniform(vnext);
         __syncthreads();
-        kr.template store<true, true>(kt, kc, kscale, kscales.rows, krows, j0, last);
-        vr.template store<true, false>(vt, nullptr, vscale, vscales.rows, vrows, j0, last);
+        kr.template store<true, true>(kt, kc, kscale, kscales, krows, j0, last);
+        vr.template store<true, false>(vt, nullptr, vscale, vscales, vrows, j0, last);
         __syncthreads();
         if (j0 + kAttnRows < last) {
             kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
@@ -1217,12 +1244,11 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
     for (int i0 = first; i0 < last; i0 += kAttnRows) {
         const float qscale = uniform(qnext), gscale = uniform(gnext);
         __syncthreads();
-        qr.template store<true, true>(qt, qc, qscale, qscales.rows, qrows, i0, last);
-        gr.template store<true, true>(gt, gc, gscale, gscales.rows, grows, i0, last);
+        qr.template store<true, true>(qt, qc, qscale, qscales, qrows, i0, last);
+        gr.template store<true, true>(gt, gc, gscale, gscales, grows, i0, last);
         if (threadIdx.x < kAttnRows) {
             const int i = i0 + threadIdx.x;
-            const float v = i < last ? lse[stat0 + i] : INFINITY;
-            stats[threadIdx.x] = v == -INFINITY ? INFINITY : to_log2(v);
+            stats[threadIdx.x] = row_reference(i < last ? lse[stat0 + i] : INFINITY);
             stats[kAttnRows + threadIdx.x] = i < last ? delta[stat0 + i] : 0.0f;
         }
         __syncthreads();
@@ -1333,7 +1359,7 @@ static int attn_launch(const char* name, void (*kernel)(P...), long grid, int gr
 }
 
 static size_t scale_floats(long heads, long T) { return (size_t)heads * (cdiv(T, kAttnRows) + T); }
-// Fills `scales` (of n arrays of Tk or Tq rows) and the bias window behind them, both at `ws`.
+// Fills `scales` (of n arrays of Tk or Tq rows), the weights (if there is lse) and the bias window behind them, all at `ws`.
 static int launch_scales(const Attn& a, const ScaledArrays& arrays, int n_arrays, int runs, float* ws, Scales* scales, hipStream_t st) {
     const long heads = (long)a.B * a.H;
     long at = 0;
@@ -1341,10 +1367,11 @@ static int launch_scales(const Attn& a, const ScaledArrays& arrays, int n_arrays
         scales->start[n] = at;
         at += (long)scale_floats(heads, arrays.keys[n] ? a.Tk : a.Tq);
     }
-    scales->arrays = ws, scales->window = ws + at, scales->heads = (int)heads;
+    scales->arrays = ws, scales->weights = ws + at, scales->window = ws + at + (arrays.lse ? heads * a.Tq : 0), scales->heads = (int)heads;
     return attn_width(a, [&](auto width) {
-        return attn_launch("attention scales", attn_scale_kernel<decltype(width)::value>, heads * runs, n_arrays + (a.table ? 1 : 0), kAttnThreads, 0,
-                           st, a, arrays, *scales, n_arrays, runs);
+        constexpr int W = decltype(width)::value;
+        return attn_launch("attention scales", arrays.lse ? attn_scale_kernel<W, true> : attn_scale_kernel<W, false>, heads * runs,
+                           n_arrays + (a.table ? 1 : 0), kAttnThreads, 0, st, a, arrays, *scales, n_arrays, runs);
     });
 }
 // Runs of rows whose scales are found by workgroups of their own: 256 rows or more, 64 at most.  (16 at most:
@@ -1457,7 +1484,7 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
         ml = reinterpret_cast<float2*>(ws + shared_floats);
         part = ws + shared_floats + 2 * rows;
         if (!token) {
-            if (int rc = launch_scales(a, {{k, v}, {1, 1}}, 2, scale_runs(Tk, Tk), ws, &scales, st)) return rc;
+            if (int rc = launch_scales(a, {{k, v}, {1, 1}, nullptr}, 2, scale_runs(Tk, Tk), ws, &scales, st)) return rc;
         }
     }
     const size_t window_bytes = table ? bias_window(a.rule) * sizeof(float) : 0;
@@ -1518,14 +1545,14 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
     // workspace: the rows' scales, the bias window, row products, the table's partial rows, partial gradients (of the queries,
     // then of the keys)
     const long parts = B * qtiles * qsplits;
-    const size_t window_floats = table ? (size_t)bias_window(a.rule) * H : 0, range_floats = 2 * (scale_floats(heads, Tk) + scale_floats(heads, Tq)) + window_floats;
+    const size_t window_floats = table ? (size_t)bias_window(a.rule) * H : 0, range_floats = 2 * (scale_floats(heads, Tk) + scale_floats(heads, Tq)) + heads * Tq + window_floats;
     const size_t table_floats = table ? (size_t)(parts * H * buckets) : 0;
     const size_t part_floats = std::max(qsplits > 1 ? (size_t)qsplits * heads * Tq * D : 0, ksplits > 1 ? (size_t)ksplits * 2 * heads * Tk * D : 0);
     float* ws = stream_workspace(stream, kWsAttention, (range_floats + heads * Tq + table_floats + part_floats) * sizeof(float), "attention backward");
     if (!ws) return CGT_AMD_ERR_NOMEM;
     float *delta = ws + range_floats, *part_table = delta + heads * Tq, *part = part_table + table_floats;
     Scales scales = {};
-    int rc = launch_scales(a, {{k, v, q, go}, {1, 1, 0, 0}}, 4, runs, ws, &scales, st);
+    int rc = launch_scales(a, {{k, v, q, go}, {1, 1, 0, 0}, lse}, 4, runs, ws, &scales, st);
     if (rc != CGT_AMD_OK) return rc;
     const size_t window_bytes = table ? bias_window(a.rule) * sizeof(float) : 0;
     rc = attn_dispatch(a, [&](auto width, auto bias, auto drop) {

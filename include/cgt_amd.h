@@ -381,7 +381,10 @@ int cgt_amd_dropout_add_layer_norm_bwd_f32(const float *h, const float *gamma, c
  * lose no term to larger ones (the forward pass: terms below 2^-37 of its
  * largest).  Values below 2^-112, and products of go and v below 2^-97, lose
  * digits.  The backward pass forms its probabilities from lse, whose rounding
- * makes them wrong by 2^-24 |lse| relatively.
+ * makes them wrong by 2^-23 |lse| relatively; a query whose |lse| is 2^22 or more
+ * contributes to no gradient.  So keys are switched off with a bias of -inf or of
+ * the lowest float: a query that sees nothing but the latter (biases below -2.3e38
+ * count as it) weighs them equally, in the gradients too.
  *
  * Uses workspaces owned by the library.  Sums run in a fixed order: same input,
  * same bits.  Inputs and outputs must not overlap. */

@@ -36,6 +36,57 @@ def test_bias_gradient_where_workgroups_have_nothing_to_do(K):
     assert not gtable.get().any()
 
 
+@pytest.mark.parametrize("p", [0.0, 0.25])
+@pytest.mark.parametrize("Tq,Tk", [(40, 70), (150, 333)])
+def test_gradients_of_rows_with_nothing_but_the_lowest_bias(K, Tq, Tk, p):
+    # such a row weighs its keys equally; head 0 has rows of all kinds (keys before the query have the lowest bias, keys after it
+    # -inf or an ordinary one), head 1 nothing else
+    lowest = np.float32(-3.4028235e38)
+    c = case(2, 2, Tq, Tk, 32, buckets=8, max_distance=16, p=p, k_lengths=[Tk, Tk - 37], q_lengths=[Tq, Tq - 5])
+    (q, k, v, table, go), _ = make(c)
+    table[:4, 0] = lowest
+    table[4:7, 0] = -np.inf
+    table[:, 1] = lowest
+    keep = T.attention_keep(2, 2, Tq, Tk, p, 31337, 2) if p else 1.0
+    # the same in float64: scores beside a bias that is 0 where it is the lowest, in rows that have no other key
+    att = T.Attention(q, k, v, table, max_distance=16, q_lengths=c["q_lengths"], k_lengths=c["k_lengths"], keep=keep if p else None)
+    bias = table[att.bucket].transpose(2, 0, 1)[None]
+    seen = (np.arange(Tk)[None, :] < np.array(c["k_lengths"])[:, None])[:, None, None, :] & att.q_seen & (bias > -np.inf)
+    alone = ~(seen & (bias > lowest)).any(-1, keepdims=True)
+    assert alone[:, 0].any() and not alone[:, 0].all() and alone[:, 1].all()
+    n = seen.sum(-1, keepdims=True)
+    att.prob = np.where(alone, seen / np.maximum(n, 1), att.prob)
+    att.o = np.einsum("bhij,bhjd->bhid", att.prob * att.keep, att.vm)
+    att.lse = np.where((alone & (n > 0))[..., 0], 0.0, att.lse)      # (for the tolerances: these rows' probabilities are exact)
+    tol = tolerances(att, go)
+    more = arguments(c)
+    o, lse = K.rel_attention_fwd(dev(q), dev(k), dev(v), dev(table), **more)
+    close(o.get(), att.o, tol["o"], "o")
+    assert np.array_equal(lse.get() == lowest, (alone & (n > 0))[..., 0])
+    got = K.rel_attention_bwd(dev(q), dev(k), dev(v), dev(table), o, lse, dev(go), **more)
+    for name, a, want in zip(("gq", "gk", "gv", "gtable"), got, att.pullback(go)):
+        close(a.get(), want, tol[name], name)
+
+
+@pytest.mark.parametrize("value", [-1e7, -1e9, -1e30, -2e38, 1e9])
+def test_rows_whose_lse_has_no_digits_contribute_to_no_gradient(K, value):
+    # head 1 has such rows only, head 0 none
+    c = case(1, 2, 70, 90, 64, buckets=8, max_distance=16)
+    (q, k, v, table, go), _ = make(c)
+    table[:, 1] = value
+    o, lse = K.rel_attention_fwd(dev(q), dev(k), dev(v), dev(table), max_distance=16)
+    assert np.isfinite(o.get()).all() and np.allclose(lse.get()[:, 1], value, rtol=1e-6, atol=0)
+    got = K.rel_attention_bwd(dev(q), dev(k), dev(v), dev(table), o, lse, dev(go), max_distance=16)
+    for a in got[:3]:
+        assert not a.get()[:, 1].any()
+    assert not got[3].get()[:, 1].any()
+    table[:, 1] = 0
+    att = T.Attention(q, k, v, table, max_distance=16)
+    tol = tolerances(att, go)
+    for name, a, want in zip(("gq", "gk", "gv"), got, att.pullback(go)):
+        close(a.get()[:, 0], want[:, 0], tol[name][:, 0], name)
+
+
 # ---------------------------------------------------------------- rows of very different size within one head
 
 def plain32(q, k, v, table, go, causal=False, max_distance=128, bidirectional=None, keep=1.0):
