@@ -101,6 +101,10 @@ PROTOTYPES = {
                                               c_void_p, c_void_p, c_double, c_void_p, c_uint] + [c_void_p] * 3),
     "cgt_amd_rel_attention_bwd_f32": (c_int, [c_void_p] * 7 + [c_long] * 5 + [c_int, c_long, c_int, c_long, c_double, c_int, c_long,
                                               c_void_p, c_void_p, c_double, c_void_p, c_uint] + [c_void_p] * 5),
+    "cgt_amd_rel_attention_at_fwd_f32": (c_int, [c_void_p] * 4 + [c_long] * 5 + [c_int, c_long, c_int, c_long, c_double, c_int, c_void_p,
+                                                 c_void_p, c_void_p, c_double, c_void_p, c_uint] + [c_void_p] * 3),
+    "cgt_amd_rel_attention_at_bwd_f32": (c_int, [c_void_p] * 7 + [c_long] * 5 + [c_int, c_long, c_int, c_long, c_double, c_int, c_void_p,
+                                                 c_void_p, c_void_p, c_double, c_void_p, c_uint] + [c_void_p] * 5),
     "cgt_amd_fill_f32": (c_int, [c_void_p, ctypes.c_float, c_long, c_void_p]),
     "cgt_amd_transpose4_f32": (c_int, [c_void_p, ctypes.POINTER(c_long), ctypes.POINTER(c_int),
                                        c_void_p, c_void_p]),

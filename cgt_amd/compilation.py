@@ -259,15 +259,15 @@ def prebuild_transformer_ops():
     T1, T2 = core.TensorType("f4", 1), core.TensorType("f4", 2)
     T3, T4 = core.TensorType("f4", 3), core.TensorType("f4", 4)
     N, R = core.TensorType("i4", 1), core.TensorType("i8", 1)
-    ainfo = nn_ops.attention.AttentionInfo(1.0, 0, 1, 128, 0, 0.1, 0, 1, 1, 1, 1)
+    ainfo = nn_ops.attention.AttentionInfo(1.0, 0, 1, 128, 0, 0.1, 0, 1, 1, 1, 1, 1)
     return _prebuild([
         (nn_ops.layer_norm.LayerNorm(1e-5), [T2, T1, T1]),
         (nn_ops.layer_norm.LayerNormBackward(), [T2, T1, T1, T1, T2]),
         (nn_ops.layer_norm.DropoutAddLayerNorm(0.1, 1e-5, 0), [T2, T2, T1, T1, R]),
         (nn_ops.layer_norm.DropoutAddLayerNormBackward(0.1, 0, True), [T2, T1, T1, T1, T2, T2, R]),
         (nn_ops.dropout.Dropout(0.1, 0), [T2, R]),
-        (nn_ops.attention.RelativeAttention(ainfo), [T4, T4, T4, T2, N, N, R]),
-        (nn_ops.attention.RelativeAttentionBackward(ainfo), [T4, T4, T4, T2, N, N, R, T4, T3, T4]),
+        (nn_ops.attention.RelativeAttention(ainfo), [T4, T4, T4, T2, N, N, N, R]),
+        (nn_ops.attention.RelativeAttentionBackward(ainfo), [T4, T4, T4, T2, N, N, N, R, T4, T3, T4]),
     ])
 
 

@@ -66,7 +66,7 @@ struct BucketRule {
 
 struct Attn {
     const float *q, *k, *v, *table;
-    const int *q_lengths, *k_lengths;
+    const int *q_lengths, *k_lengths, *q_offsets;
     const long long* rng;
     long q_b, q_h, q_t, k_b, k_h, k_t;      // strides in floats; o, go, gq as q, and v, gk, gv as k
     int B, H, Tq, Tk, D, causal, q_offset;
@@ -511,6 +511,13 @@ __device__ __forceinline__ int length_of(const int* lengths, int b, int T) {
     return n < 0 ? 0 : n > T ? T : n;
 }
 
+// Position of a sequence's first query among its keys.
+constexpr int kMaxOffset = (1 << 29) - 1;
+__device__ __forceinline__ int offset_of(const Attn& a, int b) {
+    if (!a.q_offsets) return a.q_offset;
+    return min(max(a.q_offsets[b], -kMaxOffset), kMaxOffset);
+}
+
 // Sum over aligned groups of N lanes (8, 16 or 32); every lane gets it.
 template <int N>
 __device__ __forceinline__ float group_sum(float x) {
@@ -568,10 +575,11 @@ struct Scales {
 };
 // How many keys a query may see that are not switched off by a bias of -inf.
 __device__ __forceinline__ int keys_in_sight(const Attn& a, int b, int h, int query) {
+    const int q_offset = offset_of(a, b);
     int end = length_of(a.k_lengths, b, a.Tk), n = 0;
-    if (a.causal) end = min(end, query + a.q_offset + 1);
+    if (a.causal) end = min(end, query + q_offset + 1);
     if (!a.table) return end;
-    for (int j = 0; j < end; ++j) n += a.table[(long)bucket_of(a.rule, j - query - a.q_offset) * a.H + h] >= kLowest ? 1 : 0;
+    for (int j = 0; j < end; ++j) n += a.table[(long)bucket_of(a.rule, j - query - q_offset) * a.H + h] >= kLowest ? 1 : 0;
     return n;
 }
 // BACKWARD: with lse and weights.
@@ -630,8 +638,8 @@ __device__ __forceinline__ void copy_bias(const Attn& a, const float* window, in
     for (int s = threadIdx.x; s < n; s += kAttnThreads) win[s] = window[(long)head * n + s];
 }
 // Which of a tile's 16 elements of a lane are hidden; rows are keys, the column is a query.
-__device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_end) {
-    return key >= k_end || (a.causal && key > query + a.q_offset);
+__device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_end, int q_offset) {
+    return key >= k_end || (a.causal && key > query + q_offset);
 }
 
 // ---------------------------------------------------------------- forward
@@ -648,14 +656,14 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     const Where w = where(a, tiles * splits, kHeavyLast);
     const int split = w.tile % splits, q0 = w.tile / splits * kAttnCols;
     const int lane = threadIdx.x & 63, qw = q0 + (threadIdx.x >> 6) * 32, query = qw + (lane & 31);
-    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
+    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk), q_offset = offset_of(a, w.b);
     const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
     const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
     const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
     if (BIAS) copy_bias(a, scales.window, w.h, win);
     // keys this workgroup walks: to the last one its last query sees, cut into `splits` runs of whole tiles
     int last = k_end;
-    if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
+    if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + q_offset));
     if (q0 >= q_end) last = 0;
     const int run = (last + kAttnRows * splits - 1) / (kAttnRows * splits) * kAttnRows;
     const int first = split * run;
@@ -710,16 +718,16 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
             knext = kscales.tiles[j0 / kAttnRows + 1];
             vnext = vscales.tiles[j0 / kAttnRows + 1];
         }
-        if (qw >= q_end || (a.causal && j0 > qw + 31 + a.q_offset)) continue;      // nothing here for this wavefront
-        const int rel0 = j0 - qw - a.q_offset;
+        if (qw >= q_end || (a.causal && j0 > qw + 31 + q_offset)) continue;      // nothing here for this wavefront
+        const int rel0 = j0 - qw - q_offset;
         v16f s = product_rows<DP, false>(kt, qcol);
         const TileRows key_rows(kscale, krows), value_rows(vscale, vrows);
         key_rows.undo(s);
         scores<BIAS>(s, unscale * key_rows.one, a.rule, win, rel0);
-        if (j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset)) {
+        if (j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + q_offset)) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (hidden(a, j0 + tile_row(r), query, k_end)) s[r] = -INFINITY;
+                if (hidden(a, j0 + tile_row(r), query, k_end, q_offset)) s[r] = -INFINITY;
         }
         float top = s[0];
 #pragma unroll
@@ -879,9 +887,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
     __shared__ float2 join_ml[NQ][4];
     const Where w = where(a, splits, kByHead);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % LANES * 4, group = lane / LANES, split = w.tile;
-    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
+    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk), q_offset = offset_of(a, w.b);
     int last = k_end;
-    if (a.causal) last = min(last, max(0, a.Tq + a.q_offset));
+    if (a.causal) last = min(last, max(0, a.Tq + q_offset));
     if (q_end == 0) last = 0;
     const int run = (last + 4 * STEP * splits - 1) / (4 * STEP * splits) * 4 * STEP;
     const int first = split * run;
@@ -921,8 +929,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
             for (int u = 0; u < kTokenUnroll; ++u) {
                 const int j = j0 + u * GROUPS + group;
                 s[u] = group_sum<LANES>(kv[u].x * q[i].x + kv[u].y * q[i].y + (kv[u].z * q[i].z + kv[u].w * q[i].w));
-                if (BIAS) s[u] += win[reach + max(-reach, min(reach, j - i - a.q_offset))];
-                if (j >= last || (a.causal && j > i + a.q_offset)) s[u] = -INFINITY;
+                if (BIAS) s[u] += win[reach + max(-reach, min(reach, j - i - q_offset))];
+                if (j >= last || (a.causal && j > i + q_offset)) s[u] = -INFINITY;
                 top = fmaxf(top, s[u]);
             }
             const float ref = top == -INFINITY ? 0.0f : top, f = pow2(m[i] - ref);
@@ -1002,7 +1010,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
     float* diag = win + window;      // [wavefront][window]: sums of ds by relative position
     const Where w = where(a, tiles * splits, kHeavyLast);
     const int split = w.tile % splits, q0 = w.tile / splits * kAttnCols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, qw = q0 + wave * 32, query = qw + (lane & 31);
-    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
+    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk), q_offset = offset_of(a, w.b);
     const float* kbase = a.k + w.b * a.k_b + w.h * a.k_h;
     const float* vbase = a.v + w.b * a.k_b + w.h * a.k_h;
     const long qrow = w.b * a.q_b + w.h * a.q_h + query * a.q_t;
@@ -1012,7 +1020,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         __syncthreads();      // a workgroup without a key meets no other barrier before its wavefronts add to their sums
     }
     int last = k_end;
-    if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + a.q_offset));
+    if (a.causal) last = min(last, max(0, min(q0 + kAttnCols, q_end) + q_offset));
     if (q0 >= q_end) last = 0;
     const int run = (last + kAttnRows * splits - 1) / (kAttnRows * splits) * kAttnRows, first = split * run;
     last = min(last, first + run);
@@ -1071,10 +1079,10 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
             knext = kscales.tiles[j0 / kAttnRows + 1];
             vnext = vscales.tiles[j0 / kAttnRows + 1];
         }
-        const int rel0 = j0 - qw - a.q_offset;
-        const bool edge = j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + a.q_offset);
+        const int rel0 = j0 - qw - q_offset;
+        const bool edge = j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + q_offset);
         const auto tile_shifts = [&] {
-            return shifts<BIAS>(a.rule, win, rel0, 1, edge, [&](int r) { return hidden(a, j0 + tile_row(r), query, k_end); });
+            return shifts<BIAS>(a.rule, win, rel0, 1, edge, [&](int r) { return hidden(a, j0 + tile_row(r), query, k_end, q_offset); });
         };
         v16f shift;
         if constexpr (shifts_early(DP, DROP)) shift = tile_shifts();
@@ -1204,14 +1212,14 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
     float* win = grows + kAttnRows + (DROP ? kAttnThreads : 0);
     const Where w = where(a, tiles * splits, kHeavyFirst);
     const int split = w.tile % splits, k0 = w.tile / splits * kAttnCols, lane = threadIdx.x & 63, kw = k0 + (threadIdx.x >> 6) * 32, key = kw + (lane & 31);
-    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk);
+    const int q_end = length_of(a.q_lengths, w.b, a.Tq), k_end = length_of(a.k_lengths, w.b, a.Tk), q_offset = offset_of(a, w.b);
     const float* qbase = a.q + w.b * a.q_b + w.h * a.q_h;
     const float* gbase = go + w.b * a.q_b + w.h * a.q_h;
     const long krow = w.b * a.k_b + w.h * a.k_h + key * a.k_t;
     if (BIAS) copy_bias(a, scales.window, w.h, win);
     // queries this workgroup walks: from the first that sees its first key
     int first = 0, last = q_end;
-    if (a.causal) first = max(0, k0 - a.q_offset) / kAttnRows * kAttnRows;
+    if (a.causal) first = max(0, k0 - q_offset) / kAttnRows * kAttnRows;
     if (k0 >= k_end) last = 0;
     const int run = (max(0, last - first) + kAttnRows * splits - 1) / (kAttnRows * splits) * kAttnRows;
     first += split * run;
@@ -1258,7 +1266,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
             qnext = qscales.tiles[i0 / kAttnRows + 1];
             gnext = gscales.tiles[i0 / kAttnRows + 1];
         }
-        const int rel0 = kw - i0 - a.q_offset;
+        const int rel0 = kw - i0 - q_offset;
         if (DROP) {
             // The generator's groups run along the keys of a query.  Lane l forms the numbers of query l % 32 and
             // its half's 16 keys of this tile, bit 8 b + e for number e of 16-key block b, and leaves the bits in LDS,
@@ -1276,9 +1284,9 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
             mine[lane] = mask;
             wave_lds_fence();
         }
-        const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + a.q_offset);
+        const bool edge = kw + 32 > k_end || (a.causal && kw + 31 > i0 + q_offset);
         const auto tile_shifts = [&] {
-            return shifts<BIAS>(a.rule, win, rel0, -1, edge, [&](int r) { return hidden(a, key, i0 + tile_row(r), k_end); });
+            return shifts<BIAS>(a.rule, win, rel0, -1, edge, [&](int r) { return hidden(a, key, i0 + tile_row(r), k_end, q_offset); });
         };
         v16f shift;
         if constexpr (shifts_early(DP, DROP)) shift = tile_shifts();
@@ -1421,7 +1429,7 @@ static int attn_setup(const char* what, Attn* a, long B, long H, long Tq, long T
                       int bidirectional, long max_distance, double scale, int causal, long q_offset, double p, const long long* rng, unsigned channel) {
     CGT_ARG_CHECK(B >= 0 && H >= 0 && Tq >= 0 && Tk >= 0, "%s: negative extent", what);
     CGT_ARG_CHECK(D >= 1 && D <= 128, "%s: heads of %ld columns (1 to 128)", what, D);
-    CGT_ARG_CHECK(Tq < (1L << 29) && Tk < (1L << 29) && q_offset > -(1L << 29) && q_offset < (1L << 29), "%s: lengths and offset must be below 2^29", what);
+    CGT_ARG_CHECK(Tq < (1L << 29) && Tk < (1L << 29) && q_offset >= -kMaxOffset && q_offset <= kMaxOffset, "%s: lengths and offset must be below 2^29", what);
     CGT_ARG_CHECK(B < (1L << 22) && H < (1L << 22) && B * H < (1L << 22), "%s: too many heads", what);
     CGT_ARG_CHECK(layout == 0 || layout == 1, "%s: layout %d (0: heads before positions, 1: after them)", what, layout);
     CGT_ARG_CHECK(std::isfinite(scale), "%s: scale must be finite", what);
@@ -1439,27 +1447,16 @@ static int attn_setup(const char* what, Attn* a, long B, long H, long Tq, long T
     return CGT_AMD_OK;
 }
 
-}  // namespace cgt_amd
-
-using namespace cgt_amd;
-
-CGT_API int cgt_amd_rel_bucket(long rel, int buckets, int bidirectional, int max_distance) {
-    BucketRule r;
-    if (bucket_rule("rel_bucket", buckets, bidirectional, max_distance, &r)) return -1;
-    const long lim = 2L * kMaxDistance;
-    return bucket_of(r, (int)std::max(-lim, std::min(lim, rel)));
-}
-
-CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const float* v, const float* table, long B, long H, long Tq, long Tk, long D,
-                                          int layout, long buckets, int bidirectional, long max_distance, double scale, int causal, long q_offset,
-                                          const int* q_lengths, const int* k_lengths, double p, const long long* rng, unsigned channel,
-                                          float* o, float* lse, void* stream) {
+static int attention_fwd(const float* q, const float* k, const float* v, const float* table, long B, long H, long Tq, long Tk, long D, int layout,
+                         long buckets, int bidirectional, long max_distance, double scale, int causal, long q_offset, const int* q_offsets,
+                         const int* q_lengths, const int* k_lengths, double p, const long long* rng, unsigned channel, float* o, float* lse,
+                         void* stream) {
     Attn a = {};
     if (int rc = attn_setup("attention", &a, B, H, Tq, Tk, D, layout, table, buckets, bidirectional, max_distance, scale, causal, q_offset, p, rng, channel))
         return rc;
     if (B * H * Tq == 0) return CGT_AMD_OK;
     CGT_ARG_CHECK(q && o && lse && (Tk == 0 || (k && v)), "attention: null pointer");
-    a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths;
+    a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths, a.q_offsets = q_offsets;
     hipStream_t st = as_stream(stream);
     // Up to eight queries read k and v once, on the vector units; more go through the matrix cores, whose
     // scales take a walk over k and v of their own.  Both sides, vector / matrix: 16 heads of 16 sequences (64 columns)
@@ -1517,10 +1514,10 @@ CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const 
     return CGT_AMD_OK;
 }
 
-CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const float* v, const float* table, const float* o, const float* lse,
-                                          const float* go, long B, long H, long Tq, long Tk, long D, int layout, long buckets, int bidirectional,
-                                          long max_distance, double scale, int causal, long q_offset, const int* q_lengths, const int* k_lengths,
-                                          double p, const long long* rng, unsigned channel, float* gq, float* gk, float* gv, float* gtable, void* stream) {
+static int attention_bwd(const float* q, const float* k, const float* v, const float* table, const float* o, const float* lse, const float* go, long B,
+                         long H, long Tq, long Tk, long D, int layout, long buckets, int bidirectional, long max_distance, double scale, int causal,
+                         long q_offset, const int* q_offsets, const int* q_lengths, const int* k_lengths, double p, const long long* rng,
+                         unsigned channel, float* gq, float* gk, float* gv, float* gtable, void* stream) {
     Attn a = {};
     if (int rc = attn_setup("attention backward", &a, B, H, Tq, Tk, D, layout, table, buckets, bidirectional, max_distance, scale, causal, q_offset, p, rng,
                             channel))
@@ -1536,7 +1533,7 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
         return cgt_amd_fill_u32(gv, 0u, heads * Tk * D, stream);
     }
     CGT_ARG_CHECK(q && o && lse && go && gq && (Tk == 0 || (k && v && gk && gv)), "attention backward: null pointer");
-    a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths;
+    a.q = q, a.k = k, a.v = v, a.q_lengths = q_lengths, a.k_lengths = k_lengths, a.q_offsets = q_offsets;
     hipStream_t st = as_stream(stream);
     const int DP = padded_dim(a.D), qtiles = (int)cdiv(Tq, kAttnCols), ktiles = (int)cdiv(Tk, kAttnCols);
     const int runs = scale_runs(Tq, Tk);
@@ -1593,4 +1590,50 @@ CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const 
         }
     }
     return CGT_AMD_OK;
+}
+
+}  // namespace cgt_amd
+
+using namespace cgt_amd;
+
+CGT_API int cgt_amd_rel_bucket(long rel, int buckets, int bidirectional, int max_distance) {
+    BucketRule r;
+    if (bucket_rule("rel_bucket", buckets, bidirectional, max_distance, &r)) return -1;
+    const long lim = 2L * kMaxDistance;
+    return bucket_of(r, (int)std::max(-lim, std::min(lim, rel)));
+}
+
+CGT_API int cgt_amd_rel_attention_fwd_f32(const float* q, const float* k, const float* v, const float* table, long B, long H, long Tq, long Tk, long D,
+                                          int layout, long buckets, int bidirectional, long max_distance, double scale, int causal, long q_offset,
+                                          const int* q_lengths, const int* k_lengths, double p, const long long* rng, unsigned channel,
+                                          float* o, float* lse, void* stream) {
+    return attention_fwd(q, k, v, table, B, H, Tq, Tk, D, layout, buckets, bidirectional, max_distance, scale, causal, q_offset, nullptr, q_lengths, k_lengths,
+                         p, rng, channel, o, lse, stream);
+}
+
+CGT_API int cgt_amd_rel_attention_at_fwd_f32(const float* q, const float* k, const float* v, const float* table, long B, long H, long Tq, long Tk, long D,
+                                             int layout, long buckets, int bidirectional, long max_distance, double scale, int causal,
+                                             const int* q_offsets, const int* q_lengths, const int* k_lengths, double p, const long long* rng,
+                                             unsigned channel, float* o, float* lse, void* stream) {
+    CGT_ARG_CHECK(q_offsets || B == 0, "attention: null pointer (offsets)");
+    return attention_fwd(q, k, v, table, B, H, Tq, Tk, D, layout, buckets, bidirectional, max_distance, scale, causal, 0, q_offsets, q_lengths, k_lengths,
+                         p, rng, channel, o, lse, stream);
+}
+
+CGT_API int cgt_amd_rel_attention_bwd_f32(const float* q, const float* k, const float* v, const float* table, const float* o, const float* lse,
+                                          const float* go, long B, long H, long Tq, long Tk, long D, int layout, long buckets, int bidirectional,
+                                          long max_distance, double scale, int causal, long q_offset, const int* q_lengths, const int* k_lengths,
+                                          double p, const long long* rng, unsigned channel, float* gq, float* gk, float* gv, float* gtable, void* stream) {
+    return attention_bwd(q, k, v, table, o, lse, go, B, H, Tq, Tk, D, layout, buckets, bidirectional, max_distance, scale, causal, q_offset, nullptr, q_lengths,
+                         k_lengths, p, rng, channel, gq, gk, gv, gtable, stream);
+}
+
+CGT_API int cgt_amd_rel_attention_at_bwd_f32(const float* q, const float* k, const float* v, const float* table, const float* o, const float* lse,
+                                             const float* go, long B, long H, long Tq, long Tk, long D, int layout, long buckets, int bidirectional,
+                                             long max_distance, double scale, int causal, const int* q_offsets, const int* q_lengths,
+                                             const int* k_lengths, double p, const long long* rng, unsigned channel, float* gq, float* gk, float* gv,
+                                             float* gtable, void* stream) {
+    CGT_ARG_CHECK(q_offsets || B == 0, "attention backward: null pointer (offsets)");
+    return attention_bwd(q, k, v, table, o, lse, go, B, H, Tq, Tk, D, layout, buckets, bidirectional, max_distance, scale, causal, 0, q_offsets, q_lengths,
+                         k_lengths, p, rng, channel, gq, gk, gv, gtable, stream);
 }

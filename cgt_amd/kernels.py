@@ -306,7 +306,8 @@ def rel_bucket(rel, buckets, bidirectional, max_distance):
 
 
 def _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_offset, q_lengths, k_lengths, p, rng, channel, layout):
-    """Checks the operands both directions share; returns (leading dims B, H, Tq, Tk, D, and the C arguments behind them)."""
+    """Checks the operands both directions share; returns (leading dims B, H, Tq, Tk, D, and the C arguments behind them), the last of
+    them whether q_offset is an array."""
     _f32(q, k, v)
     if layout not in ("bhtd", "bthd"):
         raise ValueError("layout is 'bhtd' or 'bthd' (got %r)" % (layout,))
@@ -323,7 +324,8 @@ def _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_off
         if table.ndim != 2 or table.shape[1] != H:
             raise ValueError("the bias table %s must be [buckets, %d heads]" % (table.shape, H))
         buckets = table.shape[0]
-    for n, name in ((q_lengths, "q_lengths"), (k_lengths, "k_lengths")):
+    each = isinstance(q_offset, GpuArray)
+    for n, name in ((q_lengths, "q_lengths"), (k_lengths, "k_lengths"), (q_offset if each else None, "q_offset")):
         if n is not None and (n.dtype != np.int32 or n.shape != (B,)):
             raise ValueError("%s must be an int32 array of %d elements" % (name, B))
     if bidirectional is None:
@@ -332,7 +334,7 @@ def _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_off
         scale = D ** -0.5 if D else 1.0
     ptr = lambda x: None if x is None else x.ptr      # noqa: E731
     return (B, H, Tq, Tk, D, int(layout == "bthd"), buckets, int(bool(bidirectional)), int(max_distance), float(scale),
-            int(bool(causal)), int(q_offset), ptr(q_lengths), ptr(k_lengths), float(p), _rng(rng, p), _channel(channel))
+            int(bool(causal)), q_offset.ptr if each else int(q_offset), ptr(q_lengths), ptr(k_lengths), float(p), _rng(rng, p), _channel(channel)), each
 
 
 def rel_attention_fwd(q, k, v, table=None, scale=None, causal=False, bidirectional=None, max_distance=128, q_offset=0,
@@ -340,10 +342,12 @@ def rel_attention_fwd(q, k, v, table=None, scale=None, causal=False, bidirection
     """softmax(scale * q k^T + table[bucket(key - query position)]) v per batch item and head, with dropout of the
     softmax's values: returns (o, lse).  q [B,H,Tq,D] and k, v [B,H,Tk,D] (layout "bthd": [B,T,H,D]); table
     [buckets, H] or None.  scale is D^-1/2 and bidirectional is `not causal` unless given; include/cgt_amd.h states
-    the rule of the buckets, of the lengths and of the generator."""
-    args = _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_offset, q_lengths, k_lengths, p, rng, channel, layout)
+    the rule of the buckets, of the lengths and of the generator.  q_offset, the position of the first query among the
+    keys, is a number or an int32 device array with one for each sequence."""
+    args, each = _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_offset, q_lengths, k_lengths, p, rng, channel, layout)
     o, lse = (_out(a, s) for a, s in zip(out or (None, None), (q.shape, args[:3])))
-    capi.check(capi.lib().cgt_amd_rel_attention_fwd_f32(q.ptr, k.ptr, v.ptr, None if table is None else table.ptr, *args, o.ptr, lse.ptr, stream))
+    call = capi.lib().cgt_amd_rel_attention_at_fwd_f32 if each else capi.lib().cgt_amd_rel_attention_fwd_f32
+    capi.check(call(q.ptr, k.ptr, v.ptr, None if table is None else table.ptr, *args, o.ptr, lse.ptr, stream))
     return o, lse
 
 
@@ -351,14 +355,15 @@ def rel_attention_bwd(q, k, v, table, o, lse, go, scale=None, causal=False, bidi
                       q_lengths=None, k_lengths=None, p=0.0, rng=None, channel=0, layout="bhtd", out=None, stream=None):
     """The gradients of rel_attention_fwd from the cotangent of o, given its results: returns (gq, gk, gv, gtable),
     gtable None without a table."""
-    args = _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_offset, q_lengths, k_lengths, p, rng, channel, layout)
+    args, each = _attention(q, k, v, table, scale, causal, bidirectional, max_distance, q_offset, q_lengths, k_lengths, p, rng, channel, layout)
     _f32(o, lse, go)
     if o.shape != q.shape or go.shape != q.shape or lse.shape != args[:3]:
         raise ValueError("results %s, %s and cotangent %s do not fit q %s" % (o.shape, lse.shape, go.shape, q.shape))
     shapes = [q.shape, k.shape, v.shape] + ([table.shape] if table is not None else [])
     outs = [_out(a, s) for a, s in zip(out or (None,) * 4, shapes)]
     gtable = outs[3] if table is not None else None
-    capi.check(capi.lib().cgt_amd_rel_attention_bwd_f32(
+    call = capi.lib().cgt_amd_rel_attention_at_bwd_f32 if each else capi.lib().cgt_amd_rel_attention_bwd_f32
+    capi.check(call(
         q.ptr, k.ptr, v.ptr, None if table is None else table.ptr, o.ptr, lse.ptr, go.ptr, *args, outs[0].ptr, outs[1].ptr, outs[2].ptr,
         None if gtable is None else gtable.ptr, stream))
     return outs[0], outs[1], outs[2], gtable

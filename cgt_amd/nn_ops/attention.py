@@ -6,11 +6,14 @@ BatchedMul22 over an array of scores that these never store.
 import ctypes
 from collections import namedtuple
 
+import numpy as np
+
 from .. import core
 from .dropout import check_rng, resolved, rng_node
 
 AttentionInfo = namedtuple("AttentionInfo", ["scale", "causal", "bidirectional", "max_distance", "q_offset", "p", "channel", "layout",
-                                             "has_table", "has_q_lengths", "has_k_lengths"])
+                                             "has_table", "has_q_lengths", "has_k_lengths", "has_q_offsets"])
+AttentionInfo.__new__.__defaults__ = (0,)
 
 
 def make_closure(info):
@@ -26,25 +29,35 @@ def make_closure(info):
         ("has_table", ctypes.c_int, info.has_table),
         ("has_q_lengths", ctypes.c_int, info.has_q_lengths),
         ("has_k_lengths", ctypes.c_int, info.has_k_lengths),
+        ("has_q_offsets", ctypes.c_int, info.has_q_offsets),
     ]
 
 
-# the operands both directions start with: q, k, v, then those of table, q_lengths, k_lengths, rng that exist
+# the operands both directions start with: q, k, v, then those of table, q_lengths, k_lengths, q_offsets, rng that exist
 _OPERANDS = r"""
                 cgtArray *q = reads[0], *k = reads[1], *v = reads[2];
                 int at = 3;
                 cgtArray *table = cl->has_table ? reads[at++] : NULL, *qn = cl->has_q_lengths ? reads[at++] : NULL;
-                cgtArray *kn = cl->has_k_lengths ? reads[at++] : NULL, *rng = cl->p > 0 ? reads[at++] : NULL;
+                cgtArray *kn = cl->has_k_lengths ? reads[at++] : NULL, *qo = cl->has_q_offsets ? reads[at++] : NULL;
+                cgtArray *rng = cl->p > 0 ? reads[at++] : NULL;
                 const int t = cl->layout ? 1 : 2;
                 const long B = q->shape()[0], H = q->shape()[3 - t], Tq = q->shape()[t], D = q->shape()[3], Tk = k->shape()[t];
                 cgt_check(k->size() == B * H * Tk * D && k->shape()[3 - t] == H && k->shape()[3] == D && v->size() == k->size() &&
                           (!table || (table->ndim() == 2 && table->shape()[1] == H)) && (!qn || (qn->size() == B && qn->dtype() == cgt_i4)) &&
-                          (!kn || (kn->size() == B && kn->dtype() == cgt_i4)) && (!rng || rng->size() == 2),
+                          (!kn || (kn->size() == B && kn->dtype() == cgt_i4)) && (!qo || (qo->size() == B && qo->dtype() == cgt_i4)) &&
+                          (!rng || rng->size() == 2),
                           "RelativeAttention: operands do not fit each other");
 """
-_ARGUMENTS = r"""B, H, Tq, Tk, D, cl->layout, table ? table->shape()[0] : 0,
-                    cl->bidirectional, cl->max_distance, cl->scale, cl->causal, cl->q_offset, qn ? (const int*)qn->data() : NULL,
-                    kn ? (const int*)kn->data() : NULL, cl->p, rng ? (const long long*)rng->data() : NULL, (unsigned)cl->channel"""
+
+def _call(name, before, after):
+    """The call of one of the two forms of an entry point: one position for all sequences, or an array of them."""
+    both = []
+    for form, position in (("_at", "(const int*)qo->data()"), ("", "cl->q_offset")):
+        both.append("cgt_amd_rel_attention" + form + "_" + name + "_f32(" + before + r""", B, H, Tq, Tk, D, cl->layout, table ? table->shape()[0] : 0,
+                    cl->bidirectional, cl->max_distance, cl->scale, cl->causal, """ + position + r""", qn ? (const int*)qn->data() : NULL,
+                    kn ? (const int*)kn->data() : NULL, cl->p, rng ? (const long long*)rng->data() : NULL, (unsigned)cl->channel,
+                    """ + after + ", cgt_get_stream())")
+    return "qo ? " + both[0] + "\n                  : " + both[1]
 
 
 def _check_types(info, types):
@@ -52,9 +65,9 @@ def _check_types(info, types):
     rest = list(types[3:])
     if info.has_table:
         assert rest.pop(0) == core.TensorType("f4", 2), "RelativeAttention: the bias table is a float32 matrix [buckets, heads]"
-    for has in (info.has_q_lengths, info.has_k_lengths):
+    for has in (info.has_q_lengths, info.has_k_lengths, info.has_q_offsets):
         if has:
-            assert rest.pop(0) == core.TensorType("i4", 1), "RelativeAttention: lengths are int32 arrays of one axis"
+            assert rest.pop(0) == core.TensorType("i4", 1), "RelativeAttention: lengths and offsets are int32 arrays of one axis"
     if info.p:
         check_rng(rest.pop(0))
 
@@ -67,13 +80,13 @@ def _check_shapes(info, inputs):
     rest = list(inputs[3:])
     if info.has_table and core.shape(rest.pop(0))[1] != q[3 - t]:
         raise ValueError("RelativeAttention: the bias table must have a column for each of the %d heads" % q[3 - t])
-    for has in (info.has_q_lengths, info.has_k_lengths):
+    for has in (info.has_q_lengths, info.has_k_lengths, info.has_q_offsets):
         if has and core.shape(rest.pop(0)) != q[:1]:
-            raise ValueError("RelativeAttention: one length for each of the %d sequences" % q[0])
+            raise ValueError("RelativeAttention: one length or offset for each of the %d sequences" % q[0])
 
 
 class RelativeAttention(core.Op):
-    """inputs [q, k, v] (+ [table]) (+ [q_lengths]) (+ [k_lengths]) (+ [rng] when p > 0) -> (o, lse)."""
+    """inputs [q, k, v] (+ [table]) (+ [q_lengths]) (+ [k_lengths]) (+ [q_offsets]) (+ [rng] when p > 0) -> (o, lse)."""
     available_impls = ("native_gpu",)
 
     def __init__(self, info):
@@ -109,9 +122,8 @@ class RelativeAttention(core.Op):
                 cgtArray *o = (cgtArray*)write->getitem(0), *lse = (cgtArray*)write->getitem(1);
                 cgt_check(o->size() == q->size() && lse->size() == B * H * Tq, "RelativeAttention: outputs do not fit the input");
                 if (cgtGlobalStatus != cgtStatusOK) return;
-                int rc = cgt_amd_rel_attention_fwd_f32((const float*)q->data(), (const float*)k->data(), (const float*)v->data(),
-                    table ? (const float*)table->data() : NULL, """ + _ARGUMENTS + r""",
-                    (float*)o->data(), (float*)lse->data(), cgt_get_stream());
+                int rc = """ + _call("fwd", "(const float*)q->data(), (const float*)k->data(), (const float*)v->data(), "
+                                     "table ? (const float*)table->data() : NULL", "(float*)o->data(), (float*)lse->data()") + r""";
                 cgt_check(rc == CGT_AMD_OK, "RelativeAttention: %s", cgt_amd_last_error());
             }"""
         return core.NativeCompileInfo(code, includes=["cgt_amd.h"], closure_triples=make_closure(self.info),
@@ -147,10 +159,9 @@ class RelativeAttentionBackward(core.Op):
                           gk->size() == k->size() && gv->size() == k->size() && (!gtable || gtable->size() == table->size()),
                           "RelativeAttentionBackward: operands do not fit the input");
                 if (cgtGlobalStatus != cgtStatusOK) return;
-                int rc = cgt_amd_rel_attention_bwd_f32((const float*)q->data(), (const float*)k->data(), (const float*)v->data(),
-                    table ? (const float*)table->data() : NULL, (const float*)o->data(), (const float*)lse->data(), (const float*)go->data(),
-                    """ + _ARGUMENTS + r""",
-                    (float*)gq->data(), (float*)gk->data(), (float*)gv->data(), gtable ? (float*)gtable->data() : NULL, cgt_get_stream());
+                int rc = """ + _call("bwd", "(const float*)q->data(), (const float*)k->data(), (const float*)v->data(), "
+                                     "table ? (const float*)table->data() : NULL, (const float*)o->data(), (const float*)lse->data(), (const float*)go->data()",
+                                     "(float*)gq->data(), (float*)gk->data(), (float*)gv->data(), gtable ? (float*)gtable->data() : NULL") + r""";
                 cgt_check(rc == CGT_AMD_OK, "RelativeAttentionBackward: %s", cgt_amd_last_error());
             }"""
         return core.NativeCompileInfo(code, includes=["cgt_amd.h"], closure_triples=make_closure(self.info),
@@ -158,12 +169,12 @@ class RelativeAttentionBackward(core.Op):
 
 
 def _lengths_node(lengths):
+    """int32 [B] on the device: the sequences' lengths or offsets."""
     if isinstance(lengths, core.Node) or isinstance(lengths, core.GpuArray):
         return core.as_node(lengths)
-    import numpy as np
     lengths = np.asarray(lengths)
     if lengths.dtype.kind not in "iu":
-        raise TypeError("lengths are whole numbers, got %s" % lengths.dtype)
+        raise TypeError("lengths and offsets are whole numbers, got %s" % lengths.dtype)
     return core.as_node(core.to_gpu(lengths.astype(np.int32)))
 
 
@@ -172,7 +183,10 @@ def relative_attention(q, k, v, table=None, scale=None, causal=False, bidirectio
     """softmax(scale * q k^T + table[bucket(key - query position)]) v per sequence and head.
 
     q [B,H,Tq,D], k and v [B,H,Tk,D] (layout "bthd": [B,T,H,D], as a projection leaves them), table [buckets, H].
-    scale is D^-1/2 and bidirectional `not causal` unless given.  Lengths (int32 [B]) describe a padded batch;
+    scale is D^-1/2 and bidirectional `not causal` unless given.  Lengths (int32 [B]) describe a padded batch.
+    q_offset is the position of the first query among the keys: a number, or int32 [B] with one for each sequence
+    (q_offset = k_lengths - Tq for new tokens at the ends of sequences of different lengths).  Lengths and such offsets are inputs of the op:
+    a compiled function that takes them as arguments steps through a cache of fixed size.
     p, rng and channel drop values of the softmax as nn.dropout would."""
     q, k, v = (core.as_node(x) for x in (q, k, v))
     if layout not in ("bhtd", "bthd"):
@@ -182,9 +196,10 @@ def relative_attention(q, k, v, table=None, scale=None, causal=False, bidirectio
     p = resolved(p)
     if not 0 <= int(channel) < 1 << 32:
         raise ValueError("channel must be a whole number of 32 bits (got %s)" % (channel,))
+    each = not isinstance(q_offset, (int, np.integer))
     info = AttentionInfo(float(int(q.shape[3]) ** -0.5 if scale is None else scale), int(bool(causal)),
-                         int(bool(not causal if bidirectional is None else bidirectional)), int(max_distance), int(q_offset), p, int(channel),
-                         int(layout == "bthd"), int(table is not None), int(q_lengths is not None), int(k_lengths is not None))
+                         int(bool(not causal if bidirectional is None else bidirectional)), int(max_distance), 0 if each else int(q_offset), p, int(channel),
+                         int(layout == "bthd"), int(table is not None), int(q_lengths is not None), int(k_lengths is not None), int(each))
     inputs = [q, k, v] + ([core.as_node(table)] if table is not None else [])
-    inputs += [_lengths_node(n) for n in (q_lengths, k_lengths) if n is not None] + ([rng_node(rng)] if p else [])
+    inputs += [_lengths_node(n) for n in (q_lengths, k_lengths, q_offset if each else None) if n is not None] + ([rng_node(rng)] if p else [])
     return core.Result(RelativeAttention(info), inputs)[0]

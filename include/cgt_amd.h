@@ -348,8 +348,10 @@ int cgt_amd_dropout_add_layer_norm_bwd_f32(const float *h, const float *gamma, c
  *   s[i][j] = scale * q[i] . k[j] + table[bucket(j - i - q_offset)][head]
  *   o[i] = sum_j softmax_j(s[i])[j] * v[j],  lse[i] = log sum_j exp(s[i][j])
  * over the keys j that query i may see: j < k_lengths[b] and, if causal,
- * j <= i + q_offset (q_offset is the position of the first query among the
- * keys: Tk - Tq where new tokens meet a cache).  The scores are never stored.
+ * j <= i + q_offset.  q_offset is the position of the first query among the
+ * keys: Tk - Tq where new tokens meet a cache that they end, and a number of each
+ * sequence's own (the _at_ calls) where the sequences of a batch are at different
+ * positions or step through a cache of fixed size.  The scores are never stored.
  *
  * q, o are [B][H][Tq][D] (layout 0) or [B][Tq][H][D] (layout 1), k, v the same
  * with Tk, fp32; lse is [B][H][Tq].  1 <= D <= 128; lengths and |q_offset|
@@ -410,6 +412,25 @@ int cgt_amd_rel_attention_bwd_f32(const float *q, const float *k, const float *v
                                   const int *q_lengths, const int *k_lengths, double p,
                                   const long long *rng, unsigned channel, float *gq, float *gk, float *gv,
                                   float *gtable, void *stream);
+
+/* The same with q_offsets, int32 [B] on the device (clamped to below 2^29 in
+ * magnitude) in place of q_offset: the position of each sequence's first query among
+ * its own keys.  Kernels read it when they run, as they read the lengths and rng,
+ * so a replayed graph takes the positions that are in it then.  New tokens of
+ * sequences with n[b] keys (their own included): k_lengths = n, q_offsets = n - Tq. */
+int cgt_amd_rel_attention_at_fwd_f32(const float *q, const float *k, const float *v, const float *table,
+                                     long B, long H, long Tq, long Tk, long D, int layout, long buckets,
+                                     int bidirectional, long max_distance, double scale, int causal,
+                                     const int *q_offsets, const int *q_lengths, const int *k_lengths,
+                                     double p, const long long *rng, unsigned channel, float *o, float *lse,
+                                     void *stream);
+int cgt_amd_rel_attention_at_bwd_f32(const float *q, const float *k, const float *v, const float *table,
+                                     const float *o, const float *lse, const float *go, long B, long H,
+                                     long Tq, long Tk, long D, int layout, long buckets, int bidirectional,
+                                     long max_distance, double scale, int causal, const int *q_offsets,
+                                     const int *q_lengths, const int *k_lengths, double p,
+                                     const long long *rng, unsigned channel, float *gq, float *gk, float *gv,
+                                     float *gtable, void *stream);
 
 /* ---------------------------------------------------------------- GEMM */
 

@@ -87,6 +87,94 @@ def test_rows_whose_lse_has_no_digits_contribute_to_no_gradient(K, value):
         close(a.get()[:, 0], want[:, 0], tol[name][:, 0], name)
 
 
+# ---------------------------------------------------------------- sequences at positions of their own
+
+def by_sequence(c, arrays, offsets, go=None, keep=None):
+    """Each sequence by itself in float64: (o, lse, tolerances of both, gradients, their tolerances)."""
+    q, k, v, table = arrays
+    parts = []
+    for b, off in enumerate(offsets):
+        more = {n: c[n] for n in ("causal", "bidirectional", "max_distance", "scale") if n in c}
+        for n in ("q_lengths", "k_lengths"):
+            if n in c:
+                more[n] = c[n][b:b + 1]
+        att = T.Attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], table, q_offset=int(off), keep=None if keep is None else keep[b:b + 1], **more)
+        tol = tolerances(att, None if go is None else go[b:b + 1])
+        parts.append((att.o, att.lse, tol["o"], tol["lse"]) + (() if go is None else att.pullback(go[b:b + 1])[:3 + (table is not None)]
+                                                               + tuple(tol[n] for n in ("gq", "gk", "gv", "gtable")[:3 + (table is not None)])))
+    n = 4 + (0 if go is None else 2 * (3 + (table is not None)))
+    out = [np.concatenate([p[i] for p in parts]) if not (go is not None and table is not None and i in (7, 11)) else sum(p[i] for p in parts)
+           for i in range(n)]
+    return out
+
+
+OFFSETS = [
+    (case(4, 2, 1, 500, 64, buckets=32, causal=True, k_lengths=[500, 1, 133, 0]), None),                 # one token each, sequences of different lengths
+    (case(3, 2, 5, 1300, 40, buckets=16, causal=True, k_lengths=[1300, 700, 6]), None),
+    (case(3, 2, 40, 700, 64, buckets=32, causal=True, k_lengths=[700, 333, 40], layout="bthd"), None),      # chunks of a prompt
+    (case(2, 2, 150, 400, 128, buckets=32, causal=True, k_lengths=[400, 151], q_lengths=[150, 100]), None),
+    (case(3, 1, 33, 90, 32, buckets=8, max_distance=9, p=0.2), [0, 57, -1000]),                            # positions without a mask
+    (case(2, 2, 20, 60, 24, causal=True), [-5, 2 ** 31 - 1]),                                              # no bias; clamped
+]
+
+
+@pytest.mark.parametrize("c,offsets", OFFSETS, ids=["%dx%dx%dx%d" % (c["B"], c["H"], c["Tq"], c["Tk"]) for c, _ in OFFSETS])
+def test_a_position_for_each_sequence(K, c, offsets):
+    offsets = [n - c["Tq"] for n in c["k_lengths"]] if offsets is None else offsets
+    (q, k, v, table, go), _ = make(dict(c, q_offset=0))
+    keep = T.attention_keep(c["B"], c["H"], c["Tq"], c["Tk"], c["p"], 31337, 2) if c.get("p") else None
+    want = by_sequence(c, (q, k, v, table), np.clip(offsets, -2 ** 20, 2 ** 20), go, keep)
+    more = dict(arguments(c), q_offset=dev(np.array(offsets), np.int32))
+    dt = None if table is None else dev(table)
+    ins = [place(a, c) for a in (q, k, v)]
+    o, lse = K.rel_attention_fwd(*ins, dt, **more)
+    close(fetch(o, c), want[0], want[2], "o")
+    close(lse.get(), want[1], want[3], "lse")
+    got = K.rel_attention_bwd(*ins, dt, o, lse, place(go, c), **more)
+    n = 3 + (table is not None)
+    for name, a, w, t in zip(("gq", "gk", "gv", "gtable"), got, want[4:4 + n], want[4 + n:]):
+        close(a.get() if name == "gtable" else fetch(a, c), w, t, name)
+    # one number for all is the same as an array of it
+    if len(set(offsets)) == 1 or c["Tk"] == 700:
+        off = c["Tk"] - c["Tq"]
+        more = arguments(c)
+        a = K.rel_attention_fwd(*ins, dt, **dict(more, q_offset=off))
+        b = K.rel_attention_fwd(*ins, dt, **dict(more, q_offset=dev(np.full(c["B"], off), np.int32)))
+        assert all(np.array_equal(x.get(), y.get()) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_one_compiled_function_steps_through_a_cache(K, use_graph):
+    # a new token of each sequence a step; lengths and positions are arguments
+    import cgt_amd as cgt
+    from cgt_amd import nn
+    rs = np.random.RandomState(21)
+    B, H, room, D = 3, 2, 300, 32
+    c = case(B, H, 1, room, D, causal=True)
+    k, v = (rs.randn(B, H, room, D).astype(np.float32) for _ in range(2))
+    table = rs.randn(16, H).astype(np.float32)
+    nq, nk, nv, lengths, offsets = (cgt.constant(a) for a in (rs.randn(B, H, 1, D).astype(np.float32), k, v, dev(np.ones(B), np.int32), dev(np.zeros(B), np.int32)))
+    o = nn.relative_attention(nq, nk, nv, cgt.constant(table), causal=True, q_offset=offsets, k_lengths=lengths)
+    f = cgt.function([nq, nk, nv, lengths, offsets], [o], use_graph=use_graph)
+    for step in range(4):
+        n = np.array([40 + step, 1 + step, 297 + step], np.int32)
+        q = rs.randn(B, H, 1, D).astype(np.float32)
+        want = by_sequence(dict(c, k_lengths=list(n)), (q, k, v, table), n - 1)
+        close(f(q, k, v, n, (n - 1).astype(np.int32))[0], want[0], want[2], "step %d" % step)
+    # gradients through the op with such an input
+    go = rs.randn(B, H, 1, D).astype(np.float32)
+    off = [7, 0, 299]
+    o = nn.relative_attention(nq, nk, nv, table, causal=True, q_offset=off)
+    grads = cgt.grad(o, [nq, nk, nv], goutput=go)
+    want = by_sequence(c, (nq.get(), k, v, table), off, go)
+    for name, g, w, t in zip(("gq", "gk", "gv"), grads, want[4:7], want[8:11]):
+        close(g.get(), w, t, name)
+    with pytest.raises(ValueError):
+        nn.relative_attention(nq, nk, nv, q_offset=[1, 2])
+    with pytest.raises(TypeError):
+        nn.relative_attention(nq, nk, nv, q_offset=np.zeros(B, np.float32))
+
+
 # ---------------------------------------------------------------- rows of very different size within one head
 
 def plain32(q, k, v, table, go, causal=False, max_distance=128, bidirectional=None, keep=1.0):
