@@ -1451,6 +1451,7 @@ static int attention_fwd(const float* q, const float* k, const float* v, const f
                          long buckets, int bidirectional, long max_distance, double scale, int causal, long q_offset, const int* q_offsets,
                          const int* q_lengths, const int* k_lengths, double p, const long long* rng, unsigned channel, float* o, float* lse,
                          void* stream) {
+    const StreamTurn turn(stream);
     Attn a = {};
     if (int rc = attn_setup("attention", &a, B, H, Tq, Tk, D, layout, table, buckets, bidirectional, max_distance, scale, causal, q_offset, p, rng, channel))
         return rc;
@@ -1518,6 +1519,7 @@ static int attention_bwd(const float* q, const float* k, const float* v, const f
                          long H, long Tq, long Tk, long D, int layout, long buckets, int bidirectional, long max_distance, double scale, int causal,
                          long q_offset, const int* q_offsets, const int* q_lengths, const int* k_lengths, double p, const long long* rng,
                          unsigned channel, float* gq, float* gk, float* gv, float* gtable, void* stream) {
+    const StreamTurn turn(stream);
     Attn a = {};
     if (int rc = attn_setup("attention backward", &a, B, H, Tq, Tk, D, layout, table, buckets, bidirectional, max_distance, scale, causal, q_offset, p, rng,
                             channel))

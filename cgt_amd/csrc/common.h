@@ -27,6 +27,20 @@ enum WorkspaceUser { kWsGemm = 0, kWsSum = 1, kWsConvFilter = 2, kWsConvTable = 
 float* stream_workspace(void* stream, WorkspaceUser user, size_t bytes, const char* what);
 void release_stream_workspaces(void* stream);
 
+// A call that hands data from one of its kernels to the next through a workspace has the stream's launches for itself
+// from the lookup of the workspace to its last launch: two host threads that share a stream take turns, call
+// by call.  (Launching is asynchronous, so a turn is short; a thread may take it again inside its own.)
+class StreamTurn {
+public:
+    explicit StreamTurn(void* stream);
+    ~StreamTurn();
+    StreamTurn(const StreamTurn&) = delete;
+    StreamTurn& operator=(const StreamTurn&) = delete;
+
+private:
+    void* mutex_;
+};
+
 // The GEMMs of a convolution layer with the layer's layouts built in (gemm.hip).
 // Over an operand read straight from a zero-padded image -- stride 1, pad = (kernel - 1) / 2,
 // no column buffer:

@@ -274,6 +274,7 @@ static bool small_wgrad_plan(SmallWgrad& a, size_t& lds_bytes, int& grid, long B
 }
 
 static int small_wgrad(const SmallWgrad& plan, size_t lds_bytes, int grid, const float* gy, const float* x, float* gf, void* stream) {
+    const StreamTurn turn(stream);
     SmallWgrad a = plan;
     a.gy = gy; a.x = x;
     // 16-byte loads of the cotangent: pixel runs that start and end on 16-byte boundaries in every unit
@@ -412,6 +413,7 @@ CGT_API int cgt_amd_conv_same_wgrad_f32(const float* gypad, const float* xpad, l
 CGT_API int cgt_amd_conv_same_fwd_f32(const float* xpad, const float* f, const float* bias, int relu, long B, long C,
                                       long H, long W, long L, int kh, int kw, float* y, signed char* mask,
                                       void* stream) {
+    const StreamTurn turn(stream);
     SameGeom g;
     int rc = check_same("conv_same_fwd", g, B, C, H, W, L, kh, kw);
     if (rc) return rc;
@@ -427,6 +429,7 @@ CGT_API int cgt_amd_conv_same_fwd_f32(const float* xpad, const float* f, const f
 
 CGT_API int cgt_amd_conv_same_bwd_data_f32(const float* gypad, const float* f, long B, long C, long H, long W, long L,
                                            int kh, int kw, float* gx, void* stream) {
+    const StreamTurn turn(stream);
     SameGeom g;
     int rc = check_same("conv_same_bwd_data", g, B, C, H, W, L, kh, kw);
     if (rc) return rc;
@@ -463,6 +466,7 @@ CGT_API int cgt_amd_conv_same_bwd_filter_f32(const float* gypad, const float* xp
 // workspace and the groups are summed in order: any batch size, fixed order of additions.
 template <class F>
 static int wgrad_in_groups(long B, long P, long Z, long L, float* gf, void* stream, const char* what, F&& product) {
+    const StreamTurn turn(stream);
     CGT_ARG_CHECK(P < (1L << 31) - 128, "%s: too many output pixels per image", what);
     const long per_image = L * Z;
     long group = std::max(1L, (64L << 20) / per_image);                 // 256 MiB of partial sums

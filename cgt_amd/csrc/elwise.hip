@@ -520,6 +520,7 @@ CGT_API int cgt_amd_repeat(const void* x, int itemsize, int ndim, const long* ou
 
 CGT_API int cgt_amd_sum_f32(const float* x, int ndim, const long* shape, const int* reduced, float* out,
                             void* stream) {
+    const StreamTurn turn(stream);
     CGT_ARG_CHECK(ndim >= 0 && ndim <= 8, "sum: ndim %d out of range (0..8)", ndim);
     CGT_ARG_CHECK(ndim == 0 || (shape && reduced), "sum: null shape");
     long nin = 1, nout = 1;

@@ -1376,6 +1376,7 @@ static void launch_trans(int tA, int tB, bool pipe, bool deep, int shape, dim3 g
 static int gemm_dispatch(int tA, int tB, long P, long M, long N, long K, const float* A, long lda,
                          long sA, const float* B, long ldb, long sB, float* C, long ldc, long sC,
                          void* stream, bool static_scratch = false, const ConvGemm* cv = nullptr) {
+    const StreamTurn turn(stream);
     CGT_ARG_CHECK(P >= 0 && M >= 0 && N >= 0 && K >= 0, "sgemm: negative size");
     if (P == 0 || M == 0 || N == 0) return CGT_AMD_OK;
     CGT_ARG_CHECK(A || K == 0, "sgemm: null A");

@@ -580,6 +580,7 @@ static int launch_norm_fwd(NormFwd a, hipStream_t st) {
 
 template <bool ADD, bool DROP, int N>
 static int launch_norm_bwd(NormBwd a, float* ggamma, float* gbeta, void* stream) {
+    const StreamTurn turn(stream);
     hipStream_t st = as_stream(stream);
     const int pieces = (int)cdiv(a.cols, N);
     const bool wave_rows = a.cols <= 1024, wide = a.cols > 8192;

@@ -2,6 +2,7 @@
 // events, error reporting.
 #include "common.h"
 #include <algorithm>
+#include <cstdint>
 #include <cstring>
 #include <mutex>
 #include <unordered_map>
@@ -29,6 +30,17 @@ struct StreamWorkspaces {
 };
 static std::mutex g_ws_mutex;
 static std::unordered_map<void*, StreamWorkspaces> g_ws;
+
+// Streams share a few mutexes by address: a stream's never goes away, and calls on two streams that meet in one
+// merely wait for each other's launches.
+static std::recursive_mutex g_turns[64];
+StreamTurn::StreamTurn(void* stream) {
+    const size_t at = reinterpret_cast<uintptr_t>(stream);
+    std::recursive_mutex* m = &g_turns[(at >> 4 ^ at >> 10 ^ at >> 16) % 64];
+    m->lock();
+    mutex_ = m;
+}
+StreamTurn::~StreamTurn() { static_cast<std::recursive_mutex*>(mutex_)->unlock(); }
 
 float* stream_workspace(void* stream, WorkspaceUser user, size_t bytes, const char* what) {
     std::lock_guard<std::mutex> lock(g_ws_mutex);

@@ -12,7 +12,8 @@
  *   - every data pointer is DEVICE memory, fp32 contiguous row-major unless
  *     noted; argmax masks are int32; sizes are `long` as in cgtArray::shape().
  *   - `stream` is a hipStream_t passed as void*; NULL is the default stream.
- *     Launches are asynchronous; nothing here synchronises.
+ *     Launches are asynchronous; nothing here synchronises.  Calls may come
+ *     from several threads, on one stream too: those take turns call by call.
  *   - return value: CGT_AMD_OK or an error code; cgt_amd_last_error() gives
  *     the message for the calling thread.  (The reference's CUDA_CHECK only
  *     prints, include/cgt_cuda.h:11-21; a status is returned here instead.)
