@@ -19,8 +19,8 @@ inline hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
 // (stream, user), grown on demand and geometrically (at least 1.5 x the block that is
 // outgrown).  An outgrown block is not freed on the spot -- kernels in flight may still
 // use it and hipFree would stall the stream -- it is retired: released at the stream's
-// next cgt_amd_synchronize, or, if it was current when a capture began on the stream (a
-// HIP graph may have its address baked in), with the stream (cgt_amd_stream_destroy).
+// next cgt_amd_synchronize, or, if it was current when a capture began on the stream or used inside one
+// (a HIP graph may have its address baked in), with the stream (cgt_amd_stream_destroy).
 // Growth while the stream is being captured is refused (an allocation would break the
 // capture): returns nullptr with the message set.
 enum WorkspaceUser { kWsGemm = 0, kWsSum = 1, kWsConvFilter = 2, kWsConvTable = 3, kWsConvData = 4, kWsNorm = 5, kWsAttention = 6, kWsUsers = 7 };

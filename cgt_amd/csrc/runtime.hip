@@ -45,10 +45,15 @@ StreamTurn::~StreamTurn() { static_cast<std::recursive_mutex*>(mutex_)->unlock()
 float* stream_workspace(void* stream, WorkspaceUser user, size_t bytes, const char* what) {
     std::lock_guard<std::mutex> lock(g_ws_mutex);
     StreamWorkspaces& w = g_ws[stream];
-    if (w.bytes[user] >= bytes) return w.ptr[user];
+    // Captures that another library began are not announced: what is handed out inside one stays with the stream too.
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(as_stream(stream), &cap) != hipSuccess) (void)hipGetLastError();
-    if (cap != hipStreamCaptureStatusNone) {
+    if (stream && hipStreamIsCapturing(as_stream(stream), &cap) != hipSuccess) (void)hipGetLastError();
+    const bool capturing = cap != hipStreamCaptureStatusNone;
+    if (w.bytes[user] >= bytes) {
+        if (capturing && w.ptr[user]) w.in_graph[user] = true;
+        return w.ptr[user];
+    }
+    if (capturing) {
         set_error("%s: the workspace would have to grow to %zu bytes while the stream is being captured; "
                   "run the sequence once on this stream before capturing it", what, bytes);
         return nullptr;
