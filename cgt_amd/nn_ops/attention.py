@@ -12,8 +12,9 @@ from .. import core
 from .dropout import check_rng, resolved, rng_node
 
 AttentionInfo = namedtuple("AttentionInfo", ["scale", "causal", "bidirectional", "max_distance", "q_offset", "p", "channel", "layout",
-                                             "has_table", "has_q_lengths", "has_k_lengths", "has_q_offsets"])
-AttentionInfo.__new__.__defaults__ = (0,)
+                                             "has_table", "has_q_lengths", "has_k_lengths", "has_q_offsets",
+                                             "scale_by_width"])
+AttentionInfo.__new__.__defaults__ = (0, 0)
 
 
 def make_closure(info):
@@ -30,6 +31,7 @@ def make_closure(info):
         ("has_q_lengths", ctypes.c_int, info.has_q_lengths),
         ("has_k_lengths", ctypes.c_int, info.has_k_lengths),
         ("has_q_offsets", ctypes.c_int, info.has_q_offsets),
+        ("scale_by_width", ctypes.c_int, info.scale_by_width),
     ]
 
 
@@ -41,6 +43,8 @@ _OPERANDS = r"""
                 cgtArray *kn = cl->has_k_lengths ? reads[at++] : NULL, *qo = cl->has_q_offsets ? reads[at++] : NULL;
                 cgtArray *rng = cl->p > 0 ? reads[at++] : NULL;
                 const int t = cl->layout ? 1 : 2;
+                // D^-1/2 of the arrays at hand: a compiled function serves any head width
+                const double scale = cl->scale_by_width && q->shape()[3] ? 1.0 / sqrt((double)q->shape()[3]) : cl->scale;
                 const long B = q->shape()[0], H = q->shape()[3 - t], Tq = q->shape()[t], D = q->shape()[3], Tk = k->shape()[t];
                 cgt_check(k->size() == B * H * Tk * D && k->shape()[3 - t] == H && k->shape()[3] == D && v->size() == k->size() &&
                           (!table || (table->ndim() == 2 && table->shape()[1] == H)) && (!qn || (qn->size() == B && qn->dtype() == cgt_i4)) &&
@@ -54,7 +58,7 @@ def _call(name, before, after):
     both = []
     for form, position in (("_at", "(const int*)qo->data()"), ("", "cl->q_offset")):
         both.append("cgt_amd_rel_attention" + form + "_" + name + "_f32(" + before + r""", B, H, Tq, Tk, D, cl->layout, table ? table->shape()[0] : 0,
-                    cl->bidirectional, cl->max_distance, cl->scale, cl->causal, """ + position + r""", qn ? (const int*)qn->data() : NULL,
+                    cl->bidirectional, cl->max_distance, scale, cl->causal, """ + position + r""", qn ? (const int*)qn->data() : NULL,
                     kn ? (const int*)kn->data() : NULL, cl->p, rng ? (const long long*)rng->data() : NULL, (unsigned)cl->channel,
                     """ + after + ", cgt_get_stream())")
     return "qo ? " + both[0] + "\n                  : " + both[1]
@@ -126,7 +130,7 @@ class RelativeAttention(core.Op):
                                      "table ? (const float*)table->data() : NULL", "(float*)o->data(), (float*)lse->data()") + r""";
                 cgt_check(rc == CGT_AMD_OK, "RelativeAttention: %s", cgt_amd_last_error());
             }"""
-        return core.NativeCompileInfo(code, includes=["cgt_amd.h"], closure_triples=make_closure(self.info),
+        return core.NativeCompileInfo(code, includes=["math.h", "cgt_amd.h"], closure_triples=make_closure(self.info),
                                       gpu_deref_mask=(True,) * len(input_types))
 
 
@@ -164,7 +168,7 @@ class RelativeAttentionBackward(core.Op):
                                      "(float*)gq->data(), (float*)gk->data(), (float*)gv->data(), gtable ? (float*)gtable->data() : NULL") + r""";
                 cgt_check(rc == CGT_AMD_OK, "RelativeAttentionBackward: %s", cgt_amd_last_error());
             }"""
-        return core.NativeCompileInfo(code, includes=["cgt_amd.h"], closure_triples=make_closure(self.info),
+        return core.NativeCompileInfo(code, includes=["math.h", "cgt_amd.h"], closure_triples=make_closure(self.info),
                                       gpu_deref_mask=(True,) * len(input_types))
 
 
@@ -197,9 +201,16 @@ def relative_attention(q, k, v, table=None, scale=None, causal=False, bidirectio
     if not 0 <= int(channel) < 1 << 32:
         raise ValueError("channel must be a whole number of 32 bits (got %s)" % (channel,))
     each = not isinstance(q_offset, (int, np.integer))
-    info = AttentionInfo(float(int(q.shape[3]) ** -0.5 if scale is None else scale), int(bool(causal)),
+    info = AttentionInfo(float(0.0 if scale is None else scale), int(bool(causal)),
                          int(bool(not causal if bidirectional is None else bidirectional)), int(max_distance), 0 if each else int(q_offset), p, int(channel),
-                         int(layout == "bthd"), int(table is not None), int(q_lengths is not None), int(k_lengths is not None), int(each))
+                         int(layout == "bthd"), int(table is not None), int(q_lengths is not None), int(k_lengths is not None), int(each),
+                         int(scale is None))
     inputs = [q, k, v] + ([core.as_node(table)] if table is not None else [])
     inputs += [_lengths_node(n) for n in (q_lengths, k_lengths, q_offset if each else None) if n is not None] + ([rng_node(rng)] if p else [])
-    return core.Result(RelativeAttention(info), inputs)[0]
+    result = core.Result(RelativeAttention(info), inputs)
+    # numbers that were computed from extents (q_offset = Tk - Tq) tie a compiled function to the shapes it was traced with
+    for n in (max_distance,) if each else (q_offset, max_distance):
+        if isinstance(n, core.ShapeInt) and not n.is_constant():
+            result.baked_expr = ("+", result.baked_expr, n.expr) if result.shape_baked else n.expr
+            result.shape_baked = True
+    return result[0]

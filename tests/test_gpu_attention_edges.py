@@ -175,6 +175,30 @@ def test_one_compiled_function_steps_through_a_cache(K, use_graph):
         nn.relative_attention(nq, nk, nv, q_offset=np.zeros(B, np.float32))
 
 
+def test_compiled_functions_follow_the_shapes_they_are_given(K):
+    import cgt_amd as cgt
+    from cgt_amd import nn
+    rs = np.random.RandomState(22)
+    draw = lambda *s: rs.randn(*s).astype(np.float32)      # noqa: E731
+    nq, nk, nv, ngo = (cgt.constant(draw(1, 2, t, 16)) for t in (7, 20, 20, 7))
+    o = nn.relative_attention(nq, nk, nv)
+    f = cgt.function([nq, nk, nv, ngo], [o] + cgt.grad(cgt.sum(o * ngo), [nq, nk, nv]))
+    for B, Tq, Tk, D in ((1, 7, 20, 16), (2, 5, 33, 64), (1, 9, 11, 20)):      # the scale is that of the head width at hand
+        q, k, v, go = draw(B, 2, Tq, D), draw(B, 2, Tk, D), draw(B, 2, Tk, D), draw(B, 2, Tq, D)
+        att = T.Attention(q, k, v)
+        tol = tolerances(att, go)
+        for name, a, want in zip(("o", "gq", "gk", "gv"), f(q, k, v, go), (att.o,) + att.pullback(go)[:3]):
+            close(a, want, tol[name], name)
+    # an offset computed from extents is a constant of the op: other shapes are refused, not answered with the old offset
+    o = nn.relative_attention(nq, nk, nv, causal=True, q_offset=nk.shape[2] - nq.shape[2])
+    f = cgt.function([nq, nk, nv], [o])
+    q, k, v = nq.get(), nk.get(), nv.get()
+    att = T.Attention(q, k, v, causal=True, q_offset=13)
+    close(f(q, k, v)[0], att.o, tolerances(att)["o"], "o")
+    with pytest.raises(ValueError, match="compiled for"):
+        f(draw(1, 2, 7, 16), draw(1, 2, 30, 16), draw(1, 2, 30, 16))
+
+
 # ---------------------------------------------------------------- rows of very different size within one head
 
 def plain32(q, k, v, table, go, causal=False, max_distance=128, bidirectional=None, keep=1.0):
