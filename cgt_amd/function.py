@@ -254,6 +254,8 @@ class Function(object):
         for before, after in updates:
             if before.op is not None:
                 raise ValueError("the left-hand side of an update must be a leaf node (a parameter)")
+            if isinstance(before.value, GpuArray):
+                before.value.check_writeable()
             if after.op is None or isinstance(after.typ, core.TupleType):
                 raise ValueError("the right-hand side of an update must be the result of an op")
             if tuple(after.shape) != tuple(before.shape) or after.typ != before.typ:

@@ -53,9 +53,18 @@ class GpuArray(object):
         return self._buffer.ptr + self._offset
 
     @property
+    def writeable(self):
+        """False for a view of another library's read-only array: it is an input, never a result."""
+        return getattr(self._buffer, "writeable", True)
+
+    def check_writeable(self):
+        if not self.writeable:
+            raise ValueError("the array %r is another library's and read-only" % self)
+
+    @property
     def __cuda_array_interface__(self):
         """Lets another library view this array without a copy."""
-        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr, False), "strides": None, "version": 2}
+        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr, not self.writeable), "strides": None, "version": 2}
 
     def reshape(self, *shape):
         """Zero-copy view with a new shape (the reference's Reshape op is a view
@@ -68,6 +77,7 @@ class GpuArray(object):
         return GpuArray(shape, self.dtype, _buffer=self._buffer, _offset=self._offset)
 
     def set(self, host):
+        self.check_writeable()
         host = _contiguous(host, self.dtype)
         if host.shape != self.shape:
             raise ValueError("shape mismatch %s vs %s" % (host.shape, self.shape))
@@ -80,6 +90,7 @@ class GpuArray(object):
         return out
 
     def fill_u32(self, word, stream=None):
+        self.check_writeable()
         capi.check(capi.lib().cgt_amd_fill_u32(self.ptr, word, self.nbytes // 4, stream))
         return self
 
@@ -94,14 +105,15 @@ def empty(shape, dtype=np.float32):
 class _Borrowed(object):
     """Device memory that belongs to another library's array, kept alive by holding on to it."""
 
-    def __init__(self, ptr, nbytes, owner):
-        self.ptr, self.nbytes, self.owner = ptr, nbytes, owner
+    def __init__(self, ptr, nbytes, owner, writeable=True):
+        self.ptr, self.nbytes, self.owner, self.writeable = ptr, nbytes, owner, writeable
 
 
 def as_gpuarray(x):
     """Zero-copy view of another library's device array (anything with `__cuda_array_interface__`, e.g. a torch
     tensor on this GPU): contiguous, of a type device arrays have.  Calls made with it must be ordered with the
-    other library's work by the caller (the same stream, or synchronisation).  Both libraries have to share one HIP
+    other library's work by the caller (the same stream, or synchronisation).  A read-only array stays one: it is
+    refused where a result is to be written.  Both libraries have to share one HIP
     runtime: import torch before the first call into this package."""
     if isinstance(x, GpuArray):
         return x
@@ -122,7 +134,7 @@ def as_gpuarray(x):
     if ptr % dtype.itemsize:
         raise ValueError("the array is not aligned to its elements")
     nbytes = int(np.prod(shape, dtype=np.int64)) * dtype.itemsize if shape else dtype.itemsize
-    return GpuArray(shape, dtype, _buffer=_Borrowed(ptr, nbytes, x))
+    return GpuArray(shape, dtype, _buffer=_Borrowed(ptr, nbytes, x, writeable=not info["data"][1]))
 
 
 def _contiguous(host, dtype=None):

@@ -23,6 +23,7 @@ def _out(out, shape, dtype=np.float32):
         return empty(shape, dtype)
     if out.shape != tuple(shape) or out.dtype != np.dtype(dtype):
         raise ValueError("out has shape %s dtype %s, expected %s %s" % (out.shape, out.dtype, tuple(shape), dtype))
+    out.check_writeable()
     return out
 
 

@@ -18,3 +18,24 @@ def test_offsets_of_each_sequence_are_checked():
     assert lib.cgt_amd_rel_attention_at_fwd_f32(None, None, None, None, 1, 1, 4, 4, 8, *rest, None, None, None) == 1 and "offsets" in capi.last_error()
     assert lib.cgt_amd_rel_attention_at_bwd_f32(None, None, None, None, None, None, None, 1, 1, 4, 4, 8, *rest, None, None, None, None, None) == 1
     assert lib.cgt_amd_rel_attention_at_fwd_f32(None, None, None, None, 0, 1, 4, 4, 8, *rest, None, None, None) == 0
+
+
+def test_read_only_arrays_of_other_libraries_are_inputs_only():
+    import cgt_amd as cgt
+    from cgt_amd import core, gpuarray, kernels as K
+
+    class Foreign(object):
+        def __init__(self, read_only):
+            self.__cuda_array_interface__ = dict(shape=(4, 8), typestr="<f4", data=(4096, read_only), strides=None, version=2)
+    free, fixed = gpuarray.as_gpuarray(Foreign(False)), gpuarray.as_gpuarray(Foreign(True))
+    assert free.writeable and not fixed.writeable and not fixed.reshape(32).writeable and _fake((4,)).writeable
+    assert fixed.__cuda_array_interface__["data"] == (4096, True)
+    g, s = _fake((8,)), _fake((4,))
+    for refused in (lambda: K.layer_norm_fwd(free, g, g, out=(fixed, s, s)), lambda: K.layer_norm_fwd(fixed, g, g, out=(fixed.reshape(4, 8), s, s)),
+                    lambda: K.dropout(free, 0.5, _fake((2,), np.int64), out=fixed), lambda: K.mul22(free, _fake((8, 8)), out=fixed),
+                    lambda: fixed.set(np.zeros((4, 8), np.float32)), lambda: fixed.fill_u32(0)):
+        with pytest.raises(ValueError, match="read-only"):
+            refused()
+    param, new = core.constant(fixed), core.constant(free)
+    with pytest.raises(ValueError, match="read-only"):
+        cgt.function([], [new], updates=[(param, new)])
