@@ -477,23 +477,29 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_wide_weights_kernel(Nor
     }
 }
 
-// ggamma, gbeta = the partial rows added up: 32 columns per workgroup, 32 groups of rows.
+// ggamma, gbeta = the partial rows added up: 32 columns per workgroup and trip, 32 groups of rows.  (A grid holds less than
+// 2^32 threads, that is 2^26 columns: wider rows take several trips.)
+constexpr long kWeightsGrid = 1L << 20;
 __global__ __launch_bounds__(1024) void norm_weights_kernel(const float* __restrict__ partial, int parts, int cols,
                                                             float* __restrict__ ggamma, float* __restrict__ gbeta) {
     __shared__ float join[32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;      // c in [0, 2 * cols)
+    const int g = threadIdx.x >> 5;
     const long pitch = 2L * cols;
-    float s = 0.0f;
-    if (c < 2 * cols) {
+    for (long c0 = blockIdx.x * 32L; c0 < pitch; c0 += gridDim.x * 32L) {
+        const long c = c0 + (threadIdx.x & 31);      // in [0, 2 * cols)
+        float s = 0.0f;
+        if (c < pitch) {
 #pragma unroll 8
-        for (int p = g; p < parts; p += 32) s += partial[p * pitch + c];
-    }
-    join[g][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (g == 0 && c < 2 * cols) {
-        for (int o = 1; o < 32; ++o) s += join[o][threadIdx.x];
-        if (c < cols) ggamma[c] = s;
-        else gbeta[c - cols] = s;
+            for (int p = g; p < parts; p += 32) s += partial[p * pitch + c];
+        }
+        join[g][threadIdx.x & 31] = s;
+        __syncthreads();
+        if (g == 0 && c < pitch) {
+            for (int o = 1; o < 32; ++o) s += join[o][threadIdx.x];
+            if (c < cols) ggamma[c] = s;
+            else gbeta[c - cols] = s;
+        }
+        __syncthreads();
     }
 }
 
@@ -602,7 +608,7 @@ static int launch_norm_bwd(NormBwd a, float* ggamma, float* gbeta, void* stream)
         norm_bwd_wide_weights_kernel<<<dim3((unsigned)cdiv(a.cols, 64), (unsigned)parts), kNormThreads, 0, st>>>(a, rows_per);
     }
     CGT_LAUNCH_CHECK("layer norm backward");
-    norm_weights_kernel<<<dim3((unsigned)cdiv(2L * a.cols, 32)), 1024, 0, st>>>(a.partial, (int)parts, a.cols, ggamma, gbeta);
+    norm_weights_kernel<<<dim3((unsigned)std::min(cdiv(2L * a.cols, 32), kWeightsGrid)), 1024, 0, st>>>(a.partial, (int)parts, a.cols, ggamma, gbeta);
     CGT_LAUNCH_CHECK("layer norm weight gradient");
     return CGT_AMD_OK;
 }
