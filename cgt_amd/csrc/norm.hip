@@ -634,6 +634,7 @@ CGT_API int cgt_amd_layer_norm_fwd_f32(const float* x, long rows, long cols, con
                                        float* y, float* mean, float* rstd, void* stream) {
     if (int rc = check_rows("layer norm", rows, cols)) return rc;
     CGT_ARG_CHECK(eps >= 0.0, "layer norm: eps must not be negative (got %g)", eps);
+    CGT_ARG_CHECK(cols > 0 || rows == 0 || !(mean || rstd), "layer norm: rows of no columns have no statistics");
     if (rows == 0 || cols == 0) return CGT_AMD_OK;
     CGT_ARG_CHECK(x && gamma && beta && y, "layer norm: null pointer");
     NormFwd a = {};
@@ -679,6 +680,7 @@ CGT_API int cgt_amd_dropout_add_layer_norm_fwd_f32(const float* x, const float* 
     CGT_ARG_CHECK(eps >= 0.0, "dropout + add + layer norm: eps must not be negative (got %g)", eps);
     NormFwd a = {};
     if (!dropout_rate(p, "dropout + add + layer norm", &a.rate)) return CGT_AMD_ERR_ARG;
+    CGT_ARG_CHECK(cols > 0 || rows == 0 || !(mean || rstd), "dropout + add + layer norm: rows of no columns have no statistics");
     if (rows == 0 || cols == 0) return CGT_AMD_OK;
     CGT_ARG_CHECK(x && residual && gamma && beta && y && h, "dropout + add + layer norm: null pointer");
     CGT_ARG_CHECK(rng || a.rate.threshold == 0, "dropout + add + layer norm: dropout needs the generator's state");

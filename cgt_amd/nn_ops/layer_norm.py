@@ -18,6 +18,8 @@ def _check_operands(name, input_types, weights, same):
 
 def _check_shapes(name, x, weights, same):
     xs = core.shape(x)
+    if xs[-1] == 0 and all(n != 0 for n in xs[:-1]):
+        raise ValueError("%s: rows of no columns have no statistics (shape %s)" % (name, xs))
     for w in weights:
         if core.shape(w) != xs[-1:]:
             raise ValueError("%s: weights of shape %s do not fit rows of %d columns" % (name, core.shape(w), xs[-1]))

@@ -296,7 +296,7 @@ int cgt_amd_lrn_bwd_from_x_f32(const float *x, const float *top_diff, long N, lo
 
 /* mean[r] = sum_c x / cols, rstd[r] = 1 / sqrt(sum_c (x - mean)^2 / cols + eps),
  * y = gamma[c] * (x - mean) * rstd + beta[c].  mean / rstd (rows floats each,
- * the operands of the gradient) may be NULL. */
+ * the operands of the gradient) may be NULL, and are where rows have no columns. */
 int cgt_amd_layer_norm_fwd_f32(const float *x, long rows, long cols, const float *gamma,
                                const float *beta, double eps, float *y, float *mean, float *rstd,
                                void *stream);

@@ -1,4 +1,4 @@
-"""Refusals of attention's entry points and of views of other libraries' arrays; no call reaches a GPU."""
+"""Refusals of the transformer operators and of views of other libraries' arrays; no call reaches a GPU."""
 import numpy as np
 import pytest
 
@@ -39,3 +39,15 @@ def test_read_only_arrays_of_other_libraries_are_inputs_only():
     param, new = core.constant(fixed), core.constant(free)
     with pytest.raises(ValueError, match="read-only"):
         cgt.function([], [new], updates=[(param, new)])
+
+
+def test_rows_of_no_columns_have_no_statistics():
+    from cgt_amd import capi, kernels as K
+    x, g, s = _fake((5, 0)), _fake((0,)), _fake((5,))
+    with pytest.raises(capi.CgtAmdError, match="no columns"):
+        K.layer_norm_fwd(x, g, g, out=(x, s, s))
+    with pytest.raises(capi.CgtAmdError, match="no columns"):
+        K.dropout_add_layer_norm_fwd(x, x, g, g, out=(x, x, s, s))
+    none = _fake((0, 0))
+    assert K.layer_norm_fwd(none, g, g, out=(none, _fake((0,)), _fake((0,))))[0] is none
+    assert capi.lib().cgt_amd_layer_norm_fwd_f32(None, 5, 0, None, None, 1e-5, None, None, None, None) == 0
