@@ -26,7 +26,7 @@
 //   what multiplies such a tile in the sums over keys or queries (p v, ds k, p go, ds q) takes over the rows' factors, so that
 //     it is of the size of the terms that are added, and gets the power of two that its largest term needs: of the tile in
 //     the backward pass, of the terms met so far in the forward pass, where the others are cut with an absolute error
-//     of 2^-37 of the largest at most.
+//     of 2^-35 of the largest at most.
 // Nothing is read behind the lengths.  A NaN or infinity in a row of q makes that row NaN, one in a row of k or v that the
 // walk meets all of its head: a key that a causal mask hides has probability 0, and 0 * NaN is NaN.
 //
@@ -174,11 +174,14 @@ __device__ __forceinline__ v16f mul_step(v16f acc, const Frag& a, const Frag& b)
 }
 
 // What a tile's rows are scaled by: one power of two, or 0 and one for each row where the rows are mixed (rare: see
-// attn_scale_kernel).  Where they are not, a tile costs one load that all lanes share.
+// attn_scale_kernel).  Where they are not, a tile costs a scalar load.
 struct ScaleArray {
     const float *tiles, *rows, *weights;      // a head's; weights of rows (null: 1) that go into what undoes the scales of a mixed tile
 };
-__device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+// One of a tile's, by the scalar unit (nothing in the same kernel writes there).
+__device__ __forceinline__ float tile_scale(const float* tiles, int n) {
+    return reinterpret_cast<const __attribute__((address_space(4))) float*>(reinterpret_cast<uintptr_t>(tiles))[__builtin_amdgcn_readfirstlane(n)];
+}
 
 // A tile of 32 rows of DP columns, shared by the workgroup.  A thread loads four neighbouring rows of
 // DP / 32 columns (rows at or beyond `end` are zero and not read), scales them, cuts them into terms and
@@ -385,6 +388,7 @@ struct TileRows {
     bool mixed;
     __device__ __forceinline__ TileRows(float tile_scale, const float* factors)
         : at(factors), one(tile_scale != 0.0f ? reciprocal_power(tile_scale) : 1.0f), mixed(__builtin_expect(tile_scale == 0.0f, 0)) {}
+    __device__ __forceinline__ float exponent() const { return (float)__builtin_amdgcn_frexp_expf(one) - 1.0f; }      // of one
     // v, but for the factor `one`
     __device__ __forceinline__ void undo(v16f& v) const {
         if (__builtin_expect(mixed, 0)) {
@@ -682,20 +686,22 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
         group0 = ((unsigned long long)(w.b * a.H + w.h) * a.Tq + query) * ((a.Tk + 15) / 16) * 2 + (lane >> 5);
     }
     v16f acc[DP / 32] = {};
-    float ref = -INFINITY, l = 0.0f;      // the exponentials are 2^(s - ref)
-    float e = 0.0f;                       // acc is the sum of p v times e; 0 while there was nothing to add
-    const auto rescale = [&](float f) {
+    float ref = -INFINITY, from = 0.0f, l = 0.0f;      // the exponentials are 2^(s - from); from = ref once a key was seen
+    float e = -INFINITY, limit = INFINITY;             // acc is the sum of p v times 2^e, -inf while there was nothing to add
+    const auto rescale = [&](float f) __attribute__((always_inline)) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] *= f;
     };
-    // e for terms p v of this size: the first to [2^12, 2^13), lowered where one outgrows that (as seldom)
-    const auto outgrows = [&](float largest) { return largest * e > 0x1p15f || (e == 0.0f && largest > 0.0f); };
-    const auto settle = [&](float largest) {
-        const float to = outgrows(largest) ? 0.25f * power_scale(largest) : e;
-        rescale(e == 0.0f ? 0.0f : to * reciprocal_power(e));
-        e = to;
+    // Settles e for terms p v of this size: the first to [2^10, 2^11), lowered where one outgrows 2^15 (as seldom); returns
+    // what acc has to be multiplied by.
+    const auto settle = [&](float largest) __attribute__((always_inline)) {
+        const bool unset = e == -INFINITY, change = unset ? largest > 0.0f : ldexpf(largest, (int)e) > 0x1p15f;
+        const int to = (int)min(268u - (__float_as_uint(largest) >> 23 & 255u), 253u) - 131;
+        const float f = !change ? 1.0f : unset ? 0.0f : ldexpf(1.0f, to - (int)e);
+        e = change ? (float)to : e;
+        return f;
     };
     const typename Tile<DP>::Offsets off(a.k_t, a.D);
     Tile<DP> kr, vr;
@@ -703,11 +709,11 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     if (first < last) {
         kr.load(off, kbase, a.k_t, first, last, a.D);
         vr.load(off, vbase, a.k_t, first, last, a.D);
-        knext = kscales.tiles[first / kAttnRows];
-        vnext = vscales.tiles[first / kAttnRows];
+        knext = tile_scale(kscales.tiles, first / kAttnRows);
+        vnext = tile_scale(vscales.tiles, first / kAttnRows);
     }
     for (int j0 = first; j0 < last; j0 += kAttnRows) {
-        const float kscale = uniform(knext), vscale = uniform(vnext);
+        const float kscale = knext, vscale = vnext;
         __syncthreads();
         kr.template store<true, false>(kt, nullptr, kscale, kscales, krows, j0, last);
         vr.template store<false, true>(nullptr, vt, vscale, vscales, vrows, j0, last);
@@ -715,8 +721,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
         if (j0 + kAttnRows < last) {
             kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
             vr.load(off, vbase, a.k_t, j0 + kAttnRows, last, a.D);
-            knext = kscales.tiles[j0 / kAttnRows + 1];
-            vnext = vscales.tiles[j0 / kAttnRows + 1];
+            knext = tile_scale(kscales.tiles, j0 / kAttnRows + 1);
+            vnext = tile_scale(vscales.tiles, j0 / kAttnRows + 1);
         }
         if (qw >= q_end || (a.causal && j0 > qw + 31 + q_offset)) continue;      // nothing here for this wavefront
         const int rel0 = j0 - qw - q_offset;
@@ -733,24 +739,26 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
         top = fmaxf(top, other_half(top));
-        // The reference, a whole number, follows the running maximum only where that is 2^7 above it: the exponentials stay
-        // below 2^7, and the results so far are seldom rescaled.  The same for the scale of the terms p v, known from the
-        // maximum where the tile has one factor.
-        const bool rise = top > ref + 7.0f;
-        const float to = rise ? ceilf(top) : ref, from = to == -INFINITY ? 0.0f : to;      // (0: a row that has seen nothing yet)
-        const float largest = value_rows.mixed ? 0.0f : pow2(top - from) * value_rows.one;
-        if (__any(rise || outgrows(largest))) {
-            const float f = to == -INFINITY ? 0.0f : pow2(ref - to);
+        // What keeps the exponentials and the terms p v in range changes seldom, and one test finds that it must: the reference, a
+        // whole number, follows the running maximum where that is 2^7 above it; the terms' scale is lowered where one outgrows
+        // it.  In a tile with one factor the scale goes into the exponent and comes out of the sum (lift), unless the sum would
+        // lose by it or the difference of the two is not exact: such tiles, and mixed ones, are scaled apart.
+        const float one = value_rows.exponent();
+        float lift = e + one;
+        bool apart = false;
+        if (value_rows.mixed || __any((top > ref + 7.0f) | (top + one > limit) | !(fabsf(lift) <= 40.0f))) {
+            const float to = top > ref + 7.0f ? ceilf(top) : ref;
+            float f = to == -INFINITY ? 0.0f : pow2(ref - to);
             ref = to;
+            from = ref == -INFINITY ? 0.0f : ref;
             l *= f;
+            if (!value_rows.mixed) f *= settle(pow2(top - from) * value_rows.one);
             rescale(f);
-            settle(largest);
+            lift = e == -INFINITY ? 0.0f : e + one;
+            apart = value_rows.mixed || __any((fabsf(lift) > 40.0f) | (fabsf(from) >= 0x1p22f));
+            if (apart) lift = 0.0f;
+            limit = fabsf(from) < 0x1p22f ? from + 15.0f - e : -INFINITY;
         }
-        // A tile with one factor: the terms' scale goes into the exponent, and comes out of the sum.  (Not where the sum would
-        // lose by it, nor where the difference of the two is no longer exact.)
-        float lift = value_rows.mixed || e == 0.0f ? 0.0f : (float)(__builtin_amdgcn_frexp_expf(e) + __builtin_amdgcn_frexp_expf(value_rows.one) - 2);
-        const bool apart = value_rows.mixed || __any(!(fabsf(lift) <= 40.0f && fabsf(from) < 0x1p22f));
-        if (__builtin_expect(apart, 0)) lift = 0.0f;
         const float lifted = from - lift;
         float part_l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -758,22 +766,23 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
             s[r] = pow2(s[r] - lifted);
             part_l[r & 3] += s[r];
         }
-        l = __builtin_fmaf((part_l[0] + part_l[1]) + (part_l[2] + part_l[3]), pow2(-lift), l);
+        l += ldexpf((part_l[0] + part_l[1]) + (part_l[2] + part_l[3]), -(int)lift);
+        asm volatile("" : "+v"(l));      // summed here: the branch below would otherwise take a copy of all terms along
         if (DROP) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 unsigned u[4];
                 random_group(rng, group0 + 2ull * (j0 / 16 + b), u);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s[8 * b + e] = random16(u, e) >= a.rate.threshold ? s[8 * b + e] : 0.0f;      // scaled at the end
+                for (int i = 0; i < 8; ++i) s[8 * b + i] = random16(u, i) >= a.rate.threshold ? s[8 * b + i] : 0.0f;      // scaled at the end
             }
         }
         if (__builtin_expect(apart, 0)) {
             value_rows.undo(s);
-            const float found = magnitude(s) * value_rows.one;
-            if (__any(outgrows(found))) settle(found);
+            rescale(settle(magnitude(s) * value_rows.one));
+            if (fabsf(from) < 0x1p22f) limit = from + 15.0f - e;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = s[r] * value_rows.one * e;
+            for (int r = 0; r < 16; ++r) s[r] = ldexpf(s[r] * value_rows.one, (int)e);
         }
         Frag b[2];
         split16(b, s);
@@ -788,7 +797,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
     }
     if (query >= a.Tq) return;
     l += other_half(l);
-    const float back = reciprocal_power(e);
+    const float back = e == -INFINITY ? 1.0f : ldexpf(1.0f, -(int)e);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -1064,11 +1073,11 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
     if (first < last) {
         kr.load(off, kbase, a.k_t, first, last, a.D);
         vr.load(off, vbase, a.k_t, first, last, a.D);
-        knext = kscales.tiles[first / kAttnRows];
-        vnext = vscales.tiles[first / kAttnRows];
+        knext = tile_scale(kscales.tiles, first / kAttnRows);
+        vnext = tile_scale(vscales.tiles, first / kAttnRows);
     }
     for (int j0 = first; j0 < last; j0 += kAttnRows) {
-        const float kscale = uniform(knext), vscale = uniform(vnext);
+        const float kscale = knext, vscale = vnext;
         __syncthreads();
         kr.template store<true, true>(kt, kc, kscale, kscales, krows, j0, last);
         vr.template store<true, false>(vt, nullptr, vscale, vscales, vrows, j0, last);
@@ -1076,8 +1085,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_ke
         if (j0 + kAttnRows < last) {
             kr.load(off, kbase, a.k_t, j0 + kAttnRows, last, a.D);
             vr.load(off, vbase, a.k_t, j0 + kAttnRows, last, a.D);
-            knext = kscales.tiles[j0 / kAttnRows + 1];
-            vnext = vscales.tiles[j0 / kAttnRows + 1];
+            knext = tile_scale(kscales.tiles, j0 / kAttnRows + 1);
+            vnext = tile_scale(vscales.tiles, j0 / kAttnRows + 1);
         }
         const int rel0 = j0 - qw - q_offset;
         const bool edge = j0 + kAttnRows > k_end || (a.causal && j0 + kAttnRows - 1 > qw + q_offset);
@@ -1246,11 +1255,11 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
     if (first < last) {
         qr.load(off, qbase, a.q_t, first, last, a.D);
         gr.load(off, gbase, a.q_t, first, last, a.D);
-        qnext = qscales.tiles[first / kAttnRows];
-        gnext = gscales.tiles[first / kAttnRows];
+        qnext = tile_scale(qscales.tiles, first / kAttnRows);
+        gnext = tile_scale(gscales.tiles, first / kAttnRows);
     }
     for (int i0 = first; i0 < last; i0 += kAttnRows) {
-        const float qscale = uniform(qnext), gscale = uniform(gnext);
+        const float qscale = qnext, gscale = gnext;
         __syncthreads();
         qr.template store<true, true>(qt, qc, qscale, qscales, qrows, i0, last);
         gr.template store<true, true>(gt, gc, gscale, gscales, grows, i0, last);
@@ -1263,8 +1272,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_k
         if (i0 + kAttnRows < last) {
             qr.load(off, qbase, a.q_t, i0 + kAttnRows, last, a.D);
             gr.load(off, gbase, a.q_t, i0 + kAttnRows, last, a.D);
-            qnext = qscales.tiles[i0 / kAttnRows + 1];
-            gnext = gscales.tiles[i0 / kAttnRows + 1];
+            qnext = tile_scale(qscales.tiles, i0 / kAttnRows + 1);
+            gnext = tile_scale(gscales.tiles, i0 / kAttnRows + 1);
         }
         const int rel0 = kw - i0 - q_offset;
         if (DROP) {

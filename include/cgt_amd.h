@@ -381,7 +381,7 @@ int cgt_amd_dropout_add_layer_norm_bwd_f32(const float *h, const float *gamma, c
  * Results have float32 accuracy row by row, whatever other rows hold: the error
  * of a score is some 2^-23 of sum |q_d k_d|, with an absolute floor of 2^-31 of
  * the products of the two rows' largest values, and sums over keys and queries
- * lose no term to larger ones (the forward pass: terms below 2^-37 of its
+ * lose no term to larger ones (the forward pass: terms below 2^-35 of its
  * largest).  Values below 2^-112, and products of go and v below 2^-97, lose
  * digits.  The backward pass forms its probabilities from lse, whose rounding
  * makes them wrong by 2^-23 |lse| relatively; a query whose |lse| is 2^22 or more
