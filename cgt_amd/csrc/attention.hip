@@ -649,8 +649,11 @@ __device__ __forceinline__ bool hidden(const Attn& a, int key, int query, int k_
 // ---------------------------------------------------------------- forward
 
 // o and lse of a block of 128 queries, or of a run of its keys.  8x16 heads of 1024, 64 columns, padded, 21.7 GFLOP of the
-// formulas' products: 134 us (and 13 for the scales), where one power of two a head, without regard to what its rows hold,
-// took 117.
+// formulas' products: 126 us (and 13 for the scales; one power of two a head, without regard to what its rows hold, took 117).
+// The matrix cores are 0.30 busy beside 10.5 other vector instructions a matrix instruction, about half the time together: a
+// tile's products and its softmax follow each other, with two barriers for each 32 keys, and three wavefronts a SIMD fill the
+// gaps in part (two take the same time).  With dropout of 0.1 139 us; 166 where every tile's rows of v are mixed, 185 with
+// those of k too.
 template <int DP, bool BIAS, bool DROP>
 __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kernel(Attn a, Scales scales, float* o, float* lse, float* part, float2* part_ml, int tiles, int splits) {
     extern __shared__ __align__(16) unsigned short lds[];
@@ -1005,8 +1008,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_token_kernel(Attn a, float*
 // ---------------------------------------------------------------- backward: queries
 
 // gq, the row products go . o (for the other kernel) and one partial row of the table's gradient.  Bound by the vector
-// instructions beside the matrix cores (8 a matrix instruction at 128 columns, 18 at 64 with dropout) and, at 128 columns, by one
+// instructions beside the matrix cores (10.5 a matrix instruction at 128 columns, 20 at 64 with dropout) and, at 128 columns, by one
 // wavefront a SIMD: its operands q and go (128 registers), gq (64) and the tiles on their way take more than half of the registers.
+// At 64 columns 4 registers (dropout; 14 without) go through scratch memory.  8x8 heads of 512, 64 columns, dropout, padded: 52 us; 2x8
+// heads of 2047, 128 columns, causal: 187 us, the matrix cores 0.20 busy.
 template <int DP, bool BIAS, bool DROP>
 __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_q_kernel(Attn a, Scales scales, const float* o, const float* lse, const float* go, float* gq,
     float* part, float* delta, float* part_table, int tiles, int splits) {
@@ -1208,8 +1213,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_table_kernel(const float* p
 // ---------------------------------------------------------------- backward: keys
 
 // gk and gv of a block of 128 keys.  Both sums stay in registers (128 of them at 128 columns) beside the columns of k and v
-// (another 128), hence one wavefront a SIMD there.  2x8 heads of 2047, 128 columns, causal: 194 us, the matrix cores 0.26 busy,
-// with 6 vector instructions a matrix instruction; 8x8 heads of 512, 64 columns, dropout, padded: 49 us.
+// (another 128), hence one wavefront a SIMD there.  2x8 heads of 2047, 128 columns, causal: 221 us, the matrix cores 0.23 busy,
+// with 10 vector instructions a matrix instruction, a third of them moves between the two register files; 8x8 heads of 512, 64
+// columns, dropout, padded: 49 us, with 16 registers through scratch memory (11 without dropout).
 template <int DP, bool BIAS, bool DROP>
 __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 1 : 2) void attn_bwd_kv_kernel(Attn a, Scales scales, const float* lse, const float* delta, const float* go, float* gk,
     float* gv, float* part, int tiles, int splits) {

@@ -1,5 +1,5 @@
 // Layer norm, dropout and the two in one pass (dropout + residual + layer norm), forward and
-// backward, for gfx950.  All are bound by HBM traffic: every array is read or written once.
+// backward, for gfx950.  All are bound by HBM traffic: up to 8192 columns every array is read or written once.
 //
 //   mean = sum_c x / C, rstd = 1 / sqrt(sum_c (x - mean)^2 / C + eps)      per row of C columns
 //   xhat = (x - mean) * rstd, y = gamma * xhat + beta
@@ -9,7 +9,8 @@
 //
 // A row is held in registers between its statistics and its result: one wavefront per row up to
 // 1024 columns, one workgroup of four up to 8192; beyond that a workgroup walks the row once per
-// statistic and once for the result (the later walks find it in cache).  The variance is the mean
+// statistic and once for the result, and in the backward pass once more for the weights (2048 x 16384: 85 us forward, 167
+// backward, at a copy's rate for one walk 43 and 65; 64 rows of 2^20 columns are 64 workgroups: 672 and 1112).  The variance is the mean
 // of the squared distances from the mean, not a difference of two sums, so rows far from zero
 // keep their digits.  A lane owns the same columns in every row it meets: gamma and beta are
 // loaded once, and the weights' gradients are summed over a workgroup's rows in registers, left
