@@ -200,7 +200,7 @@ def relative_attention(q, k, v, table=None, scale=None, causal=False, bidirectio
     p = resolved(p)
     if not 0 <= int(channel) < 1 << 32:
         raise ValueError("channel must be a whole number of 32 bits (got %s)" % (channel,))
-    each = not isinstance(q_offset, (int, np.integer))
+    each = isinstance(q_offset, (core.Node, core.GpuArray)) or np.ndim(q_offset) > 0
     info = AttentionInfo(float(0.0 if scale is None else scale), int(bool(causal)),
                          int(bool(not causal if bidirectional is None else bidirectional)), int(max_distance), 0 if each else int(q_offset), p, int(channel),
                          int(layout == "bthd"), int(table is not None), int(q_lengths is not None), int(k_lengths is not None), int(each),

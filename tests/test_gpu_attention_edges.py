@@ -161,6 +161,10 @@ def test_one_compiled_function_steps_through_a_cache(K, use_graph):
         q = rs.randn(B, H, 1, D).astype(np.float32)
         want = by_sequence(dict(c, k_lengths=list(n)), (q, k, v, table), n - 1)
         close(f(q, k, v, n, (n - 1).astype(np.int32))[0], want[0], want[2], "step %d" % step)
+    # whole numbers of any kind are one number
+    a = nn.relative_attention(nq, nk, nv, causal=True, q_offset=7)
+    for off in (np.int32(7), np.array(7), 7.0):
+        assert np.array_equal(nn.relative_attention(nq, nk, nv, causal=True, q_offset=off).get(), a.get())
     # gradients through the op with such an input
     go = rs.randn(B, H, 1, D).astype(np.float32)
     off = [7, 0, 299]
@@ -337,17 +341,22 @@ def test_rows_of_any_size_keep_float32_accuracy(K, name, D):
     assert np.all(np.abs(gtable.get() - want[3]).max(0) <= allowed)
 
 
-@pytest.mark.parametrize("Tq", [1, 5, 40])
-def test_forward_rows_of_any_size_against_long_keys(K, Tq):
-    # cut key axes and the join, at float32 accuracy
+@pytest.mark.parametrize("Tq,Tk", [(1, 6000), (5, 6000), (40, 6000), (6000, 40)])
+def test_rows_of_any_size_on_long_axes(K, Tq, Tk):
+    # cut axes and the sums of their pieces, at float32 accuracy
     rs = np.random.RandomState(Tq)
-    H, Tk, D = 2, 6000, 64
-    q, k, v = rs.randn(1, H, Tq, D), rs.randn(1, H, Tk, D), rs.randn(1, H, Tk, D)
+    H, D = 2, 64
+    q, k, v, go = (rs.randn(1, H, t, D) for t in (Tq, Tk, Tk, Tq))
     v[:, 1] *= spread(rs, Tk, 1e-5)
-    q, k, v = (a.astype(np.float32) for a in (q, k, v))
-    o, lse = K.rel_attention_fwd(dev(q), dev(k), dev(v))
+    go[:, 1] *= spread(rs, Tq, 1e-5)
+    q, k, v, go = (a.astype(np.float32) for a in (q, k, v, go))
+    ins = [dev(a) for a in (q, k, v)]
+    o, lse = K.rel_attention_fwd(*ins)
     att = T.Attention(q, k, v)
     att.scores = att.scale * np.matmul(att.q, att.k.transpose(0, 1, 3, 2))
-    zero = np.zeros_like(q)
-    rows_close(o.get(), att.o, plain32(q, k, v, None, zero)[0], units(att, zero.astype(np.float64))[0], "o")
+    plain, unit = plain32(q, k, v, None, go), units(att, go.astype(np.float64))
+    rows_close(o.get(), att.o, plain[0], unit[0], "o")
     assert np.abs(lse.get() - att.lse).max() <= 16 * U * np.abs(att.lse).max()
+    got = K.rel_attention_bwd(*ins, None, o, lse, dev(go))
+    for a, w, p32, u, n in zip(got, att.pullback(go), plain[1:], unit[1:], ("gq", "gk", "gv")):
+        rows_close(a.get(), w, p32, u, n)
