@@ -758,9 +758,9 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
             if (!value_rows.mixed) f *= settle(pow2(top - from) * value_rows.one);
             rescale(f);
             lift = e == -INFINITY ? 0.0f : e + one;
-            apart = value_rows.mixed || __any((fabsf(lift) > 40.0f) | (fabsf(from) >= 0x1p22f));
+            apart = value_rows.mixed || __any((fabsf(lift) > 40.0f) | (fabsf(from) >= 0x1p20f));
             if (apart) lift = 0.0f;
-            limit = fabsf(from) < 0x1p22f ? from + 15.0f - e : -INFINITY;
+            limit = fabsf(from) < 0x1p20f ? from + 15.0f - e : -INFINITY;
         }
         const float lifted = from - lift;
         float part_l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -783,7 +783,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 128 ? 2 : 3) void attn_fwd_kern
         if (__builtin_expect(apart, 0)) {
             value_rows.undo(s);
             rescale(settle(magnitude(s) * value_rows.one));
-            if (fabsf(from) < 0x1p22f) limit = from + 15.0f - e;
+            if (fabsf(from) < 0x1p20f) limit = from + 15.0f - e;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = ldexpf(s[r] * value_rows.one, (int)e);
         }

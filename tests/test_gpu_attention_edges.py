@@ -68,6 +68,19 @@ def test_gradients_of_rows_with_nothing_but_the_lowest_bias(K, Tq, Tk, p):
         close(a.get(), want, tol[name], name)
 
 
+@pytest.mark.parametrize("value", [-3e3, 7e5, -1.1e6, 2.9e6, -2.9e6, 1e8, -1e20])
+def test_results_stay_within_the_values_whatever_the_bias(K, value):
+    # scores whose whole digits leave no room for others: every probability is between 0 and 1, and they add up to 1
+    c = case(1, 2, 70, 300, 64, buckets=8, max_distance=16)
+    (q, k, v, table, go), _ = make(c)
+    table[:, 1] = value * (1 + np.arange(8) * 2.0 ** -20)
+    v = np.abs(v) + 1
+    o, lse = K.rel_attention_fwd(dev(q), dev(k), dev(v), dev(table), max_distance=16)
+    got = o.get()
+    assert np.isfinite(got).all() and np.all(got <= v.max(2, keepdims=True) * (1 + 1e-5)) and np.all(got >= v.min(2, keepdims=True) * (1 - 1e-5))
+    assert np.allclose(lse.get()[:, 1], value, rtol=1e-5, atol=20)
+
+
 @pytest.mark.parametrize("value", [-1e7, -1e9, -1e30, -2e38, 1e9])
 def test_rows_whose_lse_has_no_digits_contribute_to_no_gradient(K, value):
     # head 1 has such rows only, head 0 none
